@@ -442,6 +442,76 @@ int kcmm_decode_logits_bf16_on_stream(uint64_t hidden_ptr, uint64_t norm_w_ptr,
                                       uint32_t hidden_size, uint32_t vocab_size, float rms_eps,
                                       uint64_t stream_ptr);
 
+/* ---- 8-bit activations, and products with an epilogue --------------------- */
+/* No counterpart in the reference, whose projections are bf16 cuBLAS calls
+ * (ref runtime.rs:17-41).  The steps of a layer whose products read e4m3
+ * activations: a row as OCP e4m3fn codes with one fp32 scale, and products of
+ * such rows with e4m3 weights (one fp32 scale per weight row, as
+ * kcmm_gemm_fp8w_bf16_on_stream) on the fp8 matrix cores.  Everything between
+ * the inputs and the stores is fp32.  Enqueue only, on the calling thread's
+ * current device, to which the pointers and the stream belong; device
+ * addresses aligned to 16 bytes; every call may be captured into a HIP graph.
+ * An argument that a call does not take is refused with -1 and a line on
+ * stderr before any device work.
+ *
+ * Codes and scale of a row of values v: with a the largest |v| of the finite
+ * values, scale = max(a / 448, 2^-126), or 1 where a is 0, and code =
+ * e4m3(v / scale), the fp32 quotient to the nearest code, ties to even;
+ * +-infinity becomes the code of +-448, NaN a NaN code (and neither enters a).
+ * rows <= 2^20. */
+
+/** hidden = bf16(x + residual), codes and scales those of v = hidden /
+ *  sqrt(mean(hidden^2) + eps) * w; without a residual (residual_ptr and
+ *  hidden_ptr 0) those of x's norm.  All of x, residual, hidden, codes are
+ *  [rows][hidden_size], hidden_size % 8 == 0; hidden may be x or residual,
+ *  codes overlaps none of them.  Unlike kcmm_rmsnorm_bf16_on_stream nothing is
+ *  rounded between the norm and the codes. */
+int kcmm_add_rmsnorm_fp8_on_stream(uint64_t x_ptr, uint64_t residual_ptr, uint64_t w_ptr,
+                                   uint64_t hidden_ptr, uint64_t codes_ptr, uint64_t scales_ptr,
+                                   uint32_t rows, uint32_t hidden_size, float eps,
+                                   uint64_t stream_ptr);
+
+/** codes and scales of x's rows (bf16 [rows][cols], cols % 8 == 0). */
+int kcmm_quant_rows_fp8_on_stream(uint64_t x_ptr, uint64_t codes_ptr, uint64_t scales_ptr,
+                                  uint32_t rows, uint32_t cols, uint64_t stream_ptr);
+
+/** codes and scales ([rows][intermediate]) of v = silu(gate) * up, gate_up as
+ *  in kcmm_silu_mul_bf16_on_stream; intermediate % 8 == 0. */
+int kcmm_silu_mul_fp8_on_stream(uint64_t gate_up_ptr, uint64_t codes_ptr, uint64_t scales_ptr,
+                                uint32_t rows, uint32_t intermediate, uint64_t stream_ptr);
+
+/** Activations of a product's epilogue. */
+typedef enum {
+    KCMM_ACT_NONE = 0,
+    KCMM_ACT_RELU = 1,
+    KCMM_ACT_GELU = 2,      /* z Phi(z), Phi the normal distribution (erf) */
+    KCMM_ACT_GELU_TANH = 3, /* its tanh approximation */
+    KCMM_ACT_SILU = 4,
+} kcmm_activation_t;
+
+/** What a product does before its store.  A NULL epilogue is all zeros. */
+typedef struct kcmm_gemm_epilogue {
+    uint64_t bias;       /**< bf16 [n], or 0 */
+    uint64_t residual;   /**< bf16 [m][n], or 0; may be y itself */
+    int32_t activation;  /**< kcmm_activation_t */
+} kcmm_gemm_epilogue_t;
+
+/** y[m][n] = bf16(act(xscale[m] wscale[n] (x8[m][k] * w8[n][k]^T) + bias[n]) +
+ *  residual), rounded once.  k % 16 == 0 and k <= 2^24, any m and n; operands
+ *  below 4 GiB each, m * n < 2^31; y overlaps no operand but residual, where they are the
+ *  same buffer. */
+int kcmm_gemm_fp8_on_stream(uint64_t x8_ptr, uint64_t xscale_ptr, uint64_t w8_ptr,
+                            uint64_t wscale_ptr, uint64_t y_ptr,
+                            const kcmm_gemm_epilogue_t *epilogue, uint32_t m, uint32_t n,
+                            uint32_t k, uint64_t stream_ptr);
+
+/** The same with bf16 x and w and no scales; k % 8 == 0.  Unlike
+ *  kcmm_gemm_bf16_add_on_stream the product is not rounded before the
+ *  residual is added. */
+int kcmm_gemm_bf16_epi_on_stream(uint64_t x_ptr, uint64_t w_ptr, uint64_t y_ptr,
+                                 const kcmm_gemm_epilogue_t *epilogue, uint32_t m, uint32_t n,
+                                 uint32_t k, uint64_t stream_ptr);
+
 /** Device addresses of one layer's weights (bf16, row-major [out][in]). */
 typedef struct kcmm_layer_weights {
     uint64_t attn_norm; /**< [hidden] */

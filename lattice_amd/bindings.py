@@ -102,6 +102,16 @@ class KcmmLayerWeightsFp8(C.Structure):
                  "gate_up_scale", "down", "down_scale")]
 
 
+# kcmm_activation_t
+ACT_NONE, ACT_RELU, ACT_GELU, ACT_GELU_TANH, ACT_SILU = range(5)
+
+
+class KcmmGemmEpilogue(C.Structure):
+    """kcmm_gemm_epilogue_t (include/kcmm_mi355x.h): device addresses of a
+    product's bias and residual (0: none), and its activation."""
+    _fields_ = [("bias", C.c_uint64), ("residual", C.c_uint64), ("activation", C.c_int32)]
+
+
 _P, _U32, _U64, _I32 = C.c_void_p, C.c_uint32, C.c_uint64, C.c_int32
 _ATTN = [_P, _U32, _U64, _U64, _U64, _U64, _U64] + [_U32] * 6 + [C.c_float]
 
@@ -189,6 +199,13 @@ SIGNATURES = {
     "kcmm_gemm_bf16_add_on_stream": ([_U64, _U64, _U64, _U64, _U32, _U32, _U32, _U64], C.c_int),
     "kcmm_rmsnorm_bf16_on_stream": ([_U64, _U64, _U64, _U32, _U32, C.c_float, _U64], C.c_int),
     "kcmm_silu_mul_bf16_on_stream": ([_U64, _U64, _U32, _U32, _U64], C.c_int),
+    "kcmm_add_rmsnorm_fp8_on_stream": ([_U64] * 6 + [_U32, _U32, C.c_float, _U64], C.c_int),
+    "kcmm_quant_rows_fp8_on_stream": ([_U64, _U64, _U64, _U32, _U32, _U64], C.c_int),
+    "kcmm_silu_mul_fp8_on_stream": ([_U64, _U64, _U64, _U32, _U32, _U64], C.c_int),
+    "kcmm_gemm_fp8_on_stream": ([_U64] * 5 + [C.POINTER(KcmmGemmEpilogue), _U32, _U32, _U32, _U64],
+                                C.c_int),
+    "kcmm_gemm_bf16_epi_on_stream": ([_U64] * 3 + [C.POINTER(KcmmGemmEpilogue), _U32, _U32, _U32,
+                                                   _U64], C.c_int),
     "kcmm_embed_tokens_bf16_on_stream": ([_U64, _U64, _U64, _U32, _U32, _U32, _U64], C.c_int),
     "kcmm_gemm_bf16_swiglu_on_stream": ([_U64, _U64, _U64, _U32, _U32, _U32, _U64], C.c_int),
     "kcmm_decode_logits_bf16_on_stream": ([_U64, _U64, _U64, _U64, _U32, _U32, _U32, C.c_float,
@@ -316,6 +333,44 @@ class KcmmLibrary:
         if self.lib.kcmm_silu_mul_bf16_on_stream(gate_up_ptr, act_ptr, rows, intermediate,
                                                  stream_ptr) != 0:
             raise KcmmError("kcmm_silu_mul_bf16_on_stream failed")
+
+    def add_rmsnorm_fp8(self, x_ptr, residual_ptr, w_ptr, hidden_ptr, codes_ptr, scales_ptr, rows,
+                        hidden_size, eps, stream_ptr=0) -> None:
+        """hidden = x + residual; e4m3 codes and row scales of rmsnorm(hidden) (residual_ptr and
+        hidden_ptr 0: of rmsnorm(x))."""
+        if self.lib.kcmm_add_rmsnorm_fp8_on_stream(x_ptr, residual_ptr, w_ptr, hidden_ptr,
+                                                   codes_ptr, scales_ptr, rows, hidden_size,
+                                                   C.c_float(eps), stream_ptr) != 0:
+            raise KcmmError("kcmm_add_rmsnorm_fp8_on_stream failed")
+
+    def quant_rows_fp8(self, x_ptr, codes_ptr, scales_ptr, rows, cols, stream_ptr=0) -> None:
+        """e4m3 codes and row scales of bf16 rows."""
+        if self.lib.kcmm_quant_rows_fp8_on_stream(x_ptr, codes_ptr, scales_ptr, rows, cols,
+                                                  stream_ptr) != 0:
+            raise KcmmError("kcmm_quant_rows_fp8_on_stream failed")
+
+    def silu_mul_fp8(self, gate_up_ptr, codes_ptr, scales_ptr, rows, intermediate,
+                     stream_ptr=0) -> None:
+        """e4m3 codes and row scales of silu(gate) * up."""
+        if self.lib.kcmm_silu_mul_fp8_on_stream(gate_up_ptr, codes_ptr, scales_ptr, rows,
+                                                intermediate, stream_ptr) != 0:
+            raise KcmmError("kcmm_silu_mul_fp8_on_stream failed")
+
+    def gemm_fp8(self, x8_ptr, xscale_ptr, w8_ptr, wscale_ptr, y_ptr, m, n, k, *, bias_ptr=0,
+                 residual_ptr=0, activation=ACT_NONE, stream_ptr=0) -> None:
+        """y = act(xscale wscale (x8 w8^T) + bias) + residual (residual may be y)."""
+        epi = KcmmGemmEpilogue(bias_ptr, residual_ptr, activation)
+        if self.lib.kcmm_gemm_fp8_on_stream(x8_ptr, xscale_ptr, w8_ptr, wscale_ptr, y_ptr,
+                                            C.byref(epi), m, n, k, stream_ptr) != 0:
+            raise KcmmError("kcmm_gemm_fp8_on_stream failed")
+
+    def gemm_bf16_epi(self, x_ptr, w_ptr, y_ptr, m, n, k, *, bias_ptr=0, residual_ptr=0,
+                      activation=ACT_NONE, stream_ptr=0) -> None:
+        """y = act(x w^T + bias) + residual (residual may be y), rounded to bf16 once."""
+        epi = KcmmGemmEpilogue(bias_ptr, residual_ptr, activation)
+        if self.lib.kcmm_gemm_bf16_epi_on_stream(x_ptr, w_ptr, y_ptr, C.byref(epi), m, n, k,
+                                                 stream_ptr) != 0:
+            raise KcmmError("kcmm_gemm_bf16_epi_on_stream failed")
 
     def decode_logits_bf16(self, hidden_ptr, norm_w_ptr, lm_head_ptr, logits_ptr, batch,
                            hidden_size, vocab_size, eps, stream_ptr=0) -> None:

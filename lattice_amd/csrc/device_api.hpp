@@ -272,5 +272,30 @@ bool gemm_bf16_rope_append(uint64_t x, uint64_t w_qkv, uint32_t m, uint32_t k,
 bool gemm_bf16_swiglu(uint64_t x, uint64_t w_gate_up, uint64_t act, uint32_t m, uint32_t inter,
                       uint32_t k, uint64_t stream, std::string* err, uint64_t wscale = 0);
 
+// Rows as e4m3 codes with an fp32 scale per row (kernels/quant_rows.hip); cols
+// a multiple of 8, 1 <= rows <= 2^20.  residual and hidden: both or neither.
+bool add_rmsnorm_fp8(uint64_t x, uint64_t residual, uint64_t w, uint64_t hidden, uint64_t codes,
+                     uint64_t scales, uint32_t rows, uint32_t cols, float eps, uint64_t stream,
+                     std::string* err);
+bool quant_rows_fp8(uint64_t x, uint64_t codes, uint64_t scales, uint32_t rows, uint32_t cols,
+                    uint64_t stream, std::string* err);
+bool silu_mul_fp8(uint64_t gate_up, uint64_t codes, uint64_t scales, uint32_t rows, uint32_t inter,
+                  uint64_t stream, std::string* err);
+
+// Y = bf16(act(X W^T (* xscale * wscale) + bias) + residual) (kernels/gemm_epi.hip):
+// bf16 operands, or e4m3 codes where xscale (and wscale) are set.  Rows of both
+// operands are multiples of 16 bytes below 4 GiB in all; residual may be y.
+struct GemmEpiArgs {
+    uint64_t x, w, xscale, wscale, y, bias, residual;
+    int32_t act;
+    uint32_t m, n, k;
+    uint64_t stream;
+};
+bool gemm_epi(const GemmEpiArgs& a, std::string* err);
+
 }  // namespace dev
+
+// Activations of gemm_epi (kcmm_activation_t).
+constexpr int kActNone = 0, kActRelu = 1, kActGelu = 2, kActGeluTanh = 3, kActSilu = 4;
+
 }  // namespace kcmm

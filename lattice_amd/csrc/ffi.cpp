@@ -8,6 +8,8 @@
 #include <cstdio>
 #include <cstdlib>
 #include <cstring>
+#include <exception>
+#include <initializer_list>
 #include <memory>
 #include <mutex>
 #include <string>
@@ -1209,6 +1211,182 @@ int kcmm_silu_mul_bf16_on_stream(uint64_t gate_up, uint64_t act, uint32_t rows,
         return -1;
     }
     return 0;
+}
+
+// ---- 8-bit activations, and products with an epilogue ------------------------------------------
+
+extern "C++" {
+namespace {
+
+// A buffer of a call; address 0: not there.
+struct Span {
+    uint64_t at, bytes;
+};
+bool apart(const Span& a, const Span& b) {
+    return a.at == 0 || b.at == 0 || a.at + a.bytes <= b.at || b.at + b.bytes <= a.at;
+}
+bool same_or_apart(const Span& a, const Span& b) { return a.at == b.at || apart(a, b); }
+bool aligned16(std::initializer_list<uint64_t> ptrs) {
+    for (uint64_t p : ptrs)
+        if (p % 16 != 0) return false;
+    return true;
+}
+
+// What the body refuses or fails with goes to stderr, as this part of the ABI
+// has no pool to keep it; nothing is thrown across the C boundary.
+template <typename F>
+int call_without_pool(const char* fn, F&& body) {
+    try {
+        std::string err;
+        if (body(&err)) return 0;
+        std::fprintf(stderr, "%s: %s\n", fn, err.c_str());
+    } catch (const std::exception& e) {
+        std::fprintf(stderr, "%s: %s\n", fn, e.what());
+    }
+    return -1;
+}
+
+bool rows_ok(uint32_t rows, uint32_t cols, std::string* err) {
+    if (rows != 0 && rows <= (1u << 20) && cols != 0 && cols % 8 == 0 && cols <= (1u << 24)) return true;
+    *err = "needs 1 <= rows <= 2^20 and columns a positive multiple of 8 (<= 2^24)";
+    return false;
+}
+
+int gemm_epi_call(const char* fn, uint64_t x, uint64_t xscale, uint64_t w, uint64_t wscale,
+                  uint64_t y, const kcmm_gemm_epilogue_t* e, uint32_t m, uint32_t n, uint32_t k,
+                  uint64_t stream, bool fp8) {
+    return call_without_pool(fn, [&](std::string* err) {
+        const kcmm_gemm_epilogue_t epi = e != nullptr ? *e : kcmm_gemm_epilogue_t{};
+        if (x == 0 || w == 0 || y == 0 || (fp8 && (xscale == 0 || wscale == 0))) {
+            *err = "null pointer argument";
+            return false;
+        }
+        if (m == 0 || n == 0 || k == 0 || k % (fp8 ? 16 : 8) != 0 || k > (1u << 24)) {
+            *err = fp8 ? "needs m, n > 0 and k a positive multiple of 16, <= 2^24"
+                       : "needs m, n > 0 and k a positive multiple of 8, <= 2^24";
+            return false;
+        }
+        const uint64_t eb = fp8 ? 1 : 2, M = m, N = n, K = k;
+        if (M * K * eb >> 32 || N * K * eb >> 32 || M * N >> 31) {
+            *err = "operand too large (4 GiB each, m * n < 2^31)";
+            return false;
+        }
+        if (epi.activation < KCMM_ACT_NONE || epi.activation > KCMM_ACT_SILU) {
+            *err = "unknown activation " + std::to_string(epi.activation);
+            return false;
+        }
+        if (!aligned16({x, xscale, w, wscale, y, epi.bias, epi.residual})) {
+            *err = "pointers must be aligned to 16 bytes";
+            return false;
+        }
+        const Span out{y, 2 * M * N};
+        if (!apart(out, {x, M * K * eb}) || !apart(out, {w, N * K * eb}) ||
+            !apart(out, {xscale, 4 * M}) || !apart(out, {wscale, 4 * N}) ||
+            !apart(out, {epi.bias, 2 * N}) || !same_or_apart(out, {epi.residual, 2 * M * N})) {
+            *err = "y overlaps an operand";
+            return false;
+        }
+        kcmm::dev::GemmEpiArgs a{};
+        a.x = x;
+        a.w = w;
+        a.xscale = xscale;
+        a.wscale = wscale;
+        a.y = y;
+        a.bias = epi.bias;
+        a.residual = epi.residual;
+        a.act = epi.activation;
+        a.m = m;
+        a.n = n;
+        a.k = k;
+        a.stream = stream;
+        return kcmm::dev::gemm_epi(a, err);
+    });
+}
+
+}  // namespace
+}  // extern "C++"
+
+int kcmm_add_rmsnorm_fp8_on_stream(uint64_t x, uint64_t residual, uint64_t w, uint64_t hidden,
+                                   uint64_t codes, uint64_t scales, uint32_t rows,
+                                   uint32_t hidden_size, float eps, uint64_t stream) {
+    return call_without_pool("kcmm_add_rmsnorm_fp8_on_stream", [&](std::string* err) {
+        if (x == 0 || w == 0 || codes == 0 || scales == 0 || (residual == 0) != (hidden == 0)) {
+            *err = "null pointer argument (residual and hidden: both or neither)";
+            return false;
+        }
+        if (!rows_ok(rows, hidden_size, err)) return false;
+        if (!(eps >= 0.0f) || !(eps < HUGE_VALF)) {
+            *err = "eps must be finite and not negative";
+            return false;
+        }
+        if (!aligned16({x, residual, w, hidden, codes, scales})) {
+            *err = "pointers must be aligned to 16 bytes";
+            return false;
+        }
+        const uint64_t e = static_cast<uint64_t>(rows) * hidden_size;
+        const Span in{x, 2 * e}, res{residual, 2 * e}, wt{w, 2ull * hidden_size}, h{hidden, 2 * e},
+            c{codes, e}, s{scales, 4ull * rows};
+        if (!same_or_apart(h, in) || !same_or_apart(h, res) || !apart(h, wt) || !apart(c, in) ||
+            !apart(c, res) || !apart(c, wt) || !apart(c, h) || !apart(c, s) || !apart(s, in) ||
+            !apart(s, res) || !apart(s, wt) || !apart(s, h)) {
+            *err = "an output overlaps another buffer";
+            return false;
+        }
+        return kcmm::dev::add_rmsnorm_fp8(x, residual, w, hidden, codes, scales, rows, hidden_size,
+                                          eps, stream, err);
+    });
+}
+
+namespace {
+bool quant_args_ok(uint64_t x, uint64_t x_cols, uint64_t codes, uint64_t scales, uint32_t rows,
+                   uint32_t cols, std::string* err) {
+    if (x == 0 || codes == 0 || scales == 0) {
+        *err = "null pointer argument";
+        return false;
+    }
+    if (!rows_ok(rows, cols, err)) return false;
+    if (!aligned16({x, codes, scales})) {
+        *err = "pointers must be aligned to 16 bytes";
+        return false;
+    }
+    const Span in{x, 2 * rows * x_cols}, c{codes, static_cast<uint64_t>(rows) * cols},
+        s{scales, 4ull * rows};
+    if (!apart(c, in) || !apart(s, in) || !apart(s, c)) {
+        *err = "an output overlaps another buffer";
+        return false;
+    }
+    return true;
+}
+}  // namespace
+
+int kcmm_quant_rows_fp8_on_stream(uint64_t x, uint64_t codes, uint64_t scales, uint32_t rows,
+                                  uint32_t cols, uint64_t stream) {
+    return call_without_pool("kcmm_quant_rows_fp8_on_stream", [&](std::string* err) {
+        return quant_args_ok(x, cols, codes, scales, rows, cols, err) &&
+               kcmm::dev::quant_rows_fp8(x, codes, scales, rows, cols, stream, err);
+    });
+}
+
+int kcmm_silu_mul_fp8_on_stream(uint64_t gate_up, uint64_t codes, uint64_t scales, uint32_t rows,
+                                uint32_t intermediate, uint64_t stream) {
+    return call_without_pool("kcmm_silu_mul_fp8_on_stream", [&](std::string* err) {
+        return quant_args_ok(gate_up, 2ull * intermediate, codes, scales, rows, intermediate, err) &&
+               kcmm::dev::silu_mul_fp8(gate_up, codes, scales, rows, intermediate, stream, err);
+    });
+}
+
+int kcmm_gemm_fp8_on_stream(uint64_t x8, uint64_t xscale, uint64_t w8, uint64_t wscale, uint64_t y,
+                            const kcmm_gemm_epilogue_t* epilogue, uint32_t m, uint32_t n,
+                            uint32_t k, uint64_t stream) {
+    return gemm_epi_call("kcmm_gemm_fp8_on_stream", x8, xscale, w8, wscale, y, epilogue, m, n, k,
+                         stream, true);
+}
+
+int kcmm_gemm_bf16_epi_on_stream(uint64_t x, uint64_t w, uint64_t y,
+                                 const kcmm_gemm_epilogue_t* epilogue, uint32_t m, uint32_t n,
+                                 uint32_t k, uint64_t stream) {
+    return gemm_epi_call("kcmm_gemm_bf16_epi_on_stream", x, 0, w, 0, y, epilogue, m, n, k, stream,
+                         false);
 }
 
 namespace {

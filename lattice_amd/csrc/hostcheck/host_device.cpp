@@ -250,6 +250,17 @@ bool gemm_fp8w_bf16(uint64_t, uint64_t, uint64_t, uint64_t, uint32_t, uint32_t, 
                     std::string* err, uint64_t) {
     return no_device(err);
 }
+bool add_rmsnorm_fp8(uint64_t, uint64_t, uint64_t, uint64_t, uint64_t, uint64_t, uint32_t, uint32_t,
+                     float, uint64_t, std::string* err) {
+    return no_device(err);
+}
+bool quant_rows_fp8(uint64_t, uint64_t, uint64_t, uint32_t, uint32_t, uint64_t, std::string* err) {
+    return no_device(err);
+}
+bool silu_mul_fp8(uint64_t, uint64_t, uint64_t, uint32_t, uint32_t, uint64_t, std::string* err) {
+    return no_device(err);
+}
+bool gemm_epi(const GemmEpiArgs&, std::string* err) { return no_device(err); }
 bool gemm_split_reduce_launch(const float*, uint16_t*, const uint16_t*, int, int, uint64_t,
                               std::string* err) {
     return no_device(err);

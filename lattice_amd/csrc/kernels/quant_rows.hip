@@ -1,0 +1,310 @@
+// Rows as e4m3 codes with one fp32 scale per row, for products that read 8-bit
+// activations (gemm_epi.hip).  Three sources of a row's values v (fp32, never
+// rounded to bf16 on the way):
+//  * norm:  h = bf16(x + residual), or x; v = h / sqrt(mean(h^2) + eps) * w;
+//  * quant: v = x;
+//  * silu:  v = silu(gate) * up of the fused [gate | up] row.
+// Then a = max |v| over the finite v, scale = max(a / 448, 2^-126) (1 where a
+// is 0), code = e4m3(v / scale): nearest even of the fp32 quotient, infinities
+// at the largest code, NaN as NaN.  The scale keeps fp32, the codes are the
+// one rounding to fewer bits, relative 2^-4, that the 8-bit product is for.
+//
+// Bound by memory for many rows and by a launch and two dependent reductions
+// for few.  A row is read once: its values stay in registers between the sum,
+// the maximum and the codes.
+#include <algorithm>
+
+#include "../device_api.hpp"
+#include "common.hpp"
+#include "fp8_page.hpp"
+
+namespace kcmm {
+namespace {
+
+constexpr int kRowNorm = 0, kRowQuant = 1, kRowSilu = 2;
+
+struct RowParams {
+    const uint16_t* x;       // [rows][cols]; silu: [rows][2 cols], gate then up
+    const uint16_t* r;       // norm: residual [rows][cols] or null
+    const uint16_t* w;       // norm: [cols]
+    uint16_t* hidden;        // norm with residual: [rows][cols]
+    uint8_t* codes;          // [rows][cols]
+    float* scales;           // [rows]
+    int rows, cols;
+    float eps;
+};
+
+__device__ __forceinline__ void widen8(const u32x4& v, float (&f)[8]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        f[2 * i] = __uint_as_float(v[i] << 16);
+        f[2 * i + 1] = __uint_as_float(v[i] & 0xffff0000u);
+    }
+}
+
+// The row's values before the norm's factor: piece `i` (8 columns) of row
+// `row`.  norm: stores the hidden piece where there is a residual.
+template <int MODE>
+__device__ __forceinline__ void row_piece(const RowParams& p, size_t row, int i, float (&v)[8]) {
+    if constexpr (MODE == kRowSilu) {
+        const uint16_t* g = p.x + row * 2 * p.cols + i * 8;
+        float u[8];
+        widen8(*reinterpret_cast<const u32x4*>(g), v);
+        widen8(*reinterpret_cast<const u32x4*>(g + p.cols), u);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = v[e] / (1.0f + __expf(-v[e])) * u[e];
+    } else {
+        const size_t at = row * p.cols + i * 8;
+        widen8(*reinterpret_cast<const u32x4*>(p.x + at), v);
+        if constexpr (MODE == kRowNorm) {
+            if (p.r == nullptr) return;
+            float r[8];
+            widen8(*reinterpret_cast<const u32x4*>(p.r + at), r);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] += r[e];
+            const u32x4 h = pack_bf16x8(v);
+            *reinterpret_cast<u32x4*>(p.hidden + at) = h;
+            widen8(h, v);   // the norm is that of the stored row
+        }
+    }
+}
+
+__device__ __forceinline__ float finite_amax(const float (&v)[8], float a) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const float b = fabsf(v[e]);
+        a = fmaxf(a, b < __builtin_inff() ? b : 0.0f);
+    }
+    return a;
+}
+
+__device__ __forceinline__ float row_scale(float a) {
+    return a > 0.0f ? fmaxf(a / 448.0f, 0x1p-126f) : 1.0f;
+}
+
+// Eight values as codes; r = 1 / scale.
+__device__ __forceinline__ u32x2 row_codes(const float (&v)[8], float scale, float r) {
+    u32x2 o;
+    bool plain = scale >= kFp8QuotientMin && scale <= kFp8QuotientMax;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) plain &= fabsf(v[e]) < __builtin_inff();
+    if (__builtin_expect(plain, 1)) {
+        float q[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) q[e] = fp8_quotient(v[e], scale, r);
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
+            const int lo = __builtin_amdgcn_cvt_pk_fp8_f32(q[4 * w], q[4 * w + 1], 0, false);
+            o[w] = static_cast<uint32_t>(
+                __builtin_amdgcn_cvt_pk_fp8_f32(q[4 * w + 2], q[4 * w + 3], lo, true));
+        }
+        return o;
+    }
+#pragma unroll
+    for (int w = 0; w < 2; ++w) {
+        o[w] = 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[w] |= f32_to_fp8e4m3(v[4 * w + e] / scale) << (8 * e);
+    }
+    return o;
+}
+
+// Sum (or maximum) over a row's WPR waves, waves in order; `red` holds WPR
+// floats of this row.  A second use needs other floats.
+template <int WPR, bool MAX>
+__device__ __forceinline__ float row_reduce(float v, float* red, int wave) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) {
+        const float u = __shfl_xor(v, o);
+        v = MAX ? fmaxf(v, u) : v + u;
+    }
+    if constexpr (WPR == 1) return v;
+    if ((threadIdx.x & 63) == 0) red[wave] = v;
+    __syncthreads();
+    float s = red[0];
+#pragma unroll
+    for (int w = 1; w < WPR; ++w) s = MAX ? fmaxf(s, red[w]) : s + red[w];
+    return s;
+}
+
+// A row whose squares leave fp32 (a sum past 2^128, or one with eps under
+// 2^-100, where squares lose bits) is normed as 2^-80 or 2^80 times itself,
+// with eps times the square of that: the same v.  1 for any other row.
+__device__ __forceinline__ float norm_rescale(float ss, float eps) {
+    if (!(ss < __builtin_inff())) return 0x1p-80f;
+    return ss + eps < 0x1p-100f ? 0x1p80f : 1.0f;
+}
+
+// WPR waves a row, RPW rows a workgroup, at most P pieces of 8 columns a
+// lane (cols <= 512 * WPR * P).
+template <int MODE, int WPR, int P, int RPW>
+__global__ __launch_bounds__(64 * WPR * RPW) void quant_rows(RowParams p) {
+    static_assert(WPR == 1 || RPW == 1, "a barrier is all of one row's");
+    __shared__ float red[3][RPW][WPR];
+    const int slot = threadIdx.x / (64 * WPR), t = threadIdx.x % (64 * WPR), wave = t >> 6;
+    const bool live = blockIdx.x * RPW + slot < static_cast<unsigned>(p.rows);
+    const size_t row = live ? blockIdx.x * RPW + slot : 0;
+    const int n = live ? p.cols / 8 : 0;
+    float v[P][8];
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+        const int at = t + i * 64 * WPR;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[i][e] = 0.0f;
+        if (at < n) row_piece<MODE>(p, row, at, v[i]);
+    }
+    if constexpr (MODE == kRowNorm) {
+        float w[P][8], eps = p.eps;
+#pragma unroll
+        for (int i = 0; i < P; ++i) {
+            const int at = t + i * 64 * WPR;
+            widen8(*reinterpret_cast<const u32x4*>(p.w + (at < n ? at : 0) * 8), w[i]);
+        }
+        auto squares = [&](float* at) {
+            float ss = 0.0f;
+#pragma unroll
+            for (int i = 0; i < P; ++i)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) ss += v[i][e] * v[i][e];
+            return row_reduce<WPR, false>(ss, at, wave);
+        };
+        float ss = squares(red[0][slot]);
+        const float up = norm_rescale(ss, eps);
+        if (__builtin_expect(up != 1.0f, 0)) {   // the same for all of the row's threads
+#pragma unroll
+            for (int i = 0; i < P; ++i)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[i][e] *= up;
+            ss = squares(red[2][slot]);
+            eps = eps * up * up;
+        }
+        const float f = 1.0f / sqrtf(ss / static_cast<float>(p.cols) + eps);
+#pragma unroll
+        for (int i = 0; i < P; ++i)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[i][e] = v[i][e] * f * w[i][e];
+    }
+    float a = 0.0f;
+#pragma unroll
+    for (int i = 0; i < P; ++i)
+        if (t + i * 64 * WPR < n) a = finite_amax(v[i], a);
+    a = row_reduce<WPR, true>(a, red[1][slot], wave);
+    const float scale = row_scale(a), r = 1.0f / scale;
+    if (live && t == 0) p.scales[row] = scale;
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+        const int at = t + i * 64 * WPR;
+        if (at < n)
+            *reinterpret_cast<u32x2*>(p.codes + row * p.cols + at * 8) = row_codes(v[i], scale, r);
+    }
+}
+
+// Rows too long for the registers of 16 waves: each pass reads the row again
+// (from L2), the norm's from the hidden row where there is one.
+template <int MODE>
+__global__ __launch_bounds__(1024) void quant_long_rows(RowParams p) {
+    __shared__ float red[3][16];
+    const size_t row = blockIdx.x;
+    const int n = p.cols / 8, t = threadIdx.x, wave = t >> 6;
+    float f = 1.0f, up = 1.0f, a = 0.0f, v[8], w[8];
+    RowParams q = p;
+    if constexpr (MODE == kRowNorm) {
+        auto squares = [&](float* at) {
+            float ss = 0.0f;
+            for (int i = t; i < n; i += 1024) {
+                row_piece<MODE>(q, row, i, v);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) ss += v[e] * up * (v[e] * up);
+            }
+            if (p.r != nullptr) {   // from now on a thread reads what it wrote itself
+                q.x = p.hidden;
+                q.r = nullptr;
+            }
+            return row_reduce<16, false>(ss, at, wave);
+        };
+        float ss = squares(red[0]);
+        up = norm_rescale(ss, p.eps);
+        if (up != 1.0f) ss = squares(red[2]);
+        f = 1.0f / sqrtf(ss / static_cast<float>(p.cols) + p.eps * up * up);
+    }
+    auto value = [&](int i) {
+        row_piece<MODE>(q, row, i, v);
+        if constexpr (MODE == kRowNorm) {
+            widen8(*reinterpret_cast<const u32x4*>(p.w + i * 8), w);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = v[e] * up * f * w[e];
+        }
+    };
+    for (int i = t; i < n; i += 1024) {
+        value(i);
+        a = finite_amax(v, a);
+    }
+    a = row_reduce<16, true>(a, red[1], wave);
+    const float scale = row_scale(a), r = 1.0f / scale;
+    if (t == 0) p.scales[row] = scale;
+    for (int i = t; i < n; i += 1024) {
+        value(i);
+        *reinterpret_cast<u32x2*>(p.codes + row * p.cols + i * 8) = row_codes(v, scale, r);
+    }
+}
+
+template <int MODE, int WPR, int P>
+void launch_rows(const RowParams& p, hipStream_t s) {
+    constexpr int RPW = WPR == 1 ? 4 : 1;
+    hipLaunchKernelGGL((quant_rows<MODE, WPR, P, RPW>), dim3((p.rows + RPW - 1) / RPW),
+                       dim3(64 * WPR * RPW), 0, s, p);
+}
+
+template <int MODE>
+bool quant(const RowParams& p, uint64_t stream, std::string* err) {
+    hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+    const int n = p.cols / 8;   // pieces of a row
+    if (n <= 64) launch_rows<MODE, 1, 1>(p, s);
+    else if (n <= 128) launch_rows<MODE, 2, 1>(p, s);
+    else if (n <= 256) launch_rows<MODE, 4, 1>(p, s);
+    else if (n <= 512) launch_rows<MODE, 8, 1>(p, s);
+    else if (n <= 1024) launch_rows<MODE, 16, 1>(p, s);
+    else if (n <= 2048) launch_rows<MODE, 16, 2>(p, s);
+    else if (n <= 4096) launch_rows<MODE, 16, 4>(p, s);
+    else hipLaunchKernelGGL(quant_long_rows<MODE>, dim3(p.rows), dim3(1024), 0, s, p);
+    KCMM_HIP_CHECK(hipGetLastError(), err);
+    return true;
+}
+
+RowParams row_params(uint64_t x, uint64_t codes, uint64_t scales, uint32_t rows, uint32_t cols) {
+    RowParams p{};
+    p.x = reinterpret_cast<const uint16_t*>(x);
+    p.codes = reinterpret_cast<uint8_t*>(codes);
+    p.scales = reinterpret_cast<float*>(scales);
+    p.rows = static_cast<int>(rows);
+    p.cols = static_cast<int>(cols);
+    return p;
+}
+
+}  // namespace
+
+namespace dev {
+
+bool add_rmsnorm_fp8(uint64_t x, uint64_t residual, uint64_t w, uint64_t hidden, uint64_t codes,
+                     uint64_t scales, uint32_t rows, uint32_t cols, float eps, uint64_t stream,
+                     std::string* err) {
+    RowParams p = row_params(x, codes, scales, rows, cols);
+    p.r = reinterpret_cast<const uint16_t*>(residual);
+    p.w = reinterpret_cast<const uint16_t*>(w);
+    p.hidden = reinterpret_cast<uint16_t*>(hidden);
+    p.eps = eps;
+    return quant<kRowNorm>(p, stream, err);
+}
+
+bool quant_rows_fp8(uint64_t x, uint64_t codes, uint64_t scales, uint32_t rows, uint32_t cols,
+                    uint64_t stream, std::string* err) {
+    return quant<kRowQuant>(row_params(x, codes, scales, rows, cols), stream, err);
+}
+
+bool silu_mul_fp8(uint64_t gate_up, uint64_t codes, uint64_t scales, uint32_t rows, uint32_t inter,
+                  uint64_t stream, std::string* err) {
+    return quant<kRowSilu>(row_params(gate_up, codes, scales, rows, inter), stream, err);
+}
+
+}  // namespace dev
+}  // namespace kcmm
