@@ -48,6 +48,7 @@ HIP_SOURCES = ["kernels/backing.hip", "kernels/attn_decode.hip", "kernels/attn_p
                "kernels/page_copy.hip", "kernels/gemm.hip", "kernels/gemm_tiled.hip",
                "kernels/gemm_wide.hip",
                "kernels/glue.hip", "kernels/quant_rows.hip", "kernels/gemm_epi.hip",
+               "kernels/gemm_epi_wide.hip",
                "kernels/tier_copy.hip"]
 
 

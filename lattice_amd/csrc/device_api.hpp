@@ -32,6 +32,9 @@ enum class Tun {
     kGemmTile,      // KCMM_GEMM_TILE
     kGemmWaves,     // KCMM_GEMM_WAVES (waves per workgroup of unsplit plain / SwiGLU products)
     kGemmHelpers,   // KCMM_GEMM_HELPERS (0: split products without activation-staging helper waves)
+    kEpiKernel,     // KCMM_EPI_KERNEL (products with an epilogue: 1 the row kernel, 2 the wide
+                    // kernel, whatever the token count)
+    kEpiCfg,
     kCount
 };
 // true and *value = atoi(variable) when the variable is set.
