@@ -32,9 +32,8 @@ enum class Tun {
     kGemmTile,      // KCMM_GEMM_TILE
     kGemmWaves,     // KCMM_GEMM_WAVES (waves per workgroup of unsplit plain / SwiGLU products)
     kGemmHelpers,   // KCMM_GEMM_HELPERS (0: split products without activation-staging helper waves)
-    kEpiKernel,     // KCMM_EPI_KERNEL (products with an epilogue: 1 the row kernel, 2 the wide
-                    // kernel, whatever the token count)
-    kEpiCfg,
+    kEpiTile,       // KCMM_EPI_TILE (products with an epilogue: 1.. that tile of the tile
+                    // kernel with KCMM_GEMM_SPLITS K splits, 100 the 256-row tiles)
     kCount
 };
 // true and *value = atoi(variable) when the variable is set.
@@ -47,7 +46,8 @@ void reload_tunables();
 // attention segment table, 3: decode layer-step activations, 4: the final
 // norm's output, 5: prefill attention key splits, 6: tiering staging on
 // the null stream, 7: fp8 RoPE/append staging, 8: fp8 page-writer row
-// table, 9: counts of the prefill key splits).  `zero_fill` buffers start zeroed by a fill kernel, and their
+// table, 9: counts of the prefill key splits, 10: K splits of the products
+// with an epilogue).  `zero_fill` buffers start zeroed by a fill kernel, and their
 // users leave them zeroed.  Keyed by host thread as well, so a thread that
 // grows a buffer never frees one another thread has been handed.  Growth
 // synchronizes the stream and calls hipMalloc, so it cannot happen under

@@ -9,184 +9,329 @@
 // outputs' error against 64 bits stays that of the bf16 store (1.7e-3 of the
 // norm with and without), a 40th of the operands' own rounding to 2^-4.
 //
-// gemm_epi_rows: one workgroup of 8 waves on 16 NB weight rows x 16 MB tokens,
-// K split over its waves, the sums joined in LDS in wave order: no partials in
-// memory and no second launch, so a captured call needs no workspace.
-//  * both operands go from memory to registers in the layout of the matrix
-//    instructions: lane (row ln, group lg) takes 32 bytes at 32 lg of a
-//    128-byte line of its row.  The instructions sum over k in whatever order
-//    both operands have in common, so no operand is permuted;
-//  * stage s + 1 (U lines of each row a wave, whole lines) is in flight while
-//    stage s is consumed.
+// This file: the tile kernel, for up to a few hundred tokens, and the choice of
+// a tile; many tokens run the 256-row tiles of gemm_epi_wide.hip.  A product of
+// few tokens is bound by the weights' way from HBM, one of some tens by what a
+// CU can take in (a tile of R weight rows by T tokens loads R + T rows for R * T
+// outputs; about 23 bytes a cycle and CU were reached), so:
+//  * both operands reach LDS by direct loads, 128-byte lines of 8 rows an
+//    instruction, in a ring that keeps 64-128 KiB a CU in flight; fragments
+//    straight from memory to registers, 16 rows of 64 bytes an instruction,
+//    were slower wherever more than a token's row had to come with the weights
+//    (4096 x 14336, us, one / 16 / 64 tokens: 13.1 / 17.5 / 33.7 against 10.6 /
+//    12.4 / 21.3 from e4m3, 24.8 / 32.8 / 65.3 against 19.5 / 22.9 / 40.8 from bf16);
+//  * K is shared by the waves of a workgroup first (one wave each, no barrier
+//    until the sums are joined in LDS, in share order), by workgroups only where
+//    too few tiles would leave CUs idle for long (fp32 partials, summed by a
+//    second kernel in split order), and never under a capture, whose graph would
+//    keep the partials' address;
+//  * what the epilogue reads is loaded before the operands; outputs pass through
+//    LDS so that a thread stores 8 consecutive columns of a token, with
+//    unaligned vector stores where N is odd (226 x 7507 x 256: 8.9 -> 5.6 us).
+// The dot products sum over k in whatever order both operands have in common,
+// so a lane takes pieces lg and 4 + lg of a line for either operand.
 #include <algorithm>
+#include <cmath>
 #include <type_traits>
 
 #include "../device_api.hpp"
 #include "common.hpp"
 #include "gemm_epi.hpp"
+#include "wide_pipe.hpp"
 
 namespace kcmm {
 namespace {
 
-constexpr int kRowWaves = 8;
+// Waits until at most `left` (0 .. MOST) groups of LOADS loads are in flight.
+template <int LOADS, int MOST>
+__device__ __forceinline__ void wait_loads_in_flight(int left) {
+    if (left == MOST) {
+        wait_vm_lgkm0<LOADS * MOST>();
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_sched_barrier(0);
+    } else if constexpr (MOST > 0) {
+        wait_loads_in_flight<LOADS, MOST - 1>(left);
+    }
+}
 
-template <bool F8, int NB, int MB, int U, bool VEC>
-__global__ __launch_bounds__(64 * kRowWaves) void gemm_epi_rows(EpiParams p) {
-    __shared__ f32x4 red[kRowWaves][NB * MB][64];
+// The tile kernel: R = 16 NB WN weight rows by T = 16 MB WM tokens, its lines of
+// k dealt in turn to WK shares of WN x WM waves.  part: this K split's fp32
+// partials, `klines` lines a split.
+template <bool F8, int NB, int MB, int WN, int WM, int WK, int ST>
+__global__ __launch_bounds__(64 * WN * WM * WK) void gemm_epi_tile(EpiParams p, float* part, int klines) {
+    constexpr bool SHARED = WN * WM > 1;      // several waves read a place
+    constexpr int AHEAD = SHARED ? ST - 1 : ST;
+    constexpr int WL = 2 * NB / WM, XL = 2 * MB / WN;   // loads of 1 KiB a wave and line
+    static_assert(WL * WM == 2 * NB && XL * WN == 2 * MB, "loads divide over the waves");
+    constexpr int SHARE = (NB * WN + MB * WM) * 2048, PLACE = WK * SHARE;
+    constexpr int R = 16 * NB * WN, T = 16 * MB * WM, NT = 64 * WN * WM * WK;   // the tile, threads
+    constexpr int ROW = R + 4;                          // floats of a token's sums in LDS, padded
+    constexpr int RED = WK * T * ROW * 4, ITEMS = (R * T / 8 + NT - 1) / NT;
+    static_assert(RED <= 160 * 1024 && ST * PLACE <= 160 * 1024, "LDS");
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[ST * PLACE > RED ? ST * PLACE : RED];
     const int lane = threadIdx.x & 63, ln = lane & 15, lg = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int n0 = blockIdx.x * 16 * NB, m0 = blockIdx.y * 16 * MB;
-    const int lines = static_cast<int>((p.kb + 127) / 128);            // the last may be partial
-    const int full = static_cast<int>(p.kb / (128 * kRowWaves * U));   // stages of whole lines
+    const int wn = wave % WN, wm = wave / WN % WM, wk = wave / (WN * WM);
+    const int n0 = blockIdx.x * R, m0 = blockIdx.y * T;
+    const int all = static_cast<int>((p.kb + 127) / 128);
+    const int first = blockIdx.z * klines, lines = min(klines, all - first);
+    const int last = static_cast<int>(p.kb) - (all - 1) * 128;   // bytes of the row's last line
+    const int steps = SHARED ? (lines + WK - 1) / WK : (lines - wk + WK - 1) / WK;
 
-    // rows past the last are clamped; their outputs are not stored
-    const uint8_t* wr[NB];
-    const uint8_t* xr[MB];
+    const int lrow = lane >> 3, piece = (lane & 7) ^ lrow;
+    const uint32_t back = max(0, piece * 16 - (last - 16));
+    const int wload = (wn * WM + wm) * WL, xload = (wm * WN + wn) * XL;   // this wave's first loads
+    uint32_t wof[WL], xof[XL];
 #pragma unroll
-    for (int i = 0; i < NB; ++i) wr[i] = p.W + static_cast<size_t>(min(n0 + 16 * i + ln, p.N - 1)) * p.kb;
+    for (int i = 0; i < WL; ++i)
+        wof[i] = static_cast<uint32_t>(min(n0 + 8 * (wload + i) + lrow, p.N - 1)) * p.kb + piece * 16;
 #pragma unroll
-    for (int j = 0; j < MB; ++j) xr[j] = p.X + static_cast<size_t>(min(m0 + 16 * j + ln, p.M - 1)) * p.kb;
-
+    for (int i = 0; i < XL; ++i)
+        xof[i] = static_cast<uint32_t>(min(m0 + 8 * (xload + i) + lrow, p.M - 1)) * p.kb + piece * 16;
+    uint8_t* const share = lds + wk * SHARE;
+    int to = 0;   // the place that issue fills next
+    auto issue = [&](int i) {
+        const int line = first + min(i * WK + wk, lines - 1);
+        const uint32_t b = line + 1 == all ? back : 0;
+        const uint8_t* w = p.W + static_cast<size_t>(line) * 128;
+        const uint8_t* x = p.X + static_cast<size_t>(line) * 128;
+        uint8_t* dst = share + to * PLACE;
+#pragma unroll
+        for (int k = 0; k < WL; ++k) load_lds16_nt(w + (wof[k] - b), dst + (wload + k) * 1024);
+#pragma unroll
+        for (int k = 0; k < XL; ++k)
+            load_lds16(x + (xof[k] - b), dst + NB * WN * 2048 + (xload + k) * 1024);
+        to = to + 1 == ST ? 0 : to + 1;
+    };
     f32x4 acc[NB][MB];
 #pragma unroll
     for (int i = 0; i < NB; ++i)
 #pragma unroll
         for (int j = 0; j < MB; ++j) acc[i][j] = f32x4{0, 0, 0, 0};
 
-    struct Stage {
-        u32x4 a[U][NB][2], b[U][MB][2];
-    };
-    // Stage s < full: U consecutive lines of each wave.  Stage `full`: what is
-    // left, a line a wave in turn, addresses held inside the row.
-    auto load = [&](Stage& t, int s) {
-        uint32_t o[U][2];
+    const int sw[2] = {((0 + lg) ^ (ln & 7)) * 16, ((4 + lg) ^ (ln & 7)) * 16};
+    const bool cut[2] = {lg * 16 >= last, (4 + lg) * 16 >= last};
+    // output item q: 8 columns of a token, columns fastest; what its epilogue
+    // reads is on its way before the operands are
+    auto item_n = [&](int j) { return n0 + (static_cast<int>(threadIdx.x) + j * NT) % (R / 8) * 8; };
+    auto item_m = [&](int j) { return m0 + (static_cast<int>(threadIdx.x) + j * NT) / (R / 8); };
+    EpiCols cols[ITEMS];
+    EpiToken tokens[ITEMS];
 #pragma unroll
-        for (int u = 0; u < U; ++u)
+    for (int j = 0; j < ITEMS; ++j) {
+        cols[j] = epi_cols<F8>(p, part == nullptr ? item_n(j) : p.N);
+        tokens[j] = epi_token<F8>(p, part == nullptr ? item_m(j) : p.M, item_n(j));
+    }
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i)
+        if (i < steps) issue(i);
+    int at = 0;   // the place of step i
+    for (int i = 0; i < steps; ++i) {
+        wait_loads_in_flight<WL + XL, AHEAD - 1>(min(AHEAD - 1, steps - 1 - i));
+        if constexpr (SHARED) {
+            phase_barrier();   // all of step i is there, step i - 1 has been read
+            if (i + AHEAD < steps) issue(i + AHEAD);
+        }
+        const uint8_t* src = share + at * PLACE + ln * 128;
+        u32x4 a[NB][2], b[MB][2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+#pragma unroll
+            for (int k = 0; k < NB; ++k)
+                a[k][h] = *reinterpret_cast<const u32x4*>(src + (wn * NB + k) * 2048 + sw[h]);
+#pragma unroll
+            for (int k = 0; k < MB; ++k)
+                b[k][h] = *reinterpret_cast<const u32x4*>(src + (NB * WN + wm * MB + k) * 2048 + sw[h]);
+        }
+        wait_vm_lgkm0<63>();   // the operands are in registers: the place is free
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_sched_barrier(0);
+        if constexpr (!SHARED) {
+            if (i + AHEAD < steps) issue(i + AHEAD);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        at = at + 1 == ST ? 0 : at + 1;
+        const int line = i * WK + wk;
+        if (SHARED && WK > 1 && line >= lines) continue;
+        if (last < 128 && first + line + 1 == all) {   // the row's end: zeros behind it
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                if (s < full) o[u][h] = ((s * kRowWaves + wave) * U + u) * 128 + lg * 32 + h * 16;
-                else o[u][h] = min((full * kRowWaves * U + wave + kRowWaves * u) * 128 + lg * 32 + h * 16,
-                                   p.kb - 16);
+                if (!cut[h]) continue;
+#pragma unroll
+                for (int k = 0; k < NB; ++k) a[k][h] = u32x4{0, 0, 0, 0};
+#pragma unroll
+                for (int k = 0; k < MB; ++k) b[k][h] = u32x4{0, 0, 0, 0};
             }
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-#pragma unroll
-            for (int j = 0; j < MB; ++j)
-#pragma unroll
-                for (int h = 0; h < 2; ++h) t.b[u][j][h] = *reinterpret_cast<const u32x4*>(xr[j] + o[u][h]);
-#pragma unroll
-            for (int i = 0; i < NB; ++i)
-#pragma unroll
-                for (int h = 0; h < 2; ++h)
-                    t.a[u][i][h] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(wr[i] + o[u][h]));
         }
-    };
-    auto compute = [&](Stage& t, int s) {
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            if (s == full) {
-                const int line = full * kRowWaves * U + wave + kRowWaves * u;
-                if (line >= lines) continue;
-                if (line * 128 + 128 > static_cast<int>(p.kb)) {   // the row's end: zeros behind it
+        for (int k = 0; k < NB; ++k)
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        if (line * 128 + lg * 32 + h * 16 < static_cast<int>(p.kb)) continue;
-#pragma unroll
-                        for (int i = 0; i < NB; ++i) t.a[u][i][h] = u32x4{0, 0, 0, 0};
-#pragma unroll
-                        for (int j = 0; j < MB; ++j) t.b[u][j][h] = u32x4{0, 0, 0, 0};
-                    }
-                }
-            }
-#pragma unroll
-            for (int i = 0; i < NB; ++i)
-#pragma unroll
-                for (int j = 0; j < MB; ++j) acc[i][j] = mfma_line<F8>(t.a[u][i], t.b[u][j], acc[i][j]);
-        }
-    };
-    const int stages = full + (lines > full * kRowWaves * U);
-    Stage t0, t1;
-    load(t0, 0);
-    int s = 0;
-    for (; s + 2 < stages; s += 2) {
-        load(t1, s + 1);
-        compute(t0, s);
-        load(t0, s + 2);
-        compute(t1, s + 1);
+            for (int j = 0; j < MB; ++j) acc[k][j] = mfma_line<F8>(a[k], b[j], acc[k][j]);
     }
-    if (s + 1 < stages) {
-        load(t1, s + 1);
-        compute(t0, s);
-        compute(t1, s + 1);
-    } else {
-        compute(t0, s);
-    }
+    __syncthreads();   // every place is done with
+    float* const red = reinterpret_cast<float*>(lds);
 #pragma unroll
     for (int i = 0; i < NB; ++i)
 #pragma unroll
-        for (int j = 0; j < MB; ++j) red[wave][i * MB + j][lane] = acc[i][j];
+        for (int j = 0; j < MB; ++j)
+            *reinterpret_cast<f32x4*>(red + (wk * T + (wm * MB + j) * 16 + ln) * ROW + (wn * NB + i) * 16 +
+                                      4 * lg) = acc[i][j];
     __syncthreads();
-    // block b: weight rows 16 (b / MB) + 4 lg .. + 3, token 16 (b % MB) + ln
-    for (int b = wave; b < NB * MB; b += kRowWaves) {
-        f32x4 v = red[0][b][lane];
 #pragma unroll
-        for (int w = 1; w < kRowWaves; ++w) v += red[w][b][lane];
-        epi_store4<F8, VEC>(p, m0 + 16 * (b % MB) + ln, n0 + 16 * (b / MB) + 4 * lg, v);
+    for (int j = 0; j < ITEMS; ++j) {
+        const int q = static_cast<int>(threadIdx.x) + j * NT;
+        if (q >= R * T / 8) break;
+        float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll
+        for (int k = 0; k < WK; ++k) {
+            const f32x4* at = reinterpret_cast<const f32x4*>(red + (k * T + q / (R / 8)) * ROW + q % (R / 8) * 8);
+#pragma unroll
+            for (int r = 0; r < 8; ++r) v[r] += at[r >> 2][r & 3];
+        }
+        if (part == nullptr) epi_store<F8>(p, item_m(j), item_n(j), v, cols[j], tokens[j]);
+        else epi_store_part(p, part + static_cast<size_t>(blockIdx.z) * p.M * p.N, item_m(j), item_n(j), v);
     }
 }
 
-template <bool F8, int NB, int MB, int U>
-void launch_epi_rows(const EpiParams& p, hipStream_t s) {
-    const dim3 grid((p.N + 16 * NB - 1) / (16 * NB), (p.M + 16 * MB - 1) / (16 * MB));
-    if (p.N % 4 == 0)
-        hipLaunchKernelGGL((gemm_epi_rows<F8, NB, MB, U, true>), grid, dim3(64 * kRowWaves), 0, s, p);
-    else
-        hipLaunchKernelGGL((gemm_epi_rows<F8, NB, MB, U, false>), grid, dim3(64 * kRowWaves), 0, s, p);
-}
-
-// Many tokens: the 256-row tiles, K split where the stream has room for the
-// partials (never under a capture: a graph would keep their address).
-bool many_tokens(const EpiParams& p, uint64_t stream, std::string* err) {
-    dev::GemmWidePlan plan = dev::gemm_epi_wide_plan(p, 8);
-    void* part = nullptr;
-    if (plan.splits > 1) {
-        const size_t bytes = static_cast<size_t>(plan.splits) * p.M * p.N * sizeof(float);
-        if (!dev::stream_scratch(stream, 1, bytes)) plan = dev::gemm_epi_wide_plan(p, 1);
-        else if (!dev::stream_workspace(stream, 1, bytes, &part, false, err)) return false;
+// A tile and its modelled time in us: a workgroup alone takes f + g a step (a
+// line of each share), one among others on its CU e + l of that CU's time, the
+// weights come at h TB/s.
+// Fitted to timings of 2900 products (M 1 .. 4096, N 64 .. 32768, K 64 .. 14336,
+// either type): within 10% at the median, 30% for nine in ten; the tile chosen
+// by it is 2.4% slower than the best of all in the mean.
+struct Tile {
+    int nb, mb, wn, wm, wk, st;
+    float f, g, e, l, h;
+    constexpr int rows() const { return 16 * nb * wn; }
+    constexpr int tokens() const { return 16 * mb * wm; }
+    constexpr int waves() const { return wn * wm * wk; }
+    constexpr int lds() const {
+        const int ring = st * wk * (nb * wn + mb * wm) * 2048, sums = wk * tokens() * (rows() + 4) * 4;
+        return ring > sums ? ring : sums;
     }
-    return dev::gemm_epi_wide(p, plan, static_cast<float*>(part), stream, err);
+};
+constexpr Tile kTiles[] = {
+    {1, 1, 1, 1, 8, 2, 1.84f, 0.13f, 0.10f, 0.71f, 7.3f},   //  16 rows x  16 tokens
+    {2, 1, 1, 1, 8, 3, 0.38f, 1.17f, 2.01f, 0.01f, 5.3f},   //  32 x  16
+    {2, 1, 2, 1, 4, 3, 0.76f, 1.07f, 1.84f, 0.01f, 5.6f},   //  64 x  16
+    {1, 2, 1, 1, 8, 3, 1.35f, 0.71f, 0.03f, 1.07f, 8.0f},   //  16 x  32
+    {2, 2, 1, 1, 8, 2, 0.54f, 1.47f, 0.69f, 1.05f, 6.6f},   //  32 x  32
+    {1, 2, 4, 1, 2, 4, 1.53f, 0.51f, 0.34f, 0.59f, 8.0f},   //  64 x  32
+    {2, 2, 4, 1, 2, 3, 1.20f, 1.03f, 0.00f, 0.82f, 6.2f},   // 128 x  32
+    {2, 4, 1, 1, 4, 2, 1.32f, 0.82f, 0.29f, 1.04f, 8.0f},   //  32 x  64
+    {1, 4, 4, 1, 2, 4, 1.33f, 0.74f, 0.91f, 0.71f, 8.0f},   //  64 x  64
+    {1, 4, 8, 1, 1, 5, 1.96f, 0.54f, 1.24f, 0.57f, 8.0f},   // 128 x  64
+    {2, 4, 2, 2, 2, 3, 2.22f, 0.80f, 1.41f, 1.08f, 8.0f},   //  64 x 128
+    {1, 8, 8, 1, 1, 4, 3.98f, 0.38f, 2.53f, 0.84f, 8.0f},   // 128 x 128
+};
+constexpr int kTileCount = sizeof(kTiles) / sizeof(kTiles[0]);
+
+int div_up(int a, int b) { return (a + b - 1) / b; }
+
+double tile_us(const Tile& t, const EpiParams& p, int splits) {
+    const int lines = div_up(static_cast<int>(p.kb), 128), klines = div_up(lines, splits);
+    const double q = static_cast<double>(div_up(p.N, t.rows())) * div_up(p.M, t.tokens()) *
+                     div_up(lines, klines) / 256;
+    const int steps = div_up(klines, t.wk), held = std::min(160 * 1024 / t.lds(), 32 / t.waves());
+    const double alone = std::max(1.0, std::ceil(q / held)) * (t.f + steps * t.g);
+    const double loaded = (q <= 1 ? 1.0 : std::min(std::ceil(q), q + 0.5)) * (t.e + steps * t.l);
+    const double hbm = static_cast<double>(p.N) * p.kb / (t.h * 1e6);
+    auto p4 = [](double x) { return x * x * x * x; };
+    const double sum = splits > 1 ? 4.3 + 4e-6 * splits * p.M * p.N : 0.0;
+    return 1.7 + std::sqrt(std::sqrt(p4(alone) + p4(loaded) + p4(hbm))) + sum;
 }
 
-template <bool F8>
-bool gemm_epi_typed(const EpiParams& p, uint64_t stream, std::string* err) {
+struct Choice {
+    int tile = 0, splits = 1;
+    double us = 0.0;
+};
+
+// The tile and K splits of least modelled time.  Tiles at least twice as high
+// as M are left out, and those of a tenth of it (the model's data holds none of
+// either); splits only where the tiles do not fill the chip.
+Choice choose_tile(const EpiParams& p, bool may_split) {
+    Choice best;
+    best.us = -1.0;
+    for (int i = 0; i < kTileCount; ++i) {
+        const Tile& t = kTiles[i];
+        if (t.tokens() >= 2 * div_up(p.M, 16) * 16 ||
+            (t.tokens() * 10 < p.M && t.tokens() < 64)) continue;
+        const int wgs = div_up(p.N, t.rows()) * div_up(p.M, t.tokens());
+        for (int s : {1, 2, 3, 4, 6, 8}) {
+            if (s > 1 && (!may_split || wgs >= 256 || wgs * s > 520 ||
+                          div_up(static_cast<int>(p.kb), 128) / s < 2 * t.wk))
+                break;
+            const double us = tile_us(t, p, s);
+            if (best.us < 0 || us < best.us) best = Choice{i, s, us};
+        }
+    }
+    return best;
+}
+
+template <bool F8, int I>
+void launch_tile(const EpiParams& p, int splits, int klines, float* part, hipStream_t s) {
+    constexpr Tile t = kTiles[I];
+    const dim3 grid(div_up(p.N, t.rows()), div_up(p.M, t.tokens()), splits);
+    hipLaunchKernelGGL((gemm_epi_tile<F8, t.nb, t.mb, t.wn, t.wm, t.wk, t.st>), grid, dim3(64 * t.waves()), 0,
+                       s, p, part, klines);
+}
+
+template <bool F8, int... I>
+void launch_tile_at(int at, std::integer_sequence<int, I...>, const EpiParams& p, int splits, int klines,
+                    float* part, hipStream_t s) {
+    (void)((at == I && (launch_tile<F8, I>(p, splits, klines, part, s), true)) || ...);
+}
+
+bool run_tile(const EpiParams& p, const Choice& c, float* part, uint64_t stream, std::string* err) {
+    const int lines = div_up(static_cast<int>(p.kb), 128), klines = div_up(lines, c.splits);
+    const int splits = div_up(lines, klines);   // (none of them empty)
+    float* const to = splits > 1 ? part : nullptr;
     hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-    const int forced = dev::tunable_or(dev::Tun::kEpiKernel, 0);
-    if (forced == 2 || (forced == 0 && p.M > 64)) return many_tokens(p, stream, err);
-    const int cfg = dev::tunable_or(dev::Tun::kEpiCfg, 0);
-    switch (cfg) {
-        case 114: launch_epi_rows<F8, 1, 1, 4>(p, s); break;
-        case 112: launch_epi_rows<F8, 1, 1, 2>(p, s); break;
-        case 214: launch_epi_rows<F8, 2, 1, 4>(p, s); break;
-        case 212: launch_epi_rows<F8, 2, 1, 2>(p, s); break;
-        case 412: launch_epi_rows<F8, 4, 1, 2>(p, s); break;
-        case 411: launch_epi_rows<F8, 4, 1, 1>(p, s); break;
-        case 122: launch_epi_rows<F8, 1, 2, 2>(p, s); break;
-        case 124: launch_epi_rows<F8, 1, 2, 4>(p, s); break;
-        case 222: launch_epi_rows<F8, 2, 2, 2>(p, s); break;
-        case 221: launch_epi_rows<F8, 2, 2, 1>(p, s); break;
-        case 421: launch_epi_rows<F8, 4, 2, 1>(p, s); break;
-        case 141: launch_epi_rows<F8, 1, 4, 1>(p, s); break;
-        case 142: launch_epi_rows<F8, 1, 4, 2>(p, s); break;
-        case 241: launch_epi_rows<F8, 2, 4, 1>(p, s); break;
-        case 242: launch_epi_rows<F8, 2, 4, 2>(p, s); break;
-        case 441: launch_epi_rows<F8, 4, 4, 1>(p, s); break;
-        default:
-            if (p.M <= 16) launch_epi_rows<F8, 1, 1, 4>(p, s);
-            else if (p.M <= 32) launch_epi_rows<F8, 1, 2, 4>(p, s);
-            else launch_epi_rows<F8, 2, 4, 2>(p, s);
-    }
+    constexpr auto all = std::make_integer_sequence<int, kTileCount>{};
+    if (p.xs != nullptr) launch_tile_at<true>(c.tile, all, p, splits, klines, to, s);
+    else launch_tile_at<false>(c.tile, all, p, splits, klines, to, s);
     KCMM_HIP_CHECK(hipGetLastError(), err);
-    return true;
+    return splits == 1 || dev::gemm_epi_sum(p, to, splits, stream, err);
+}
+
+// fp32 partials of K splits on `stream`; null where they cannot be had, or
+// where a capture would keep their address.
+float* partials(const EpiParams& p, int splits, uint64_t stream) {
+    const size_t bytes = static_cast<size_t>(splits) * p.M * p.N * sizeof(float);
+    void* part = nullptr;
+    std::string why;
+    if (!dev::stream_scratch(stream, kEpiSlot, bytes) ||
+        !dev::stream_workspace(stream, kEpiSlot, bytes, &part, false, &why))
+        return nullptr;
+    return static_cast<float*>(part);
+}
+
+// Modelled time of the 256-row tiles, which no product of up to 96 tokens, and
+// none of a single line, of those timed needed.
+double wide_us(const dev::GemmWidePlan& plan) { return 2.0 + plan.us; }
+
+bool run_epi(const EpiParams& p, uint64_t stream, std::string* err) {
+    const int forced = dev::tunable_or(dev::Tun::kEpiTile, 0);   // (tests and tuning)
+    if (forced >= 1 && forced <= kTileCount) {
+        Choice c{forced - 1, std::max(1, std::min(16, dev::tunable_or(dev::Tun::kGemmSplits, 1))), 0.0};
+        float* part = c.splits > 1 ? partials(p, c.splits, stream) : nullptr;
+        if (part == nullptr) c.splits = 1;
+        return run_tile(p, c, part, stream, err);
+    }
+    float* part = nullptr;
+    for (int most : {8, 1}) {
+        dev::GemmWidePlan wide;
+        const bool many = forced == 100 || (p.M > 96 && p.kb > 128);
+        if (many) wide = dev::gemm_epi_wide_plan(p, most);
+        Choice tile;
+        if (forced != 100) tile = choose_tile(p, most > 1);
+        const bool take_wide = many && (forced == 100 || tile.us < 0 || wide_us(wide) < tile.us);
+        const int splits = take_wide ? wide.splits : tile.splits;
+        if (splits > 1 && (part = partials(p, splits, stream)) == nullptr) continue;   // without, then
+        if (take_wide) return dev::gemm_epi_wide(p, wide, part, stream, err);
+        return run_tile(p, tile, part, stream, err);
+    }
+    return false;
 }
 
 }  // namespace
@@ -205,9 +350,8 @@ bool gemm_epi(const GemmEpiArgs& a, std::string* err) {
     p.M = static_cast<int>(a.m);
     p.N = static_cast<int>(a.n);
     p.act = a.act;
-    const bool f8 = a.xscale != 0;
-    p.kb = a.k * (f8 ? 1 : 2);
-    return f8 ? gemm_epi_typed<true>(p, a.stream, err) : gemm_epi_typed<false>(p, a.stream, err);
+    p.kb = a.k * (a.xscale != 0 ? 1 : 2);
+    return run_epi(p, a.stream, err);
 }
 
 }  // namespace dev

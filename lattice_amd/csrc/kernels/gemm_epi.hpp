@@ -21,6 +21,8 @@ struct EpiParams {
 
 namespace {
 
+constexpr int kEpiSlot = 10;   // the stream workspace of their K splits
+
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 
 // erfc(a) e^(a^2) for a >= 0 as a polynomial in t = 1 / (1 + 0.3275911 a)
@@ -65,41 +67,110 @@ __device__ __forceinline__ void activate_all(float (&z)[R], int act) {
     }
 }
 
-// Outputs (m, n .. n + 3) from their sums.  VEC: N % 4 == 0.
-template <bool F8, bool VEC>
-__device__ __forceinline__ void epi_store4(const EpiParams& p, int m, int n, f32x4 v) {
-    if (m >= p.M || n >= p.N) return;
-    if constexpr (F8) v *= p.xs[m];
-    const size_t at = static_cast<size_t>(m) * p.N + n;
-    if constexpr (VEC) {
-        if constexpr (F8) v *= *reinterpret_cast<const f32x4*>(p.ws + n);
-        if (p.bias != nullptr) {
-            const u32x2 b = *reinterpret_cast<const u32x2*>(p.bias + n);
-            v += f32x4{__uint_as_float(b[0] << 16), __uint_as_float(b[0] & 0xffff0000u),
-                       __uint_as_float(b[1] << 16), __uint_as_float(b[1] & 0xffff0000u)};
-        }
+// Eight bf16 of a row of Y or R: rows start at any even address when N is odd,
+// and global memory takes vector accesses there.
+typedef uint32_t u32x4_rows __attribute__((ext_vector_type(4), aligned(2)));
+typedef float f32x4_rows __attribute__((ext_vector_type(4), aligned(4)));
+
+// What the epilogue of columns n .. n + 7 (n % 8 == 0) takes from memory, loaded
+// ahead of the sums: the columns' part, and the token's.
+struct EpiCols {
+    float ws[8];
+    u32x4 bias;
+};
+struct EpiToken {
+    float xs;
+    u32x4 r;
+};
+template <bool F8>
+__device__ __forceinline__ EpiCols epi_cols(const EpiParams& p, int n) {
+    EpiCols c;
+    c.bias = u32x4{0, 0, 0, 0};
+    if (n + 8 <= p.N) {
+        if constexpr (F8) {
 #pragma unroll
-        for (int r = 0; r < 4; ++r) v[r] = activate(v[r], p.act);
-        if (p.R != nullptr) {
-            const u32x2 b = *reinterpret_cast<const u32x2*>(p.R + at);
-            v += f32x4{__uint_as_float(b[0] << 16), __uint_as_float(b[0] & 0xffff0000u),
-                       __uint_as_float(b[1] << 16), __uint_as_float(b[1] & 0xffff0000u)};
+            for (int h = 0; h < 2; ++h) {
+                const f32x4 w = *reinterpret_cast<const f32x4*>(p.ws + n + 4 * h);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) c.ws[4 * h + r] = w[r];
+            }
         }
-        u32x2 o;
-        o[0] = f32_to_bf16_bits(v[0]) | (f32_to_bf16_bits(v[1]) << 16);
-        o[1] = f32_to_bf16_bits(v[2]) | (f32_to_bf16_bits(v[3]) << 16);
-        *reinterpret_cast<u32x2*>(p.Y + at) = o;
+        if (p.bias != nullptr) c.bias = *reinterpret_cast<const u32x4*>(p.bias + n);
     } else {
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            if (n + r >= p.N) continue;
-            float z = v[r];
-            if constexpr (F8) z *= p.ws[n + r];
-            if (p.bias != nullptr) z += bf16_bits_to_f32(p.bias[n + r]);
-            z = activate(z, p.act);
-            if (p.R != nullptr) z += bf16_bits_to_f32(p.R[at + r]);
-            p.Y[at + r] = static_cast<uint16_t>(f32_to_bf16_bits(z));
+        for (int r = 0; r < 8; ++r) {
+            if constexpr (F8) c.ws[r] = n + r < p.N ? p.ws[n + r] : 0.0f;
+            if (p.bias != nullptr && n + r < p.N)
+                c.bias[r >> 1] |= static_cast<uint32_t>(p.bias[n + r]) << (16 * (r & 1));
         }
+    }
+    return c;
+}
+template <bool F8>
+__device__ __forceinline__ EpiToken epi_token(const EpiParams& p, int m, int n) {
+    EpiToken t;
+    t.r = u32x4{0, 0, 0, 0};
+    if (m >= p.M || n >= p.N) return t;
+    if constexpr (F8) t.xs = p.xs[m];
+    if (p.R == nullptr) return t;
+    const uint16_t* at = p.R + static_cast<size_t>(m) * p.N + n;
+    if (n + 8 <= p.N) {
+        t.r = *reinterpret_cast<const u32x4_rows*>(at);
+    } else {
+#pragma unroll
+        for (int r = 0; r < 8; ++r)
+            if (n + r < p.N) t.r[r >> 1] |= static_cast<uint32_t>(at[r]) << (16 * (r & 1));
+    }
+    return t;
+}
+
+// Columns n .. n + 7 of token m from their sums.
+template <bool F8>
+__device__ __forceinline__ void epi_store(const EpiParams& p, int m, int n, float (&v)[8],
+                                          const EpiCols& c, const EpiToken& t) {
+    if (m >= p.M || n >= p.N) return;
+    if constexpr (F8) {
+#pragma unroll
+        for (int r = 0; r < 8; ++r) v[r] = v[r] * t.xs * c.ws[r];
+    }
+    if (p.bias != nullptr) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            v[2 * r] += __uint_as_float(c.bias[r] << 16);
+            v[2 * r + 1] += __uint_as_float(c.bias[r] & 0xffff0000u);
+        }
+    }
+    activate_all(v, p.act);
+    if (p.R != nullptr) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            v[2 * r] += __uint_as_float(t.r[r] << 16);
+            v[2 * r + 1] += __uint_as_float(t.r[r] & 0xffff0000u);
+        }
+    }
+    const u32x4 o = pack_bf16x8(v);
+    uint16_t* at = p.Y + static_cast<size_t>(m) * p.N + n;
+    if (n + 8 <= p.N) {
+        *reinterpret_cast<u32x4_rows*>(at) = o;
+    } else {
+#pragma unroll
+        for (int r = 0; r < 8; ++r)
+            if (n + r < p.N) at[r] = static_cast<uint16_t>(o[r >> 1] >> (16 * (r & 1)));
+    }
+}
+
+// The same columns of a K split's fp32 partials [M][N].
+__device__ __forceinline__ void epi_store_part(const EpiParams& p, float* part, int m, int n,
+                                               const float (&v)[8]) {
+    if (m >= p.M || n >= p.N) return;
+    float* at = part + static_cast<size_t>(m) * p.N + n;
+    if (n + 8 <= p.N) {
+        *reinterpret_cast<f32x4_rows*>(at) = f32x4_rows{v[0], v[1], v[2], v[3]};
+        *reinterpret_cast<f32x4_rows*>(at + 4) = f32x4_rows{v[4], v[5], v[6], v[7]};
+    } else {
+#pragma unroll
+        for (int r = 0; r < 8; ++r)
+            if (n + r < p.N) at[r] = v[r];
     }
 }
 
@@ -127,5 +198,8 @@ namespace dev {
 GemmWidePlan gemm_epi_wide_plan(const EpiParams& p, int max_splits);
 bool gemm_epi_wide(const EpiParams& p, const GemmWidePlan& plan, float* part, uint64_t stream,
                    std::string* err);
+// The epilogue of the sum of `splits` fp32 partials [splits][M][N].
+bool gemm_epi_sum(const EpiParams& p, const float* part, int splits, uint64_t stream,
+                         std::string* err);
 }  // namespace dev
 }  // namespace kcmm

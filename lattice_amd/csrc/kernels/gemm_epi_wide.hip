@@ -32,39 +32,6 @@ struct EpiWideParams {
 
 constexpr int kEpiWideLds = 160 * 1024;
 
-// Columns n .. n + 7 of token m from their sums.
-template <bool F8>
-__device__ __forceinline__ void epi_store8(const EpiParams& p, int m, int n, float (&v)[8],
-                                           const float (&ws)[8], const float (&bias)[8]) {
-    const size_t at = static_cast<size_t>(m) * p.N + n;
-    if constexpr (F8) {
-        const float xs = p.xs[m];
-#pragma unroll
-        for (int r = 0; r < 8; ++r) v[r] = v[r] * xs * ws[r];
-    }
-#pragma unroll
-    for (int r = 0; r < 8; ++r) v[r] += bias[r];
-    activate_all(v, p.act);
-    if (p.N % 8 == 0) {
-        if (p.R != nullptr) {
-            const u32x4 rr = *reinterpret_cast<const u32x4*>(p.R + at);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                v[2 * e] += __uint_as_float(rr[e] << 16);
-                v[2 * e + 1] += __uint_as_float(rr[e] & 0xffff0000u);
-            }
-        }
-        *reinterpret_cast<u32x4*>(p.Y + at) = pack_bf16x8(v);
-        return;
-    }
-#pragma unroll
-    for (int r = 0; r < 8; ++r) {
-        if (n + r >= p.N) continue;
-        if (p.R != nullptr) v[r] += bf16_bits_to_f32(p.R[at + r]);
-        p.Y[at + r] = static_cast<uint16_t>(f32_to_bf16_bits(v[r]));
-    }
-}
-
 // One tile: 256 weight rows of weight tile tn by BM = 64 * FB tokens from m0.
 // The phases, waits and places are those of wide_tile in gemm_wide.hip.
 template <bool F8, int FB, bool WNT>
@@ -235,42 +202,28 @@ __device__ __forceinline__ void epi_wide_tile(const EpiWideParams& p, uint8_t* l
 
     // acc[ah][i][bh][j][r] = token m0 + bh*BM/2 + wm*16*FB + 16j + ln, weight
     // row (of half ah) wn*32 + 8*lg + 4*i + r
+    auto token = [&](int bh, int j) { return m0 + bh * (BM / 2) + wm * 16 * FB + 16 * j + ln; };
+    const bool plain = p.part == nullptr;
 #pragma unroll
     for (int ah = 0; ah < 2; ++ah) {
         const int n = n0 + ah * 128 + wn * 32 + 8 * lg;
-        if (n >= e.N) continue;
-        float ws[8], bias[8];
+        const EpiCols cols = epi_cols<F8>(e, plain ? n : e.N);
 #pragma unroll
-        for (int r = 0; r < 8; ++r) {
-            const int at = min(n + r, e.N - 1);
-            ws[r] = F8 ? e.ws[at] : 1.0f;
-            bias[r] = e.bias != nullptr ? bf16_bits_to_f32(e.bias[at]) : 0.0f;
-        }
+        for (int bh = 0; bh < 2; ++bh) {
+            EpiToken t[FB];   // every load of the half before its stores
 #pragma unroll
-        for (int bh = 0; bh < 2; ++bh)
+            for (int j = 0; j < FB; ++j) t[j] = epi_token<F8>(e, plain ? token(bh, j) : e.M, n);
 #pragma unroll
             for (int j = 0; j < FB; ++j) {
-                const int m = m0 + bh * (BM / 2) + wm * 16 * FB + 16 * j + ln;
-                if (m >= e.M) continue;
                 float v[8];
 #pragma unroll
                 for (int i = 0; i < 2; ++i)
 #pragma unroll
                     for (int r = 0; r < 4; ++r) v[4 * i + r] = acc[ah][i][bh][j][r];
-                if (p.part != nullptr) {
-                    float* d = p.part + (static_cast<size_t>(blockIdx.y) * e.M + m) * e.N + n;
-                    if (e.N % 8 == 0) {
-                        *reinterpret_cast<f32x4*>(d) = acc[ah][0][bh][j];
-                        *reinterpret_cast<f32x4*>(d + 4) = acc[ah][1][bh][j];
-                    } else {
-#pragma unroll
-                        for (int r = 0; r < 8; ++r)
-                            if (n + r < e.N) d[r] = v[r];
-                    }
-                    continue;
-                }
-                epi_store8<F8>(e, m, n, v, ws, bias);
+                if (plain) epi_store<F8>(e, token(bh, j), n, v, cols, t[j]);
+                else epi_store_part(e, p.part + static_cast<size_t>(blockIdx.y) * e.M * e.N, token(bh, j), n, v);
             }
+        }
     }
 }
 
@@ -313,26 +266,35 @@ void gemm_epi_wide_kernel(EpiWideParams p) {
     }
 }
 
-// The epilogue of the summed K splits, 4 columns a thread.
-template <bool F8, bool VEC>
-__global__ __launch_bounds__(256) void gemm_epi_sum(EpiParams e, const float* __restrict__ part,
+// The epilogue of the summed K splits, 8 columns a thread.
+template <bool F8>
+__global__ __launch_bounds__(256) void sum_partials_epi(EpiParams e, const float* __restrict__ part,
                                                     int splits) {
-    const int groups = (e.N + 3) / 4;
+    const int groups = (e.N + 7) / 8;
     const size_t i = static_cast<size_t>(blockIdx.x) * 256 + threadIdx.x;
     if (i >= static_cast<size_t>(groups) * e.M) return;
-    const int m = static_cast<int>(i / groups), n = static_cast<int>(i - static_cast<size_t>(m) * groups) * 4;
+    const int m = static_cast<int>(i / groups), n = static_cast<int>(i - static_cast<size_t>(m) * groups) * 8;
+    const EpiCols cols = epi_cols<F8>(e, n);
+    const EpiToken t = epi_token<F8>(e, m, n);
     const size_t MN = static_cast<size_t>(e.M) * e.N;
     const float* at = part + static_cast<size_t>(m) * e.N + n;
-    f32x4 s = f32x4{0, 0, 0, 0};
+    float s[8] = {0, 0, 0, 0, 0, 0, 0, 0};
     for (int k = 0; k < splits; ++k, at += MN) {
-        if constexpr (VEC) {
-            s += *reinterpret_cast<const f32x4*>(at);
+        if (n + 8 <= e.N) {
+            const f32x4 a = *reinterpret_cast<const f32x4_rows*>(at);
+            const f32x4 b = *reinterpret_cast<const f32x4_rows*>(at + 4);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                s[r] += a[r];
+                s[4 + r] += b[r];
+            }
         } else {
 #pragma unroll
-            for (int r = 0; r < 4; ++r) s[r] += at[min(r, e.N - 1 - n)];
+            for (int r = 0; r < 8; ++r)
+                if (n + r < e.N) s[r] += at[r];
         }
     }
-    epi_store4<F8, VEC>(e, m, n, s);
+    epi_store<F8>(e, m, n, s, cols, t);
 }
 
 template <bool F8>
@@ -341,29 +303,33 @@ void launch_epi_wide(const EpiWideParams& p, int grid, int splits, bool once, hi
         hipLaunchKernelGGL((gemm_epi_wide_kernel<F8, true>), dim3(grid, splits), dim3(512), 0, s, p);
     else
         hipLaunchKernelGGL((gemm_epi_wide_kernel<F8, false>), dim3(grid, splits), dim3(512), 0, s, p);
-    if (splits == 1) return;
-    const EpiParams& e = p.e;
-    const size_t n = static_cast<size_t>((e.N + 3) / 4) * e.M;
-    const dim3 sum(static_cast<unsigned>((n + 255) / 256));
-    if (e.N % 4 == 0)
-        hipLaunchKernelGGL((gemm_epi_sum<F8, true>), sum, dim3(256), 0, s, e, p.part, splits);
-    else
-        hipLaunchKernelGGL((gemm_epi_sum<F8, false>), sum, dim3(256), 0, s, e, p.part, splits);
 }
 
 }  // namespace
 
 namespace dev {
 
+bool gemm_epi_sum(const EpiParams& e, const float* part, int splits, uint64_t stream,
+                         std::string* err) {
+    const size_t n = static_cast<size_t>((e.N + 7) / 8) * e.M;
+    hipLaunchKernelGGL(e.xs != nullptr ? sum_partials_epi<true> : sum_partials_epi<false>,
+                       dim3(static_cast<unsigned>((n + 255) / 256)), dim3(256), 0,
+                       reinterpret_cast<hipStream_t>(stream), e, part, splits);
+    KCMM_HIP_CHECK(hipGetLastError(), err);
+    return true;
+}
+
 // The plan of the bf16 product of as many bytes: chunks cost the same here for
-// either type.
+// either type.  Its K splits are of equal length; from 32 lines on it is asked
+// for a multiple of 8, and the last split is shorter (542 x 3700 x 10928, 171
+// lines: unsplit 174 us).
 GemmWidePlan gemm_epi_wide_plan(const EpiParams& p, int max_splits) {
-    const uint32_t lines = (p.kb + 127) / 128;
+    const uint32_t lines = (p.kb + 127) / 128, round = lines >= 32 ? (lines + 7) / 8 * 8 : lines;
     GemmWidePlan plan;
-    if (lines >= 2)
-        plan = gemm_wide_plan(static_cast<uint32_t>(p.M), static_cast<uint32_t>(p.N), lines * 64, false,
+    if (round >= 2)
+        plan = gemm_wide_plan(static_cast<uint32_t>(p.M), static_cast<uint32_t>(p.N), round * 64, false,
                               max_splits);
-    if (lines < 2 || plan.splits < 1) plan = GemmWidePlan{};
+    if (round < 2 || plan.splits < 1) plan = GemmWidePlan{};
     return plan;
 }
 
@@ -371,13 +337,14 @@ bool gemm_epi_wide(const EpiParams& e, const GemmWidePlan& c, float* part, uint6
                    std::string* err) {
     EpiWideParams p{};
     p.e = e;
-    p.part = c.splits > 1 ? part : nullptr;
     const int lines = static_cast<int>((e.kb + 127) / 128);
-    if (c.splits < 1 || lines % c.splits != 0 || (c.splits > 1 && part == nullptr)) {
-        *err = "epilogue product: K splits of whole lines, with their partials";
+    p.lines = (lines + std::max(1, c.splits) - 1) / std::max(1, c.splits);
+    const int splits = (lines + p.lines - 1) / p.lines;   // (none of them empty)
+    p.part = splits > 1 ? part : nullptr;
+    if (splits > 1 && part == nullptr) {
+        *err = "epilogue product: K splits need their partials";
         return false;
     }
-    p.lines = lines / c.splits;
     const int tiles_n = (e.N + 255) / 256;
     const int fb[2] = {c.fb0, c.fb1};
     p.nw[1] = std::min(c.nw1, tiles_n);
@@ -395,10 +362,10 @@ bool gemm_epi_wide(const EpiParams& e, const GemmWidePlan& c, float* part, uint6
     }
     const bool once = e.M <= 64 * c.fb0 && c.nw1 == 0;   // one token tile
     hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-    if (e.xs != nullptr) launch_epi_wide<true>(p, grid, c.splits, once, s);
-    else launch_epi_wide<false>(p, grid, c.splits, once, s);
+    if (e.xs != nullptr) launch_epi_wide<true>(p, grid, splits, once, s);
+    else launch_epi_wide<false>(p, grid, splits, once, s);
     KCMM_HIP_CHECK(hipGetLastError(), err);
-    return true;
+    return splits == 1 || gemm_epi_sum(e, p.part, splits, stream, err);
 }
 
 }  // namespace dev

@@ -52,7 +52,7 @@ __device__ __forceinline__ void row_piece(const RowParams& p, size_t row, int i,
         widen8(*reinterpret_cast<const u32x4*>(g), v);
         widen8(*reinterpret_cast<const u32x4*>(g + p.cols), u);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = v[e] / (1.0f + __expf(-v[e])) * u[e];
+        for (int e = 0; e < 8; ++e) v[e] = v[e] / (1.0f + expf(-v[e])) * u[e];
     } else {
         const size_t at = row * p.cols + i * 8;
         widen8(*reinterpret_cast<const u32x4*>(p.x + at), v);

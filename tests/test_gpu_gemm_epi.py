@@ -128,6 +128,32 @@ def test_whole_numbers_bit_for_bit(gpu_lib, m, n, k, fp8):
 
 
 @pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("tile", [*range(1, 13), 100])
+def test_every_tile_whole_numbers(gpu_lib, tunables, tile, fp8):
+    """Each tile of the tile kernel, and the 256-row tiles (100), with the sizes
+    they are not chosen for too: one token, tiles that M and N end inside, rows
+    of less than a line, of one share's lines, of more; with K splits."""
+    import torch
+    rng = np.random.default_rng([tile, fp8])
+    tunables.setenv("KCMM_EPI_TILE", str(tile))
+    for splits in (1, 2, 3):
+        tunables.setenv("KCMM_GEMM_SPLITS", str(splits))
+        for m, n, k in [(1, 5, 16), (9, 137, 112), (33, 64, 1168), (70, 203, 2320), (130, 264, 4112),
+                        (301, 520, 1024)]:
+            x = rng.integers(-3, 4, (m, k)).astype(np.float64)
+            w = rng.integers(-3, 4, (n, k)).astype(np.float64)
+            bias = E.bf16(rng.integers(-100, 101, n))
+            res = E.bf16(rng.integers(-100, 101, (m, n)))
+            xs = ws = None
+            if fp8:
+                xs, ws = np.exp2(rng.integers(-1, 2, m)), np.exp2(rng.integers(-1, 2, n))
+            y, s = E.product(x, w, xs, ws, bias, res, ACT_NONE)
+            assert s.max() < 2 ** 20
+            got = call(torch, gpu_lib, x, w, xs, ws, bias, res)
+            assert np.array_equal(got, E.bf16(y)), (splits, m, n, k)
+
+
+@pytest.mark.parametrize("fp8", [False, True])
 @pytest.mark.parametrize("act", [ACT_NONE, ACT_RELU, ACT_GELU, ACT_GELU_TANH, ACT_SILU])
 def test_activations_over_their_range(gpu_lib, act, fp8):
     """x = 1 column of ones, so z is the bias: -40 .. 40, fine near zero."""
