@@ -60,7 +60,6 @@ __device__ __forceinline__ void wait_loads_in_flight(int left) {
 template <bool F8, int NB, int MB, int WN, int WM, int WK, int ST>
 __global__ __launch_bounds__(64 * WN * WM * WK) void gemm_epi_tile(EpiParams p, float* part, int klines) {
     constexpr bool SHARED = WN * WM > 1;      // several waves read a place
-    constexpr int AHEAD = SHARED ? ST - 1 : ST;
     constexpr int WL = 2 * NB / WM, XL = 2 * MB / WN;   // loads of 1 KiB a wave and line
     static_assert(WL * WM == 2 * NB && XL * WN == 2 * MB, "loads divide over the waves");
     constexpr int SHARE = (NB * WN + MB * WM) * 2048, PLACE = WK * SHARE;
@@ -90,14 +89,25 @@ __global__ __launch_bounds__(64 * WN * WM * WK) void gemm_epi_tile(EpiParams p, 
         xof[i] = static_cast<uint32_t>(min(m0 + 8 * (xload + i) + lrow, p.M - 1)) * p.kb + piece * 16;
     uint8_t* const share = lds + wk * SHARE;
     int to = 0;   // the place that issue fills next
+    // Where weights are read once, the workgroups of an XCD (workgroup i runs on
+    // XCD i % 8) begin at lines spread over k, so that all but the first to come
+    // to a line of X find it in L2; in step, each of them waits for the same miss.
+    const bool once = gridDim.y == 1;
+    const int turn = once ? static_cast<int>((blockIdx.x >> 3) * steps / ((gridDim.x + 7) >> 3)) : 0;
+    auto line_of = [&](int i) { return (i + turn < steps ? i + turn : i + turn - steps) * WK + wk; };
     auto issue = [&](int i) {
-        const int line = first + min(i * WK + wk, lines - 1);
+        const int line = first + min(line_of(i), lines - 1);
         const uint32_t b = line + 1 == all ? back : 0;
         const uint8_t* w = p.W + static_cast<size_t>(line) * 128;
         const uint8_t* x = p.X + static_cast<size_t>(line) * 128;
         uint8_t* dst = share + to * PLACE;
+        if (once) {
 #pragma unroll
-        for (int k = 0; k < WL; ++k) load_lds16_nt(w + (wof[k] - b), dst + (wload + k) * 1024);
+            for (int k = 0; k < WL; ++k) load_lds16_nt(w + (wof[k] - b), dst + (wload + k) * 1024);
+        } else {
+#pragma unroll
+            for (int k = 0; k < WL; ++k) load_lds16(w + (wof[k] - b), dst + (wload + k) * 1024);
+        }
 #pragma unroll
         for (int k = 0; k < XL; ++k)
             load_lds16(x + (xof[k] - b), dst + NB * WN * 2048 + (xload + k) * 1024);
@@ -112,62 +122,93 @@ __global__ __launch_bounds__(64 * WN * WM * WK) void gemm_epi_tile(EpiParams p, 
     const int sw[2] = {((0 + lg) ^ (ln & 7)) * 16, ((4 + lg) ^ (ln & 7)) * 16};
     const bool cut[2] = {lg * 16 >= last, (4 + lg) * 16 >= last};
     // output item q: 8 columns of a token, columns fastest; what its epilogue
-    // reads is on its way before the operands are
+    // reads is on its way before the operands are (where registers allow it)
+    constexpr bool EARLY = ITEMS <= 2;
     auto item_n = [&](int j) { return n0 + (static_cast<int>(threadIdx.x) + j * NT) % (R / 8) * 8; };
     auto item_m = [&](int j) { return m0 + (static_cast<int>(threadIdx.x) + j * NT) / (R / 8); };
     EpiCols cols[ITEMS];
     EpiToken tokens[ITEMS];
+    auto load_epilogue = [&]() {
 #pragma unroll
-    for (int j = 0; j < ITEMS; ++j) {
-        cols[j] = epi_cols<F8>(p, part == nullptr ? item_n(j) : p.N);
-        tokens[j] = epi_token<F8>(p, part == nullptr ? item_m(j) : p.M, item_n(j));
-    }
-#pragma unroll
-    for (int i = 0; i < AHEAD; ++i)
-        if (i < steps) issue(i);
-    int at = 0;   // the place of step i
-    for (int i = 0; i < steps; ++i) {
-        wait_loads_in_flight<WL + XL, AHEAD - 1>(min(AHEAD - 1, steps - 1 - i));
-        if constexpr (SHARED) {
-            phase_barrier();   // all of step i is there, step i - 1 has been read
-            if (i + AHEAD < steps) issue(i + AHEAD);
+        for (int j = 0; j < ITEMS; ++j) {
+            cols[j] = epi_cols<F8>(p, part == nullptr ? item_n(j) : p.N);
+            tokens[j] = epi_token<F8>(p, part == nullptr ? item_m(j) : p.M, item_n(j));
         }
-        const uint8_t* src = share + at * PLACE + ln * 128;
+    };
+    if constexpr (EARLY) load_epilogue();
+#pragma unroll
+    for (int i = 0; i < ST; ++i)
+        if (i < steps) issue(i);
+    struct Operands {
         u32x4 a[NB][2], b[MB][2];
+    };
+    int at = 0;   // the place of the step that is read next
+    auto read = [&](Operands& o) {
+        const uint8_t* src = share + at * PLACE + ln * 128;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
 #pragma unroll
             for (int k = 0; k < NB; ++k)
-                a[k][h] = *reinterpret_cast<const u32x4*>(src + (wn * NB + k) * 2048 + sw[h]);
+                o.a[k][h] = *reinterpret_cast<const u32x4*>(src + (wn * NB + k) * 2048 + sw[h]);
 #pragma unroll
             for (int k = 0; k < MB; ++k)
-                b[k][h] = *reinterpret_cast<const u32x4*>(src + (NB * WN + wm * MB + k) * 2048 + sw[h]);
-        }
-        wait_vm_lgkm0<63>();   // the operands are in registers: the place is free
-        asm volatile("" ::: "memory");
-        __builtin_amdgcn_sched_barrier(0);
-        if constexpr (!SHARED) {
-            if (i + AHEAD < steps) issue(i + AHEAD);
-            __builtin_amdgcn_sched_barrier(0);
+                o.b[k][h] = *reinterpret_cast<const u32x4*>(src + (NB * WN + wm * MB + k) * 2048 + sw[h]);
         }
         at = at + 1 == ST ? 0 : at + 1;
-        const int line = i * WK + wk;
-        if (SHARED && WK > 1 && line >= lines) continue;
+    };
+    auto compute = [&](Operands& o, int i) {
+        const int line = line_of(i);
+        if (SHARED && WK > 1 && line >= lines) return;
         if (last < 128 && first + line + 1 == all) {   // the row's end: zeros behind it
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 if (!cut[h]) continue;
 #pragma unroll
-                for (int k = 0; k < NB; ++k) a[k][h] = u32x4{0, 0, 0, 0};
+                for (int k = 0; k < NB; ++k) o.a[k][h] = u32x4{0, 0, 0, 0};
 #pragma unroll
-                for (int k = 0; k < MB; ++k) b[k][h] = u32x4{0, 0, 0, 0};
+                for (int k = 0; k < MB; ++k) o.b[k][h] = u32x4{0, 0, 0, 0};
             }
         }
 #pragma unroll
         for (int k = 0; k < NB; ++k)
 #pragma unroll
-            for (int j = 0; j < MB; ++j) acc[k][j] = mfma_line<F8>(a[k], b[j], acc[k][j]);
+            for (int j = 0; j < MB; ++j) acc[k][j] = mfma_line<F8>(o.a[k], o.b[j], acc[k][j]);
+    };
+    // Steps i + 1 .. i + ST - 1 are on their way or there, step i's operands in
+    // `now`, so its place may be filled (a shared one once the barrier has shown
+    // that every wave is that far); the matrix instructions run while the next
+    // operands come from LDS.
+    auto step = [&](Operands& now, Operands& next, int i) {
+        if (i + 1 < steps) {
+            if constexpr (SHARED) {
+                wait_loads_in_flight<WL + XL, ST - 2>(min(ST - 2, steps - 2 - i));
+                phase_barrier();
+                if (i + ST < steps) issue(i + ST);
+            } else {
+                if (i + ST < steps) issue(i + ST);
+                wait_loads_in_flight<WL + XL, ST - 1>(min(ST - 1, steps - 2 - i));
+            }
+            read(next);
+        }
+        compute(now, i);
+        wait_vm_lgkm0<63>();
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    if (steps > 0) {   // (a share of a private ring may have no line)
+        Operands o0, o1;
+        wait_loads_in_flight<WL + XL, ST - 1>(min(ST - 1, steps - 1));
+        if constexpr (SHARED) phase_barrier();
+        read(o0);
+        wait_vm_lgkm0<63>();
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_sched_barrier(0);
+        for (int i = 0; i < steps; i += 2) {
+            step(o0, o1, i);
+            if (i + 1 < steps) step(o1, o0, i + 1);
+        }
     }
+    if constexpr (!EARLY) load_epilogue();
     __syncthreads();   // every place is done with
     float* const red = reinterpret_cast<float*>(lds);
 #pragma unroll
@@ -194,14 +235,15 @@ __global__ __launch_bounds__(64 * WN * WM * WK) void gemm_epi_tile(EpiParams p, 
 }
 
 // A tile and its modelled time in us: a workgroup alone takes f + g a step (a
-// line of each share), one among others on its CU e + l of that CU's time, the
-// weights come at h TB/s.
-// Fitted to timings of 2900 products (M 1 .. 4096, N 64 .. 32768, K 64 .. 14336,
-// either type): within 10% at the median, 30% for nine in ten; the tile chosen
-// by it is 2.4% slower than the best of all in the mean.
+// line of each share), one among others on its CU e + l of that CU's time; the
+// weights come at h TB/s, the outputs go at s.  Fitted to timings of 5066
+// products (M 1 .. 3000, N 64 .. 65536, K 64 .. 14336, either type): within 10% at
+// the median, 20-30% for nine in ten; what it chooses among the tiles, K splits
+// and the 256-row tiles is 1.8% slower than the best of them in the mean (7.5%
+// or less for nine in ten, 22% for 99 in a hundred).
 struct Tile {
     int nb, mb, wn, wm, wk, st;
-    float f, g, e, l, h;
+    float f, g, e, l, h, s;
     constexpr int rows() const { return 16 * nb * wn; }
     constexpr int tokens() const { return 16 * mb * wm; }
     constexpr int waves() const { return wn * wm * wk; }
@@ -211,18 +253,18 @@ struct Tile {
     }
 };
 constexpr Tile kTiles[] = {
-    {1, 1, 1, 1, 8, 2, 1.84f, 0.13f, 0.10f, 0.71f, 7.3f},   //  16 rows x  16 tokens
-    {2, 1, 1, 1, 8, 3, 0.38f, 1.17f, 2.01f, 0.01f, 5.3f},   //  32 x  16
-    {2, 1, 2, 1, 4, 3, 0.76f, 1.07f, 1.84f, 0.01f, 5.6f},   //  64 x  16
-    {1, 2, 1, 1, 8, 3, 1.35f, 0.71f, 0.03f, 1.07f, 8.0f},   //  16 x  32
-    {2, 2, 1, 1, 8, 2, 0.54f, 1.47f, 0.69f, 1.05f, 6.6f},   //  32 x  32
-    {1, 2, 4, 1, 2, 4, 1.53f, 0.51f, 0.34f, 0.59f, 8.0f},   //  64 x  32
-    {2, 2, 4, 1, 2, 3, 1.20f, 1.03f, 0.00f, 0.82f, 6.2f},   // 128 x  32
-    {2, 4, 1, 1, 4, 2, 1.32f, 0.82f, 0.29f, 1.04f, 8.0f},   //  32 x  64
-    {1, 4, 4, 1, 2, 4, 1.33f, 0.74f, 0.91f, 0.71f, 8.0f},   //  64 x  64
-    {1, 4, 8, 1, 1, 5, 1.96f, 0.54f, 1.24f, 0.57f, 8.0f},   // 128 x  64
-    {2, 4, 2, 2, 2, 3, 2.22f, 0.80f, 1.41f, 1.08f, 8.0f},   //  64 x 128
-    {1, 8, 8, 1, 1, 4, 3.98f, 0.38f, 2.53f, 0.84f, 8.0f},   // 128 x 128
+    {1, 1, 1, 1, 8, 2, 1.91f, 0.07f, 0.23f, 0.52f, 4.4f, 50.0f},   //  16 rows x  16 tokens
+    {2, 1, 1, 1, 8, 3, 1.95f, 0.42f, 0.00f, 0.76f, 4.1f, 50.0f},   //  32 x  16
+    {2, 1, 2, 1, 4, 3, 1.48f, 0.65f, 1.88f, 0.01f, 4.3f, 2.2f},    //  64 x  16
+    {1, 2, 1, 1, 8, 3, 2.13f, 0.01f, 0.80f, 0.69f, 4.0f, 50.0f},   //  16 x  32
+    {2, 2, 1, 1, 8, 2, 1.92f, 0.43f, 0.00f, 0.99f, 4.0f, 2.0f},    //  32 x  32
+    {1, 2, 4, 1, 2, 4, 1.89f, 0.28f, 0.00f, 0.44f, 4.2f, 2.3f},    //  64 x  32
+    {2, 2, 4, 1, 2, 3, 1.79f, 0.43f, 0.00f, 0.70f, 4.0f, 2.1f},    // 128 x  32
+    {2, 4, 1, 1, 4, 2, 1.63f, 0.54f, 0.00f, 0.73f, 4.0f, 2.4f},    //  32 x  64
+    {1, 4, 4, 1, 2, 4, 1.66f, 0.48f, 0.00f, 0.46f, 4.0f, 3.2f},    //  64 x  64
+    {1, 4, 8, 1, 1, 5, 1.25f, 0.42f, 1.79f, 0.27f, 4.0f, 3.4f},    // 128 x  64
+    {2, 4, 2, 2, 2, 3, 2.01f, 0.67f, 0.00f, 0.73f, 4.0f, 3.0f},    //  64 x 128
+    {2, 4, 4, 2, 1, 5, 2.52f, 0.45f, 1.38f, 0.55f, 4.0f, 3.1f},    // 128 x 128
 };
 constexpr int kTileCount = sizeof(kTiles) / sizeof(kTiles[0]);
 
@@ -238,7 +280,8 @@ double tile_us(const Tile& t, const EpiParams& p, int splits) {
     const double hbm = static_cast<double>(p.N) * p.kb / (t.h * 1e6);
     auto p4 = [](double x) { return x * x * x * x; };
     const double sum = splits > 1 ? 4.3 + 4e-6 * splits * p.M * p.N : 0.0;
-    return 1.7 + std::sqrt(std::sqrt(p4(alone) + p4(loaded) + p4(hbm))) + sum;
+    const double out = 2e-6 * p.M * p.N / t.s;
+    return 1.7 + std::sqrt(std::sqrt(p4(alone) + p4(loaded) + p4(hbm))) + out + sum;
 }
 
 struct Choice {

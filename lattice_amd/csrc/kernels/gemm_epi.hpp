@@ -44,8 +44,8 @@ __device__ __forceinline__ float activate(float z, int act) {
         case kActRelu: return z < 0.0f ? 0.0f : z;
         case kActGelu: return gelu_erf(z);
         case kActGeluTanh:   // z sigmoid(2 u): the tanh form without its cancellation
-            return z / (1.0f + __expf(-1.59576912f * z * fmaf(0.044715f * z, z, 1.0f)));
-        case kActSilu: return z / (1.0f + __expf(-z));
+            return z * __builtin_amdgcn_rcpf(1.0f + __expf(-1.59576912f * z * fmaf(0.044715f * z, z, 1.0f)));
+        case kActSilu: return z * __builtin_amdgcn_rcpf(1.0f + __expf(-z));
         default: return z;
     }
 }
@@ -82,10 +82,21 @@ struct EpiToken {
     float xs;
     u32x4 r;
 };
+// Elements n .. n + 7 of a row of N, the last one in the place of those behind it.
+__device__ __forceinline__ u32x4 row_end(const uint16_t* row, int n, int N) {
+    uint16_t h[8];
+#pragma unroll
+    for (int r = 0; r < 8; ++r) h[r] = row[min(n + r, N - 1)];
+    u32x4 v;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) v[r] = h[2 * r] | (static_cast<uint32_t>(h[2 * r + 1]) << 16);
+    return v;
+}
 template <bool F8>
 __device__ __forceinline__ EpiCols epi_cols(const EpiParams& p, int n) {
     EpiCols c;
     c.bias = u32x4{0, 0, 0, 0};
+    if (n >= p.N) return c;
     if (n + 8 <= p.N) {
         if constexpr (F8) {
 #pragma unroll
@@ -96,13 +107,12 @@ __device__ __forceinline__ EpiCols epi_cols(const EpiParams& p, int n) {
             }
         }
         if (p.bias != nullptr) c.bias = *reinterpret_cast<const u32x4*>(p.bias + n);
-    } else {
+    } else {   // the row's end: the last column again, so that no load waits for another
+        if constexpr (F8) {
 #pragma unroll
-        for (int r = 0; r < 8; ++r) {
-            if constexpr (F8) c.ws[r] = n + r < p.N ? p.ws[n + r] : 0.0f;
-            if (p.bias != nullptr && n + r < p.N)
-                c.bias[r >> 1] |= static_cast<uint32_t>(p.bias[n + r]) << (16 * (r & 1));
+            for (int r = 0; r < 8; ++r) c.ws[r] = p.ws[min(n + r, p.N - 1)];
         }
+        if (p.bias != nullptr) c.bias = row_end(p.bias, n, p.N);
     }
     return c;
 }
@@ -117,9 +127,7 @@ __device__ __forceinline__ EpiToken epi_token(const EpiParams& p, int m, int n) 
     if (n + 8 <= p.N) {
         t.r = *reinterpret_cast<const u32x4_rows*>(at);
     } else {
-#pragma unroll
-        for (int r = 0; r < 8; ++r)
-            if (n + r < p.N) t.r[r >> 1] |= static_cast<uint32_t>(at[r]) << (16 * (r & 1));
+        t.r = row_end(at - n, n, p.N);
     }
     return t;
 }

@@ -42,6 +42,15 @@ __device__ __forceinline__ void widen8(const u32x4& v, float (&f)[8]) {
     }
 }
 
+// e^x to two units in the last place: 2^(x log2 e) by the hardware's exp2, what
+// the product's rounding leaves out as a factor.
+__device__ __forceinline__ float exp_f32(float x) {
+    const float hi = x * 1.44269502f;
+    const float lo = fmaf(x, 1.92596299e-8f, fmaf(x, 1.44269502f, -hi));
+    const float e = __builtin_amdgcn_exp2f(hi);
+    return fabsf(hi) < 128.0f ? fmaf(e, lo * 0.693147181f, e) : e;
+}
+
 // The row's values before the norm's factor: piece `i` (8 columns) of row
 // `row`.  norm: stores the hidden piece where there is a residual.
 template <int MODE>
@@ -52,7 +61,7 @@ __device__ __forceinline__ void row_piece(const RowParams& p, size_t row, int i,
         widen8(*reinterpret_cast<const u32x4*>(g), v);
         widen8(*reinterpret_cast<const u32x4*>(g + p.cols), u);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = v[e] / (1.0f + expf(-v[e])) * u[e];
+        for (int e = 0; e < 8; ++e) v[e] = v[e] * __builtin_amdgcn_rcpf(1.0f + exp_f32(-v[e])) * u[e];
     } else {
         const size_t at = row * p.cols + i * 8;
         widen8(*reinterpret_cast<const u32x4*>(p.x + at), v);
