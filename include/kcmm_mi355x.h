@@ -497,9 +497,12 @@ typedef struct kcmm_gemm_epilogue {
 } kcmm_gemm_epilogue_t;
 
 /** y[m][n] = bf16(act(xscale[m] wscale[n] (x8[m][k] * w8[n][k]^T) + bias[n]) +
- *  residual), rounded once.  k % 16 == 0 and k <= 2^24, any m and n; operands
- *  below 4 GiB each, m * n < 2^31; y overlaps no operand but residual, where they are the
- *  same buffer. */
+ *  residual), rounded once.  Any m <= 2^20 and n <= 2^22, k % 16 == 0 and <= 2^24;
+ *  operands below 4 GiB each, m * n < 2^31.  y overlaps no operand but
+ *  residual, where the two are one buffer.  The same bits for the same
+ *  operands on any stream; in a capture, and where memory is short, another
+ *  order of the sums over k may be taken (K is then not split over
+ *  workgroups, as that needs a workspace of the library's). */
 int kcmm_gemm_fp8_on_stream(uint64_t x8_ptr, uint64_t xscale_ptr, uint64_t w8_ptr,
                             uint64_t wscale_ptr, uint64_t y_ptr,
                             const kcmm_gemm_epilogue_t *epilogue, uint32_t m, uint32_t n,

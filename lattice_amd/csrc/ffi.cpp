@@ -1267,8 +1267,8 @@ int gemm_epi_call(const char* fn, uint64_t x, uint64_t xscale, uint64_t w, uint6
             return false;
         }
         const uint64_t eb = fp8 ? 1 : 2, M = m, N = n, K = k;
-        if (M * K * eb >> 32 || N * K * eb >> 32 || M * N >> 31) {
-            *err = "operand too large (4 GiB each, m * n < 2^31)";
+        if (M > 1u << 20 || N > 1u << 22 || M * K * eb >> 32 || N * K * eb >> 32 || M * N >> 31) {
+            *err = "operand too large (m <= 2^20, n <= 2^22, 4 GiB each, m * n < 2^31)";
             return false;
         }
         if (epi.activation < KCMM_ACT_NONE || epi.activation > KCMM_ACT_SILU) {

@@ -349,9 +349,12 @@ float* partials(const EpiParams& p, int splits, uint64_t stream) {
     return static_cast<float*>(part);
 }
 
-// Modelled time of the 256-row tiles, which no product of up to 96 tokens, and
-// none of a single line, of those timed needed.
+// Modelled time of the 256-row tiles.  They are looked at above 96 tokens and
+// not for rows of a single line: up to 96 tokens no product of those timed was
+// clearly faster on them, and the model is too kind to them there (64 x 28672 x
+// 4096 e4m3 33.5 us, 21.6 on a tile).
 double wide_us(const dev::GemmWidePlan& plan) { return 2.0 + plan.us; }
+bool wide_may_do(const EpiParams& p) { return p.kb > 128 && p.M > 96; }
 
 bool run_epi(const EpiParams& p, uint64_t stream, std::string* err) {
     const int forced = dev::tunable_or(dev::Tun::kEpiTile, 0);   // (tests and tuning)
@@ -364,7 +367,7 @@ bool run_epi(const EpiParams& p, uint64_t stream, std::string* err) {
     float* part = nullptr;
     for (int most : {8, 1}) {
         dev::GemmWidePlan wide;
-        const bool many = forced == 100 || (p.M > 96 && p.kb > 128);
+        const bool many = forced == 100 || wide_may_do(p);
         if (many) wide = dev::gemm_epi_wide_plan(p, most);
         Choice tile;
         if (forced != 100) tile = choose_tile(p, most > 1);

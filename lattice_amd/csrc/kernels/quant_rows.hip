@@ -9,9 +9,11 @@
 // at the largest code, NaN as NaN.  The scale keeps fp32, the codes are the
 // one rounding to fewer bits, relative 2^-4, that the 8-bit product is for.
 //
-// Bound by memory for many rows and by a launch and two dependent reductions
-// for few.  A row is read once: its values stay in registers between the sum,
-// the maximum and the codes.
+// Bound by memory for many rows (residual + norm of 8192 x 4096, 235 MB, 39 us =
+// 6.0 TB/s; SwiGLU of 2048 x 14336 29.9 us = 4.9; a large copy moves 5.0) and by a
+// launch and two dependent reductions for few (3.1 us in a graph for one row of
+// 4096).  A row is read once: its values stay in registers between the sum, the
+// maximum and the codes.
 #include <algorithm>
 
 #include "../device_api.hpp"
@@ -42,13 +44,34 @@ __device__ __forceinline__ void widen8(const u32x4& v, float (&f)[8]) {
     }
 }
 
-// e^x to two units in the last place: 2^(x log2 e) by the hardware's exp2, what
-// the product's rounding leaves out as a factor.
-__device__ __forceinline__ float exp_f32(float x) {
-    const float hi = x * 1.44269502f;
-    const float lo = fmaf(x, 1.92596299e-8f, fmaf(x, 1.44269502f, -hi));
-    const float e = __builtin_amdgcn_exp2f(hi);
-    return fabsf(hi) < 128.0f ? fmaf(e, lo * 0.693147181f, e) : e;
+// silu(g) u of 8 columns.  e^-g is 2^hi by the hardware's exp2, with what the
+// rounding of hi leaves out as a factor; the quotient by its reciprocal, each with
+// one step of its residual, so that both are rounded as if exact but for rare
+// last places.  |hi| >= 128 (an infinite or vanishing e^-g, infinities, NaN) takes
+// the library's functions.  (2048 x 14336: 37.7 us with those everywhere, 33.9 with
+// the guards on every element; with the reciprocal alone three times the wrong
+// codes.)
+__device__ __forceinline__ void silu_mul8(float (&g)[8], const float (&u)[8]) {
+    bool in = true;
+    float v[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const float hi = g[e] * -1.44269502f;
+        const float lo = fmaf(g[e], -1.92596299e-8f, fmaf(g[e], -1.44269502f, -hi));
+        const float x = __builtin_amdgcn_exp2f(hi);
+        const float s = 1.0f + fmaf(x, lo * 0.693147181f, x);
+        const float r0 = __builtin_amdgcn_rcpf(s);
+        const float r = fmaf(fmaf(-s, r0, 1.0f), r0, r0);
+        const float q = g[e] * r;
+        v[e] = fmaf(fmaf(-s, q, g[e]), r, q) * u[e];
+        in &= fabsf(hi) < 128.0f;
+    }
+    if (__builtin_expect(!in, 0)) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = g[e] / (1.0f + expf(-g[e])) * u[e];
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) g[e] = v[e];
 }
 
 // The row's values before the norm's factor: piece `i` (8 columns) of row
@@ -60,8 +83,7 @@ __device__ __forceinline__ void row_piece(const RowParams& p, size_t row, int i,
         float u[8];
         widen8(*reinterpret_cast<const u32x4*>(g), v);
         widen8(*reinterpret_cast<const u32x4*>(g + p.cols), u);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = v[e] * __builtin_amdgcn_rcpf(1.0f + exp_f32(-v[e])) * u[e];
+        silu_mul8(v, u);
     } else {
         const size_t at = row * p.cols + i * 8;
         widen8(*reinterpret_cast<const u32x4*>(p.x + at), v);
@@ -78,12 +100,16 @@ __device__ __forceinline__ void row_piece(const RowParams& p, size_t row, int i,
     }
 }
 
-__device__ __forceinline__ float finite_amax(const float (&v)[8], float a) {
+// The largest |v| (of those that are no NaN: the hardware's maximum passes it
+// over), and that of the finite ones.
+__device__ __forceinline__ float amax8(const float (&v)[8], float a) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        const float b = fabsf(v[e]);
-        a = fmaxf(a, b < __builtin_inff() ? b : 0.0f);
-    }
+    for (int e = 0; e < 8; ++e) a = fmaxf(a, fabsf(v[e]));
+    return a;
+}
+__device__ __forceinline__ float finite_amax8(const float (&v)[8], float a) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) a = fmaxf(a, fabsf(v[e]) < __builtin_inff() ? fabsf(v[e]) : 0.0f);
     return a;
 }
 
@@ -91,12 +117,12 @@ __device__ __forceinline__ float row_scale(float a) {
     return a > 0.0f ? fmaxf(a / 448.0f, 0x1p-126f) : 1.0f;
 }
 
-// Eight values as codes; r = 1 / scale.
-__device__ __forceinline__ u32x2 row_codes(const float (&v)[8], float scale, float r) {
+// Eight values as codes; r = 1 / scale; finite: the row has no infinity.
+__device__ __forceinline__ u32x2 row_codes(const float (&v)[8], float scale, float r, bool finite) {
     u32x2 o;
-    bool plain = scale >= kFp8QuotientMin && scale <= kFp8QuotientMax;
+    bool plain = finite && scale >= kFp8QuotientMin && scale <= kFp8QuotientMax;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) plain &= fabsf(v[e]) < __builtin_inff();
+    for (int e = 0; e < 4; ++e) plain &= !__builtin_isunordered(v[2 * e], v[2 * e + 1]);
     if (__builtin_expect(plain, 1)) {
         float q[8];
 #pragma unroll
@@ -144,12 +170,22 @@ __device__ __forceinline__ float norm_rescale(float ss, float eps) {
     return ss + eps < 0x1p-100f ? 0x1p80f : 1.0f;
 }
 
+template <int P>
+__device__ __forceinline__ float squares(const float (&v)[P][8]) {
+    float ss = 0.0f;
+#pragma unroll
+    for (int i = 0; i < P; ++i)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) ss += v[i][e] * v[i][e];
+    return ss;
+}
+
 // WPR waves a row, RPW rows a workgroup, at most P pieces of 8 columns a
 // lane (cols <= 512 * WPR * P).
 template <int MODE, int WPR, int P, int RPW>
 __global__ __launch_bounds__(64 * WPR * RPW) void quant_rows(RowParams p) {
     static_assert(WPR == 1 || RPW == 1, "a barrier is all of one row's");
-    __shared__ float red[3][RPW][WPR];
+    __shared__ float red[4][RPW][WPR];
     const int slot = threadIdx.x / (64 * WPR), t = threadIdx.x % (64 * WPR), wave = t >> 6;
     const bool live = blockIdx.x * RPW + slot < static_cast<unsigned>(p.rows);
     const size_t row = live ? blockIdx.x * RPW + slot : 0;
@@ -169,22 +205,14 @@ __global__ __launch_bounds__(64 * WPR * RPW) void quant_rows(RowParams p) {
             const int at = t + i * 64 * WPR;
             widen8(*reinterpret_cast<const u32x4*>(p.w + (at < n ? at : 0) * 8), w[i]);
         }
-        auto squares = [&](float* at) {
-            float ss = 0.0f;
-#pragma unroll
-            for (int i = 0; i < P; ++i)
-#pragma unroll
-                for (int e = 0; e < 8; ++e) ss += v[i][e] * v[i][e];
-            return row_reduce<WPR, false>(ss, at, wave);
-        };
-        float ss = squares(red[0][slot]);
+        float ss = row_reduce<WPR, false>(squares(v), red[0][slot], wave);
         const float up = norm_rescale(ss, eps);
         if (__builtin_expect(up != 1.0f, 0)) {   // the same for all of the row's threads
 #pragma unroll
             for (int i = 0; i < P; ++i)
 #pragma unroll
                 for (int e = 0; e < 8; ++e) v[i][e] *= up;
-            ss = squares(red[2][slot]);
+            ss = row_reduce<WPR, false>(squares(v), red[2][slot], wave);
             eps = eps * up * up;
         }
         const float f = 1.0f / sqrtf(ss / static_cast<float>(p.cols) + eps);
@@ -193,18 +221,24 @@ __global__ __launch_bounds__(64 * WPR * RPW) void quant_rows(RowParams p) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[i][e] = v[i][e] * f * w[i][e];
     }
-    float a = 0.0f;
+    float a = 0.0f;   // (a piece past the row's end is zeros)
 #pragma unroll
-    for (int i = 0; i < P; ++i)
-        if (t + i * 64 * WPR < n) a = finite_amax(v[i], a);
+    for (int i = 0; i < P; ++i) a = amax8(v[i], a);
     a = row_reduce<WPR, true>(a, red[1][slot], wave);
+    const bool finite = a < __builtin_inff();
+    if (__builtin_expect(!finite, 0)) {   // the same for all of the row's threads
+        a = 0.0f;
+#pragma unroll
+        for (int i = 0; i < P; ++i) a = finite_amax8(v[i], a);
+        a = row_reduce<WPR, true>(a, red[3][slot], wave);
+    }
     const float scale = row_scale(a), r = 1.0f / scale;
     if (live && t == 0) p.scales[row] = scale;
 #pragma unroll
     for (int i = 0; i < P; ++i) {
         const int at = t + i * 64 * WPR;
         if (at < n)
-            *reinterpret_cast<u32x2*>(p.codes + row * p.cols + at * 8) = row_codes(v[i], scale, r);
+            *reinterpret_cast<u32x2*>(p.codes + row * p.cols + at * 8) = row_codes(v[i], scale, r, finite);
     }
 }
 
@@ -212,7 +246,7 @@ __global__ __launch_bounds__(64 * WPR * RPW) void quant_rows(RowParams p) {
 // (from L2), the norm's from the hidden row where there is one.
 template <int MODE>
 __global__ __launch_bounds__(1024) void quant_long_rows(RowParams p) {
-    __shared__ float red[3][16];
+    __shared__ float red[4][16];
     const size_t row = blockIdx.x;
     const int n = p.cols / 8, t = threadIdx.x, wave = t >> 6;
     float f = 1.0f, up = 1.0f, a = 0.0f, v[8], w[8];
@@ -246,14 +280,23 @@ __global__ __launch_bounds__(1024) void quant_long_rows(RowParams p) {
     };
     for (int i = t; i < n; i += 1024) {
         value(i);
-        a = finite_amax(v, a);
+        a = amax8(v, a);
     }
     a = row_reduce<16, true>(a, red[1], wave);
+    const bool finite = a < __builtin_inff();
+    if (!finite) {
+        a = 0.0f;
+        for (int i = t; i < n; i += 1024) {
+            value(i);
+            a = finite_amax8(v, a);
+        }
+        a = row_reduce<16, true>(a, red[3], wave);
+    }
     const float scale = row_scale(a), r = 1.0f / scale;
     if (t == 0) p.scales[row] = scale;
     for (int i = t; i < n; i += 1024) {
         value(i);
-        *reinterpret_cast<u32x2*>(p.codes + row * p.cols + i * 8) = row_codes(v, scale, r);
+        *reinterpret_cast<u32x2*>(p.codes + row * p.cols + i * 8) = row_codes(v, scale, r, finite);
     }
 }
 
@@ -264,15 +307,24 @@ void launch_rows(const RowParams& p, hipStream_t s) {
                        dim3(64 * WPR * RPW), 0, s, p);
 }
 
+// Up to 512 rows a piece a lane, for the shorter chain (512 x 4096 norm 5.4 us;
+// two pieces a lane 5.6); more rows fill the chip, and half as many waves a row
+// wait less at its reductions (8192 x 4096 norm 41.9 / 39.0 us, 8192 x 1024 13.0 /
+// 12.6, 8192 x 2816 35.3 / 31.0).
 template <int MODE>
 bool quant(const RowParams& p, uint64_t stream, std::string* err) {
     hipStream_t s = reinterpret_cast<hipStream_t>(stream);
     const int n = p.cols / 8;   // pieces of a row
+    const bool few = p.rows <= 512;
     if (n <= 64) launch_rows<MODE, 1, 1>(p, s);
-    else if (n <= 128) launch_rows<MODE, 2, 1>(p, s);
-    else if (n <= 256) launch_rows<MODE, 4, 1>(p, s);
-    else if (n <= 512) launch_rows<MODE, 8, 1>(p, s);
-    else if (n <= 1024) launch_rows<MODE, 16, 1>(p, s);
+    else if (few && n <= 128) launch_rows<MODE, 2, 1>(p, s);
+    else if (few && n <= 256) launch_rows<MODE, 4, 1>(p, s);
+    else if (few && n <= 512) launch_rows<MODE, 8, 1>(p, s);
+    else if (few && n <= 1024) launch_rows<MODE, 16, 1>(p, s);
+    else if (n <= 128) launch_rows<MODE, 1, 2>(p, s);
+    else if (n <= 256) launch_rows<MODE, 2, 2>(p, s);
+    else if (n <= 512) launch_rows<MODE, 4, 2>(p, s);
+    else if (n <= 1024) launch_rows<MODE, 8, 2>(p, s);
     else if (n <= 2048) launch_rows<MODE, 16, 2>(p, s);
     else if (n <= 4096) launch_rows<MODE, 16, 4>(p, s);
     else hipLaunchKernelGGL(quant_long_rows<MODE>, dim3(p.rows), dim3(1024), 0, s, p);

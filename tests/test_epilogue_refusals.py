@@ -94,6 +94,8 @@ GEMM = dict(y_ptr=at(4), m=4, n=48, k=64, bias_ptr=at(5), residual_ptr=at(6), ac
     (dict(y_ptr=at(6) - 16), "overlaps"),
     (dict(m=1 << 20, k=1 << 12), "too large"), (dict(n=1 << 20, k=1 << 12), "too large"),
     (dict(m=1 << 16, n=1 << 15), "too large"),
+    (dict(m=(1 << 20) + 1), "too large"), (dict(n=(1 << 22) + 1), "too large"),
+    (dict(m=1 << 20), "no device"), (dict(n=1 << 22), "no device"),
 ])
 def test_products(refused, fp8, change, why):
     a = {"x_ptr": at(0), "w_ptr": at(1), **GEMM, **change}

@@ -198,6 +198,37 @@ def test_silu_mul(gpu_lib, rows, inter):
     check_rows(codes, scales, g / (1 + np.exp(-g)) * u, 2.0 ** -17)
 
 
+@pytest.mark.parametrize("inter", [64, 8192, 33000])
+def test_silu_mul_not_finite(gpu_lib, inter):
+    """Gates whose exponential overflows or vanishes, infinities and NaN: as the
+    formula has them in fp32 (silu(-inf) is NaN), the rest of the row as ever."""
+    import torch
+    rng = np.random.default_rng(inter)
+    g = E.bf16(rng.standard_normal((4, inter)))
+    u = E.bf16(rng.standard_normal((4, inter)))
+    g[0, :6], u[0, :6] = [-200, -100, -89, 100, 200, -88], 1.0
+    g[1, :4], u[1, :4] = [np.inf, -np.inf, np.nan, 2.0], [1.0, 1.0, 1.0, -np.inf]
+    g[2], u[2] = -300, 1.0                    # every value vanishes
+    gu = np.concatenate([g, u], axis=1)
+    bits = (np.ascontiguousarray(gu).view(np.uint32) >> 16).astype(np.uint16)
+    xd = torch.from_numpy(bits.view(np.int16)).view(torch.bfloat16).cuda()
+    o = Outputs(torch, 4, inter)
+    gpu_lib.silu_mul_fp8(xd.data_ptr(), o.c.data_ptr(), o.s.data_ptr(), 4, inter,
+                         torch.cuda.current_stream().cuda_stream)
+    torch.cuda.synchronize()
+    codes, scales = o.get()
+    with np.errstate(over="ignore", invalid="ignore"):
+        d = g.astype(np.float64)
+        v = d / (1 + np.exp(-d)) * u
+    v[0, 0] = v[0, 1] = 0                     # e^100 is past fp32
+    v[2] = 0
+    assert scales[2] == 1 and np.all((codes[2] & 0x7f) == 0)
+    assert (codes[1, 0], codes[1, 3]) == (0x7e, 0xfe) and np.all((codes[1, 1:3] & 0x7f) == 0x7f)
+    v[1, :4] = 0
+    codes[1, :4] = 0
+    check_rows(codes, scales, v, 2.0 ** -17)
+
+
 def test_rows_past_four_gib(gpu_lib):
     """Element offsets above 2^31 (byte offsets above 2^32): the rows written
     near the end are quantised, and only with their own values."""
