@@ -9,10 +9,10 @@
 // at the largest code, NaN as NaN.  The scale keeps fp32, the codes are the
 // one rounding to fewer bits, relative 2^-4, that the 8-bit product is for.
 //
-// Bound by memory for many rows (residual + norm of 8192 x 4096, 235 MB, 39 us =
-// 6.0 TB/s; SwiGLU of 2048 x 14336 29.9 us = 4.9; a large copy moves 5.0) and by a
-// launch and two dependent reductions for few (3.1 us in a graph for one row of
-// 4096).  A row is read once: its values stay in registers between the sum, the
+// Bound by memory for many rows (residual + norm of 8192 x 4096, 235 MB that no
+// cache holds, 46.3 us = 5.1 TB/s; SwiGLU of 2048 x 14336 31.7 us = 4.6; a large copy
+// moves 5.0) and by a launch and two dependent reductions for few (3.1 us in a
+// graph for one row of 4096).  A row is read once: its values stay in registers between the sum, the
 // maximum and the codes.
 #include <algorithm>
 
@@ -307,10 +307,10 @@ void launch_rows(const RowParams& p, hipStream_t s) {
                        dim3(64 * WPR * RPW), 0, s, p);
 }
 
-// Up to 512 rows a piece a lane, for the shorter chain (512 x 4096 norm 5.4 us;
-// two pieces a lane 5.6); more rows fill the chip, and half as many waves a row
-// wait less at its reductions (8192 x 4096 norm 41.9 / 39.0 us, 8192 x 1024 13.0 /
-// 12.6, 8192 x 2816 35.3 / 31.0).
+// Up to 512 rows a piece a lane, for the shorter chain (512 x 4096 norm 5.7 us;
+// two pieces a lane 6.0); more rows fill the chip, and half as many waves a row
+// wait less at its reductions (one piece / two: norm of 8192 x 4096 42.7 / 42.5 us,
+// 8192 x 2816 38.2 / 33.3, 8192 x 1024 15.0 / 14.6, quant of 8192 x 4096 22.0 / 18.9).
 template <int MODE>
 bool quant(const RowParams& p, uint64_t stream, std::string* err) {
     hipStream_t s = reinterpret_cast<hipStream_t>(stream);
