@@ -237,10 +237,11 @@ __global__ __launch_bounds__(64 * WN * WM * WK) void gemm_epi_tile(EpiParams p, 
 // A tile and its modelled time in us: a workgroup alone takes f + g a step (a
 // line of each share), one among others on its CU e + l of that CU's time; the
 // weights come at h TB/s, the outputs go at s.  Fitted to timings of 5066
-// products (M 1 .. 3000, N 64 .. 65536, K 64 .. 14336, either type): within 10% at
-// the median, 20-30% for nine in ten; what it chooses among the tiles, K splits
-// and the 256-row tiles is 1.8% slower than the best of them in the mean (7.5%
-// or less for nine in ten, 22% for 99 in a hundred).
+// products (M 1 .. 3000, N 64 .. 65536, K 64 .. 14336, either type; those of 30 MB of
+// weights or 20 us and more weighed sixfold): within 10% at the median, 20-30% for
+// nine in ten.  What it chooses among the tiles, K splits and the 256-row tiles is
+// 1.7% slower than the best of them in the mean, 2.2% over the large ones (9% or
+// less for nine in ten of those).
 struct Tile {
     int nb, mb, wn, wm, wk, st;
     float f, g, e, l, h, s;
@@ -253,18 +254,18 @@ struct Tile {
     }
 };
 constexpr Tile kTiles[] = {
-    {1, 1, 1, 1, 8, 2, 1.91f, 0.07f, 0.23f, 0.52f, 4.4f, 50.0f},   //  16 rows x  16 tokens
-    {2, 1, 1, 1, 8, 3, 1.95f, 0.42f, 0.00f, 0.76f, 4.1f, 50.0f},   //  32 x  16
-    {2, 1, 2, 1, 4, 3, 1.48f, 0.65f, 1.88f, 0.01f, 4.3f, 2.2f},    //  64 x  16
-    {1, 2, 1, 1, 8, 3, 2.13f, 0.01f, 0.80f, 0.69f, 4.0f, 50.0f},   //  16 x  32
-    {2, 2, 1, 1, 8, 2, 1.92f, 0.43f, 0.00f, 0.99f, 4.0f, 2.0f},    //  32 x  32
-    {1, 2, 4, 1, 2, 4, 1.89f, 0.28f, 0.00f, 0.44f, 4.2f, 2.3f},    //  64 x  32
-    {2, 2, 4, 1, 2, 3, 1.79f, 0.43f, 0.00f, 0.70f, 4.0f, 2.1f},    // 128 x  32
-    {2, 4, 1, 1, 4, 2, 1.63f, 0.54f, 0.00f, 0.73f, 4.0f, 2.4f},    //  32 x  64
-    {1, 4, 4, 1, 2, 4, 1.66f, 0.48f, 0.00f, 0.46f, 4.0f, 3.2f},    //  64 x  64
-    {1, 4, 8, 1, 1, 5, 1.25f, 0.42f, 1.79f, 0.27f, 4.0f, 3.4f},    // 128 x  64
-    {2, 4, 2, 2, 2, 3, 2.01f, 0.67f, 0.00f, 0.73f, 4.0f, 3.0f},    //  64 x 128
-    {2, 4, 4, 2, 1, 5, 2.52f, 0.45f, 1.38f, 0.55f, 4.0f, 3.1f},    // 128 x 128
+    {1, 1, 1, 1, 8, 2, 2.05f, 0.01f, 0.11f, 0.60f, 5.6f, 1.5f},   //  16 rows x  16 tokens
+    {2, 1, 1, 1, 8, 3, 2.05f, 0.52f, 0.00f, 0.95f, 5.0f, 1.5f},   //  32 x  16
+    {2, 1, 2, 1, 4, 3, 1.84f, 0.79f, 0.00f, 0.66f, 5.3f, 1.5f},   //  64 x  16
+    {1, 2, 1, 1, 8, 3, 2.20f, 0.01f, 0.80f, 0.75f, 3.3f, 2.2f},   //  16 x  32
+    {2, 2, 1, 1, 8, 2, 2.06f, 0.47f, 0.00f, 1.20f, 4.2f, 1.5f},   //  32 x  32
+    {1, 2, 4, 1, 2, 4, 1.90f, 0.39f, 0.00f, 0.48f, 5.1f, 1.6f},   //  64 x  32
+    {2, 2, 4, 1, 2, 3, 1.79f, 0.58f, 0.00f, 0.90f, 4.8f, 1.7f},   // 128 x  32
+    {2, 4, 1, 1, 4, 2, 1.93f, 0.53f, 0.03f, 0.82f, 3.2f, 3.5f},   //  32 x  64
+    {1, 4, 4, 1, 2, 4, 1.87f, 0.52f, 0.58f, 0.50f, 3.9f, 5.7f},   //  64 x  64
+    {1, 4, 8, 1, 1, 5, 2.00f, 0.43f, 0.00f, 0.37f, 4.6f, 4.3f},   // 128 x  64
+    {2, 4, 2, 2, 2, 3, 2.17f, 0.65f, 0.59f, 0.83f, 3.4f, 3.9f},   //  64 x 128
+    {2, 4, 4, 2, 1, 5, 2.26f, 0.46f, 0.00f, 0.61f, 4.2f, 2.4f},   // 128 x 128
 };
 constexpr int kTileCount = sizeof(kTiles) / sizeof(kTiles[0]);
 
@@ -277,11 +278,11 @@ double tile_us(const Tile& t, const EpiParams& p, int splits) {
     const int steps = div_up(klines, t.wk), held = std::min(160 * 1024 / t.lds(), 32 / t.waves());
     const double alone = std::max(1.0, std::ceil(q / held)) * (t.f + steps * t.g);
     const double loaded = (q <= 1 ? 1.0 : std::min(std::ceil(q), q + 0.5)) * (t.e + steps * t.l);
-    const double hbm = static_cast<double>(p.N) * p.kb / (t.h * 1e6);
+    const double hbm = t.f + static_cast<double>(p.N) * p.kb / (t.h * 1e6);
     auto p4 = [](double x) { return x * x * x * x; };
     const double sum = splits > 1 ? 4.3 + 4e-6 * splits * p.M * p.N : 0.0;
     const double out = 2e-6 * p.M * p.N / t.s;
-    return 1.7 + std::sqrt(std::sqrt(p4(alone) + p4(loaded) + p4(hbm))) + out + sum;
+    return 1.2 + std::sqrt(std::sqrt(p4(alone) + p4(loaded) + p4(hbm))) + out + sum;
 }
 
 struct Choice {
@@ -353,7 +354,9 @@ float* partials(const EpiParams& p, int splits, uint64_t stream) {
 // not for rows of a single line: up to 96 tokens no product of those timed was
 // clearly faster on them, and the model is too kind to them there (64 x 28672 x
 // 4096 e4m3 33.5 us, 21.6 on a tile).
-double wide_us(const dev::GemmWidePlan& plan) { return 2.0 + plan.us; }
+double wide_us(const EpiParams& p, const dev::GemmWidePlan& plan) {
+    return 2.0 + (p.M <= 256 ? 1.15 : 1.0) * plan.us;
+}
 bool wide_may_do(const EpiParams& p) { return p.kb > 128 && p.M > 96; }
 
 bool run_epi(const EpiParams& p, uint64_t stream, std::string* err) {
@@ -371,7 +374,7 @@ bool run_epi(const EpiParams& p, uint64_t stream, std::string* err) {
         if (many) wide = dev::gemm_epi_wide_plan(p, most);
         Choice tile;
         if (forced != 100) tile = choose_tile(p, most > 1);
-        const bool take_wide = many && (forced == 100 || tile.us < 0 || wide_us(wide) < tile.us);
+        const bool take_wide = many && (forced == 100 || tile.us < 0 || wide_us(p, wide) < tile.us);
         const int splits = take_wide ? wide.splits : tile.splits;
         if (splits > 1 && (part = partials(p, splits, stream)) == nullptr) continue;   // without, then
         if (take_wide) return dev::gemm_epi_wide(p, wide, part, stream, err);
