@@ -449,8 +449,10 @@ int kcmm_decode_logits_bf16_on_stream(uint64_t hidden_ptr, uint64_t norm_w_ptr,
  * such rows with e4m3 weights (one fp32 scale per weight row, as
  * kcmm_gemm_fp8w_bf16_on_stream) on the fp8 matrix cores.  Everything between
  * the inputs and the stores is fp32.  Enqueue only, on the calling thread's
- * current device, to which the pointers and the stream belong; device
- * addresses aligned to 16 bytes; every call may be captured into a HIP graph.
+ * current device, to which the pointers and the stream belong; every call may
+ * be captured into a HIP graph.  Rows that are read or written as codes, x, w,
+ * hidden and residual of the norm start at multiples of 16 bytes; scales, and a
+ * product's y, bias and residual, anywhere an element may.
  * An argument that a call does not take is refused with -1 and a line on
  * stderr before any device work.
  *

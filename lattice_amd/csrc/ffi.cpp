@@ -1226,9 +1226,9 @@ bool apart(const Span& a, const Span& b) {
     return a.at == 0 || b.at == 0 || a.at + a.bytes <= b.at || b.at + b.bytes <= a.at;
 }
 bool same_or_apart(const Span& a, const Span& b) { return a.at == b.at || apart(a, b); }
-bool aligned16(std::initializer_list<uint64_t> ptrs) {
+bool aligned(uint64_t to, std::initializer_list<uint64_t> ptrs) {
     for (uint64_t p : ptrs)
-        if (p % 16 != 0) return false;
+        if (p % to != 0) return false;
     return true;
 }
 
@@ -1275,8 +1275,9 @@ int gemm_epi_call(const char* fn, uint64_t x, uint64_t xscale, uint64_t w, uint6
             *err = "unknown activation " + std::to_string(epi.activation);
             return false;
         }
-        if (!aligned16({x, xscale, w, wscale, y, epi.bias, epi.residual})) {
-            *err = "pointers must be aligned to 16 bytes";
+        if (!aligned(16, {x, w}) || !aligned(4, {xscale, wscale}) ||
+            !aligned(2, {y, epi.bias, epi.residual})) {
+            *err = "x and w must be aligned to 16 bytes, the others to their elements";
             return false;
         }
         const Span out{y, 2 * M * N};
@@ -1319,8 +1320,8 @@ int kcmm_add_rmsnorm_fp8_on_stream(uint64_t x, uint64_t residual, uint64_t w, ui
             *err = "eps must be finite and not negative";
             return false;
         }
-        if (!aligned16({x, residual, w, hidden, codes, scales})) {
-            *err = "pointers must be aligned to 16 bytes";
+        if (!aligned(16, {x, residual, w, hidden, codes}) || !aligned(4, {scales})) {
+            *err = "pointers must be aligned to 16 bytes (scales to 4)";
             return false;
         }
         const uint64_t e = static_cast<uint64_t>(rows) * hidden_size;
@@ -1345,8 +1346,8 @@ bool quant_args_ok(uint64_t x, uint64_t x_cols, uint64_t codes, uint64_t scales,
         return false;
     }
     if (!rows_ok(rows, cols, err)) return false;
-    if (!aligned16({x, codes, scales})) {
-        *err = "pointers must be aligned to 16 bytes";
+    if (!aligned(16, {x, codes}) || !aligned(4, {scales})) {
+        *err = "pointers must be aligned to 16 bytes (scales to 4)";
         return false;
     }
     const Span in{x, 2 * rows * x_cols}, c{codes, static_cast<uint64_t>(rows) * cols},

@@ -67,8 +67,9 @@ __device__ __forceinline__ void activate_all(float (&z)[R], int act) {
     }
 }
 
-// Eight bf16 of a row of Y or R: rows start at any even address when N is odd,
-// and global memory takes vector accesses there.
+// Eight bf16 of a row of Y or R, of the bias, four of the scales: they start at any
+// address that an element may have (rows do where N is odd), and global memory
+// takes vector accesses there.
 typedef uint32_t u32x4_rows __attribute__((ext_vector_type(4), aligned(2)));
 typedef float f32x4_rows __attribute__((ext_vector_type(4), aligned(4)));
 
@@ -101,12 +102,12 @@ __device__ __forceinline__ EpiCols epi_cols(const EpiParams& p, int n) {
         if constexpr (F8) {
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                const f32x4 w = *reinterpret_cast<const f32x4*>(p.ws + n + 4 * h);
+                const f32x4 w = *reinterpret_cast<const f32x4_rows*>(p.ws + n + 4 * h);
 #pragma unroll
                 for (int r = 0; r < 4; ++r) c.ws[4 * h + r] = w[r];
             }
         }
-        if (p.bias != nullptr) c.bias = *reinterpret_cast<const u32x4*>(p.bias + n);
+        if (p.bias != nullptr) c.bias = *reinterpret_cast<const u32x4_rows*>(p.bias + n);
     } else {   // the row's end: the last column again, so that no load waits for another
         if constexpr (F8) {
 #pragma unroll

@@ -45,7 +45,8 @@ NORM = dict(x_ptr=at(0), residual_ptr=at(1), w_ptr=at(2), hidden_ptr=at(3), code
     (dict(hidden_size=(1 << 24) + 8), "multiple of 8"),
     (dict(eps=-1e-6), "eps"), (dict(eps=float("nan")), "eps"), (dict(eps=float("inf")), "eps"),
     (dict(x_ptr=at(0) + 8), "aligned"), (dict(codes_ptr=at(4) + 8), "aligned"),
-    (dict(w_ptr=at(2) + 2), "aligned"), (dict(scales_ptr=at(5) + 4), "aligned"),
+    (dict(w_ptr=at(2) + 2), "aligned"), (dict(scales_ptr=at(5) + 2), "aligned"),
+    (dict(scales_ptr=at(5) + 4), "no device"),
     (dict(hidden_ptr=at(0) + 16), "overlaps"), (dict(hidden_ptr=at(1) + 128), "overlaps"),
     (dict(hidden_ptr=at(2)), "overlaps"), (dict(codes_ptr=at(0)), "overlaps"),
     (dict(codes_ptr=at(1) + 256), "overlaps"), (dict(codes_ptr=at(3) + 496), "overlaps"),
@@ -87,8 +88,9 @@ GEMM = dict(y_ptr=at(4), m=4, n=48, k=64, bias_ptr=at(5), residual_ptr=at(6), ac
     (dict(k=12), "multiple of"), (dict(k=(1 << 24) + 16), "2^24"),
     (dict(activation=-1), "activation"), (dict(activation=5), "activation"),
     (dict(x_ptr=at(0) + 8), "aligned"), (dict(w_ptr=at(1) + 2), "aligned"),
-    (dict(y_ptr=at(4) + 8), "aligned"), (dict(bias_ptr=at(5) + 2), "aligned"),
-    (dict(residual_ptr=at(6) + 2), "aligned"),
+    (dict(y_ptr=at(4) + 1), "aligned"), (dict(bias_ptr=at(5) + 1), "aligned"),
+    (dict(residual_ptr=at(6) + 1), "aligned"),
+    (dict(y_ptr=at(4) + 2, bias_ptr=at(5) + 2, residual_ptr=at(6) + 2), "no device"),
     (dict(y_ptr=at(0)), "overlaps"), (dict(y_ptr=at(1) + 16), "overlaps"),
     (dict(y_ptr=at(5)), "overlaps"), (dict(residual_ptr=at(4) + 16), "overlaps"),
     (dict(y_ptr=at(6) - 16), "overlaps"),
@@ -106,7 +108,9 @@ def test_products(refused, fp8, change, why):
 
 @pytest.mark.parametrize("change,why", [(dict(xscale_ptr=0), "null"), (dict(wscale_ptr=0), "null"),
                                         (dict(k=8), "multiple of 16"),
-                                        (dict(xscale_ptr=at(2) + 4), "aligned"),
+                                        (dict(xscale_ptr=at(2) + 2), "aligned"),
+                                        (dict(wscale_ptr=at(3) + 1), "aligned"),
+                                        (dict(xscale_ptr=at(2) + 4, wscale_ptr=at(3) + 4), "no device"),
                                         (dict(y_ptr=at(2)), "overlaps"),
                                         (dict(y_ptr=at(3) + 16), "overlaps")])
 def test_fp8_products(refused, change, why):

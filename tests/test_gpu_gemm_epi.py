@@ -178,6 +178,36 @@ def test_residual_in_place(gpu_lib, m, n, k, fp8):
 
 
 @pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("m,n,k", [(3, 200, 512), (70, 131, 640), (300, 1000, 512), (140, 96, 4096)])
+def test_slices_of_larger_buffers(gpu_lib, m, n, k, fp8):
+    """Some tokens and some weight rows of larger buffers: y, residual, bias and
+    scales then start at an element, not at 16 bytes; nothing else is written."""
+    import torch
+    t0, n0 = 5, 3                                   # what lies before them
+    a = inputs(np.random.default_rng(m + n), m + t0, n + n0, k, fp8, True, True)
+    bd, rd = dev16(torch, a["bias"]), dev16(torch, a["residual"][:, n0:])
+    y = torch.full(((m + t0) * n + GUARD,), 7.0, dtype=torch.bfloat16, device="cuda")
+    kw = dict(bias_ptr=bd.data_ptr() + 2 * n0, residual_ptr=rd.data_ptr() + 2 * t0 * n,
+              activation=ACT_SILU, stream_ptr=torch.cuda.current_stream().cuda_stream)
+    eb = 1 if fp8 else 2
+    if fp8:
+        xd, wd = (torch.from_numpy(codes_of(a[v])).cuda() for v in ("x", "w"))
+        xs, ws = (torch.from_numpy(E.f32(a[v])).cuda() for v in ("xs", "ws"))
+        gpu_lib.gemm_fp8(xd.data_ptr() + t0 * k, xs.data_ptr() + 4 * t0, wd.data_ptr() + n0 * k,
+                         ws.data_ptr() + 4 * n0, y.data_ptr() + 2 * t0 * n, m, n, k, **kw)
+    else:
+        xd, wd = dev16(torch, a["x"]), dev16(torch, a["w"])
+        gpu_lib.gemm_bf16_epi(xd.data_ptr() + eb * t0 * k, wd.data_ptr() + eb * n0 * k,
+                              y.data_ptr() + 2 * t0 * n, m, n, k, **kw)
+    torch.cuda.synchronize()
+    assert bool((y[:t0 * n] == 7.0).all()) and bool((y[(m + t0) * n:] == 7.0).all())
+    got = host16(y[t0 * n:(m + t0) * n]).reshape(m, n)
+    xs, ws = (a["xs"][t0:], a["ws"][n0:]) if fp8 else (None, None)
+    check_product(got, a["x"][t0:], a["w"][n0:], xs, ws, a["bias"][n0:], a["residual"][t0:, n0:],
+                  ACT_SILU)
+
+
+@pytest.mark.parametrize("fp8", [False, True])
 @pytest.mark.parametrize("m,n,k", [(2, 100, 272), (50, 100, 272), (300, 300, 272)])
 def test_not_finite_stays_in_its_row_and_column(gpu_lib, m, n, k, fp8):
     """A NaN in one token reaches that token's outputs only, one in a weight
