@@ -11,9 +11,11 @@
 //
 // This file: the tile kernel, for up to a few hundred tokens, and the choice of
 // a tile; many tokens run the 256-row tiles of gemm_epi_wide.hip.  A product of
-// few tokens is bound by the weights' way from HBM, one of some tens by what a
-// CU can take in (a tile of R weight rows by T tokens loads R + T rows for R * T
-// outputs; about 23 bytes a cycle and CU were reached), so:
+// few tokens is bound by the weights' way from HBM, one of some hundreds by a
+// step's chain: a tile of R weight rows by T tokens loads R + T rows for R * T
+// outputs, and its waves meet once a line.  The 128 x 128 tile takes 0.60 us a line
+// (777 x 4096 x 4096, either type); without the matrix instructions 0.52, with the
+// loads and barriers alone 0.43, those with every line in L2 0.30.  So:
 //  * both operands reach LDS by direct loads, 128-byte lines of 8 rows an
 //    instruction, in a ring that keeps 64-128 KiB a CU in flight; fragments
 //    straight from memory to registers, 16 rows of 64 bytes an instruction,
@@ -240,7 +242,7 @@ __global__ __launch_bounds__(64 * WN * WM * WK) void gemm_epi_tile(EpiParams p, 
 // products (M 1 .. 3000, N 64 .. 65536, K 64 .. 14336, either type; those of 30 MB of
 // weights or 20 us and more weighed sixfold): within 10% at the median, 20-30% for
 // nine in ten.  What it chooses among the tiles, K splits and the 256-row tiles is
-// 1.7% slower than the best of them in the mean, 2.2% over the large ones (9% or
+// 1.6% slower than the best of them in the mean, 2.1% over the large ones (9% or
 // less for nine in ten of those).
 struct Tile {
     int nb, mb, wn, wm, wk, st;
@@ -254,18 +256,18 @@ struct Tile {
     }
 };
 constexpr Tile kTiles[] = {
-    {1, 1, 1, 1, 8, 2, 2.05f, 0.01f, 0.11f, 0.60f, 5.6f, 1.5f},   //  16 rows x  16 tokens
-    {2, 1, 1, 1, 8, 3, 2.05f, 0.52f, 0.00f, 0.95f, 5.0f, 1.5f},   //  32 x  16
-    {2, 1, 2, 1, 4, 3, 1.84f, 0.79f, 0.00f, 0.66f, 5.3f, 1.5f},   //  64 x  16
-    {1, 2, 1, 1, 8, 3, 2.20f, 0.01f, 0.80f, 0.75f, 3.3f, 2.2f},   //  16 x  32
-    {2, 2, 1, 1, 8, 2, 2.06f, 0.47f, 0.00f, 1.20f, 4.2f, 1.5f},   //  32 x  32
-    {1, 2, 4, 1, 2, 4, 1.90f, 0.39f, 0.00f, 0.48f, 5.1f, 1.6f},   //  64 x  32
-    {2, 2, 4, 1, 2, 3, 1.79f, 0.58f, 0.00f, 0.90f, 4.8f, 1.7f},   // 128 x  32
-    {2, 4, 1, 1, 4, 2, 1.93f, 0.53f, 0.03f, 0.82f, 3.2f, 3.5f},   //  32 x  64
-    {1, 4, 4, 1, 2, 4, 1.87f, 0.52f, 0.58f, 0.50f, 3.9f, 5.7f},   //  64 x  64
-    {1, 4, 8, 1, 1, 5, 2.00f, 0.43f, 0.00f, 0.37f, 4.6f, 4.3f},   // 128 x  64
-    {2, 4, 2, 2, 2, 3, 2.17f, 0.65f, 0.59f, 0.83f, 3.4f, 3.9f},   //  64 x 128
-    {2, 4, 4, 2, 1, 5, 2.26f, 0.46f, 0.00f, 0.61f, 4.2f, 2.4f},   // 128 x 128
+    {1, 1, 1, 1, 8, 2, 2.00f, 0.11f, 0.03f, 0.61f, 5.5f, 1.5f},   //  16 rows x  16 tokens
+    {2, 1, 1, 1, 8, 3, 2.00f, 0.59f, 0.00f, 0.97f, 5.0f, 1.5f},   //  32 x  16
+    {2, 1, 2, 1, 4, 3, 1.82f, 0.87f, 0.00f, 0.44f, 5.2f, 5.1f},   //  64 x  16
+    {1, 2, 1, 1, 8, 3, 2.20f, 0.01f, 0.99f, 0.75f, 3.3f, 80.0f},   //  16 x  32
+    {2, 2, 1, 1, 8, 2, 2.02f, 0.55f, 0.00f, 1.22f, 4.1f, 1.5f},   //  32 x  32
+    {1, 2, 4, 1, 2, 4, 1.94f, 0.44f, 0.26f, 0.43f, 4.9f, 3.1f},   //  64 x  32
+    {2, 2, 4, 1, 2, 3, 1.76f, 0.71f, 0.00f, 0.86f, 4.4f, 2.4f},   // 128 x  32
+    {2, 4, 1, 1, 4, 2, 1.96f, 0.57f, 0.52f, 0.80f, 3.1f, 80.0f},   //  32 x  64
+    {1, 4, 4, 1, 2, 4, 1.93f, 0.56f, 1.06f, 0.49f, 3.7f, 51.1f},   //  64 x  64
+    {1, 4, 8, 1, 1, 5, 2.07f, 0.45f, 1.19f, 0.38f, 4.0f, 7.3f},   // 128 x  64
+    {2, 4, 2, 2, 2, 3, 2.18f, 0.67f, 1.45f, 0.84f, 3.1f, 7.4f},   //  64 x 128
+    {2, 4, 4, 2, 1, 5, 2.53f, 0.54f, 1.26f, 0.58f, 3.7f, 3.7f},   // 128 x 128
 };
 constexpr int kTileCount = sizeof(kTiles) / sizeof(kTiles[0]);
 
@@ -280,7 +282,7 @@ double tile_us(const Tile& t, const EpiParams& p, int splits) {
     const double loaded = (q <= 1 ? 1.0 : std::min(std::ceil(q), q + 0.5)) * (t.e + steps * t.l);
     const double hbm = t.f + static_cast<double>(p.N) * p.kb / (t.h * 1e6);
     auto p4 = [](double x) { return x * x * x * x; };
-    const double sum = splits > 1 ? 4.3 + 4e-6 * splits * p.M * p.N : 0.0;
+    const double sum = splits > 1 ? 4.0 + 2.4e-6 * splits * p.M * p.N : 0.0;
     const double out = 2e-6 * p.M * p.N / t.s;
     return 1.2 + std::sqrt(std::sqrt(p4(alone) + p4(loaded) + p4(hbm))) + out + sum;
 }
@@ -350,12 +352,12 @@ float* partials(const EpiParams& p, int splits, uint64_t stream) {
     return static_cast<float*>(part);
 }
 
-// Modelled time of the 256-row tiles.  They are looked at above 96 tokens and
-// not for rows of a single line: up to 96 tokens no product of those timed was
-// clearly faster on them, and the model is too kind to them there (64 x 28672 x
-// 4096 e4m3 33.5 us, 21.6 on a tile).
+// Modelled time of the 256-row tiles: their plan's, raised where few tokens make
+// the plan too kind (28672 x 4096 e4m3 of 104 tokens: 35.2 us there, 26.8 on the
+// 128 x 128 tile; 44910 x 448 bf16 of 128 tokens: 16.2 there, 22.2 on tiles).  They
+// are looked at above 96 tokens and not for rows of a single line.
 double wide_us(const EpiParams& p, const dev::GemmWidePlan& plan) {
-    return 2.0 + (p.M <= 256 ? 1.15 : 1.0) * plan.us;
+    return 2.0 + (p.M <= 128 ? 1.4 : p.M <= 256 ? 1.15 : 1.0) * plan.us;
 }
 bool wide_may_do(const EpiParams& p) { return p.kb > 128 && p.M > 96; }
 

@@ -366,6 +366,64 @@ def test_mlp_block_in_a_graph(gpu_lib, m):
         assert torch.equal(got.view(torch.int16), b.y.view(torch.int16))
 
 
+@pytest.mark.parametrize("tile", [9, 100])
+def test_captures_split_nothing(gpu_lib, tunables, tile):
+    """A product that an eager call splits over K (with partials and a second
+    kernel) is one kernel in a graph, also on a stream whose buffer is there."""
+    import torch
+    from tests.test_gpu_graph import _captured_kernels
+    tunables.setenv("KCMM_EPI_TILE", str(tile))
+    if tile == 9:
+        tunables.setenv("KCMM_GEMM_SPLITS", "4")
+    m, n, k = 130, 512, 4096
+    x, w = (torch.randn(r, k, device="cuda").bfloat16() for r in (m, n))
+    y = torch.empty(m, n, dtype=torch.bfloat16, device="cuda")
+
+    def run(st):
+        gpu_lib.gemm_bf16_epi(x.data_ptr(), w.data_ptr(), y.data_ptr(), m, n, k, stream_ptr=st)
+
+    torch.cuda.synchronize()
+    assert len(_captured_kernels(run)) == 1
+    assert len(_captured_kernels(run, warm=run)) == 1
+
+
+def test_calls_from_two_threads(gpu_lib, tunables):
+    """Split products from two threads at once, on streams of their own and on
+    one stream: each has its own partials."""
+    import concurrent.futures
+    import torch
+    tunables.setenv("KCMM_EPI_TILE", "9")
+    tunables.setenv("KCMM_GEMM_SPLITS", "4")
+    m, n, k = 64, 1024, 4096
+    data = []
+    for i in range(2):
+        x, w = (torch.randn(r, k, device="cuda").bfloat16() for r in (m, n))
+        data.append((x, w, torch.empty(m, n, dtype=torch.bfloat16, device="cuda")))
+    want = []
+    for x, w, y in data:
+        gpu_lib.gemm_bf16_epi(x.data_ptr(), w.data_ptr(), y.data_ptr(), m, n, k)
+        torch.cuda.synchronize()
+        want.append(y.clone())
+        y.zero_()
+    own = [torch.cuda.Stream() for _ in range(2)]
+
+    def work(i, stream):
+        x, w, y = data[i]
+        for _ in range(50):
+            gpu_lib.gemm_bf16_epi(x.data_ptr(), w.data_ptr(), y.data_ptr(), m, n, k,
+                                  stream_ptr=stream.cuda_stream)
+
+    for streams in (own, [own[0], own[0]]):
+        torch.cuda.synchronize()
+        with concurrent.futures.ThreadPoolExecutor(2) as ex:
+            for f in [ex.submit(work, i, streams[i]) for i in range(2)]:
+                f.result()
+        torch.cuda.synchronize()
+        for (x, w, y), v in zip(data, want):
+            assert torch.equal(y.view(torch.int16), v.view(torch.int16))
+            y.zero_()
+
+
 def test_two_graphs_of_one_stream_at_once(gpu_lib):
     """Two captures from the same stream, replayed on two streams at the same
     time: nothing that they share."""
