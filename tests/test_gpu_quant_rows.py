@@ -229,6 +229,25 @@ def test_silu_mul_not_finite(gpu_lib, inter):
     check_rows(codes, scales, v, 2.0 ** -17)
 
 
+def test_silu_mul_at_the_exponent_s_end(gpu_lib):
+    """Gates whose 1 / (1 + e^-g) is below the normal numbers while g times it is
+    not, with ups that make values of some size of it.  REL as above: |g| < 89 in
+    the place of 64, 89 log2(e) + 5 < 135 roundings of 2^-24, less than 2^-16."""
+    import torch
+    rng = np.random.default_rng(12)
+    inter = 512
+    g = E.bf16(rng.uniform(-88.5, -85, (2, inter)))
+    u = E.bf16(rng.standard_normal((2, inter)) * 1e36)
+    xd = dev16(torch, np.concatenate([g, u], axis=1))
+    o = Outputs(torch, 2, inter)
+    gpu_lib.silu_mul_fp8(xd.data_ptr(), o.c.data_ptr(), o.s.data_ptr(), 2, inter,
+                         torch.cuda.current_stream().cuda_stream)
+    torch.cuda.synchronize()
+    d = g.astype(np.float64)
+    codes, scales = o.get()
+    check_rows(codes, scales, d / (1 + np.exp(-d)) * u, 2.0 ** -16)
+
+
 def test_rows_past_four_gib(gpu_lib):
     """Element offsets above 2^31 (byte offsets above 2^32): the rows written
     near the end are quantised, and only with their own values."""
