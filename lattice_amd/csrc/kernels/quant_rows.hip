@@ -47,8 +47,8 @@ __device__ __forceinline__ void widen8(const u32x4& v, float (&f)[8]) {
 // silu(g) u of 8 columns.  e^-g is 2^hi by the hardware's exp2, with what the
 // rounding of hi leaves out as a factor; the quotient by its reciprocal, each with
 // one step of its residual, so that both are rounded as if exact but for rare
-// last places.  |hi| >= 128 (an infinite or vanishing e^-g, infinities, NaN) takes
-// the library's functions.  (2048 x 14336: 37.7 us with those everywhere, 33.9 with
+// last places.  |hi| >= 126 (an e^-g or a reciprocal outside the normal numbers,
+// which the instructions take for 0, infinities, NaN) takes the library's functions.  (2048 x 14336: 37.7 us with those everywhere, 33.9 with
 // the guards on every element; with the reciprocal alone three times the wrong
 // codes.)
 __device__ __forceinline__ void silu_mul8(float (&g)[8], const float (&u)[8]) {
@@ -64,7 +64,7 @@ __device__ __forceinline__ void silu_mul8(float (&g)[8], const float (&u)[8]) {
         const float r = fmaf(fmaf(-s, r0, 1.0f), r0, r0);
         const float q = g[e] * r;
         v[e] = fmaf(fmaf(-s, q, g[e]), r, q) * u[e];
-        in &= fabsf(hi) < 128.0f;
+        in &= fabsf(hi) < 126.0f;
     }
     if (__builtin_expect(!in, 0)) {
 #pragma unroll
