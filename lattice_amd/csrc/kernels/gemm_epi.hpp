@@ -39,13 +39,20 @@ __device__ __forceinline__ float gelu_erf(float z) {
     return z * (z >= 0.0f ? fmaf(-0.5f, c, 1.0f) : 0.5f * c);
 }
 
+// z / (1 + e^-t), both parts 2^-8 of themselves: so the reciprocal is a normal
+// number (the hardware's is 0 below) until z = t leaves nothing of it in bf16.
+__device__ __forceinline__ float z_sigmoid(float z, float t) {
+    return 0x1p-8f * z *
+           __builtin_amdgcn_rcpf(0x1p-8f + __builtin_amdgcn_exp2f(fmaf(-1.44269504f, t, -8.0f)));
+}
+
 __device__ __forceinline__ float activate(float z, int act) {
     switch (act) {
         case kActRelu: return z < 0.0f ? 0.0f : z;
         case kActGelu: return gelu_erf(z);
         case kActGeluTanh:   // z sigmoid(2 u): the tanh form without its cancellation
-            return z * __builtin_amdgcn_rcpf(1.0f + __expf(-1.59576912f * z * fmaf(0.044715f * z, z, 1.0f)));
-        case kActSilu: return z * __builtin_amdgcn_rcpf(1.0f + __expf(-z));
+            return z_sigmoid(z, 1.59576912f * z * fmaf(0.044715f * z, z, 1.0f));
+        case kActSilu: return z_sigmoid(z, z);
         default: return z;
     }
 }

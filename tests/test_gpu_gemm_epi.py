@@ -366,6 +366,24 @@ def test_mlp_block_in_a_graph(gpu_lib, m):
         assert torch.equal(got.view(torch.int16), b.y.view(torch.int16))
 
 
+@pytest.mark.parametrize("act", [ACT_SILU, ACT_GELU_TANH])
+def test_activation_at_the_exponent_s_end(gpu_lib, act):
+    """z sigmoid(t) where 1 / (1 + e^-t) is below the normal numbers and y is not:
+    off by the store's half step and by t's roundings, at most five of 89 * 2^-24
+    with log2(e)'s, and eight more of 2^-24: less than 500 * 2^-24 < 2^-15."""
+    import torch
+    rng = np.random.default_rng(act)
+    z = E.bf16(rng.uniform(-88.5, -85, 64) if act == ACT_SILU else rng.uniform(-10.06, -9.75, 64)).astype(np.float64)
+    t = z if act == ACT_SILU else np.sqrt(8 / np.pi) * (z + 0.044715 * z ** 3)
+    assert t.min() > -89 and t.max() < -80
+    want = z / (1 + np.exp(-t))
+    assert np.abs(want).min() > 2.0 ** -126
+    x, w = np.zeros((64, 16)), np.zeros((24, 16))
+    x[:, 3], w[:, 3] = z, 1
+    got = call(torch, gpu_lib, x, w, None, None, None, None, act)
+    assert np.all(np.abs(got - want[:, None]) <= (E.BF16_HALF + 2.0 ** -15) * np.abs(want[:, None]))
+
+
 @pytest.mark.parametrize("tile", [9, 100])
 def test_captures_split_nothing(gpu_lib, tunables, tile):
     """A product that an eager call splits over K (with partials and a second
