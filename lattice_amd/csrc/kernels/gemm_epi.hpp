@@ -25,18 +25,24 @@ constexpr int kEpiSlot = 10;   // the stream workspace of their K splits
 
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 
-// erfc(a) e^(a^2) for a >= 0 as a polynomial in t = 1 / (1 + 0.3275911 a)
-// (Abramowitz and Stegun 7.1.26): erfc is off by at most 1.5e-7, a bf16
-// rounding of the activation by 2^-9 of it.
+// z Phi(z).  erfc(a) e^(a^2) for a = |z| / sqrt(2) is a polynomial in t = 1 / (1 +
+// 0.6 a), fitted for the least largest relative error over 0 <= a <= 10.6 (2^-21.6;
+// with the roundings 2^-19 down to z = -8 and 2^-17 at -14, where e^(-z^2 / 2) has the
+// most of them; a bf16 store's is 2^-8).  A fit of erf alone, of the same absolute
+// error, has no bits of the lower tail: Abramowitz and Stegun 7.1.26 was 0.4% off at
+// z = -6 and 3.7% at -13.  The exponential is 2^8 of itself, so that it is a normal
+// number (the hardware's is 0 below) until nothing of the result is left in bf16.
 __device__ __forceinline__ float gelu_erf(float z) {
-    const float a = fabsf(z) * 0.70710678f;
-    const float t = __builtin_amdgcn_rcpf(fmaf(0.3275911f, a, 1.0f));
-    float c = fmaf(1.061405429f, t, -1.453152027f);
-    c = fmaf(c, t, 1.421413741f);
-    c = fmaf(c, t, -0.284496736f);
-    c = fmaf(c, t, 0.254829592f) * t * __expf(-a * a);
-    // z Phi(z): one less the upper tail, or the lower tail itself
-    return z * (z >= 0.0f ? fmaf(-0.5f, c, 1.0f) : 0.5f * c);
+    const float t = __builtin_amdgcn_rcpf(fmaf(0.42426407f, fabsf(z), 1.0f));
+    float c = fmaf(-0.0920885652f, t, 0.411972642f);
+    c = fmaf(c, t, -0.64450407f);
+    c = fmaf(c, t, 0.283816934f);
+    c = fmaf(c, t, 0.0733853355f);
+    c = fmaf(c, t, 0.291609466f);
+    c = fmaf(c, t, 0.337247759f);
+    c = fmaf(c, t, 0.338560164f) * t * __builtin_amdgcn_exp2f(fmaf(z * z, -0.72134752f, 8.0f));
+    // one less the upper tail, or the lower tail itself
+    return z >= 0.0f ? z * fmaf(-0x1p-9f, c, 1.0f) : z * c * 0x1p-9f;
 }
 
 // z / (1 + e^-t), both parts 2^-8 of themselves: so the reciprocal is a normal

@@ -1,0 +1,59 @@
+"""The ends of the epilogue products' ranges on the GPU: activations whose
+results are far below their arguments."""
+import numpy as np
+import pytest
+
+from lattice_amd.bindings import ACT_GELU
+from tests import e4m3 as E
+from tests.test_gpu_gemm_epi import call
+
+pytestmark = pytest.mark.gpu
+
+
+def activated(torch, lib, z, act):
+    """act of the bf16 values z by a product whose other operand is 1."""
+    x, w = np.zeros((len(z), 16)), np.zeros((24, 16))
+    x[:, 3], w[:, 3] = z, 1
+    got = call(torch, lib, x, w, act=act)
+    assert np.array_equal(got, np.broadcast_to(got[:, :1], got.shape))
+    return got[:, 0].astype(np.float64)
+
+
+def store_and_roundings(y):
+    """Half a step of bf16 (2^-134 below the normal numbers), and 2^-15 of y: an
+    exponent of at most 104 = 150 ln 2 whose value four roundings of 2^-24 went into,
+    with ten more of y's own, is 426 * 2^-24 off, and a fit 2^-21."""
+    return np.maximum(E.BF16_HALF * np.abs(y), 2.0 ** -134) + 2.0 ** -15 * np.abs(y)
+
+
+def test_gelu_of_the_lower_tail(gpu_lib):
+    """z Phi(z) for z of -2 to where nothing is left of it, against fp64 relative
+    to the result: 1 - erf has none of its bits there."""
+    import torch
+    z = np.unique(E.bf16(np.linspace(-14.5, -2, 1500))).astype(np.float64)
+    y = E.activation(z, 2)
+    assert np.abs(y).min() < 2.0 ** -134 and np.abs(y).max() > 0.04
+    got = activated(torch, gpu_lib, z, ACT_GELU)
+    assert np.all(np.abs(got - y) <= store_and_roundings(y))
+
+
+def test_gelu_everywhere_else(gpu_lib):
+    import torch
+    z = np.unique(E.bf16(np.concatenate([np.linspace(-2, 6, 1500), [-1e-30, -1e-5, 0, 1e-36, 1e-9,
+                                                                   30, 1e4, 1e30, 3e38]])))
+    y = E.activation(z.astype(np.float64), 2)
+    got = activated(torch, gpu_lib, z, ACT_GELU)
+    assert np.all(np.abs(got - y) <= store_and_roundings(y))
+
+
+def test_gelu_of_infinities(gpu_lib):
+    """inf Phi(inf) = inf; -inf Phi(-inf) is the product of an infinity and 0."""
+    import torch
+    bias = torch.tensor([float("inf"), float("-inf"), float("nan"), 1.0], device="cuda").bfloat16()
+    x, w = (torch.zeros(n, 16, device="cuda").bfloat16() for n in (3, 4))
+    y = torch.zeros(3, 4, device="cuda").bfloat16()
+    gpu_lib.gemm_bf16_epi(x.data_ptr(), w.data_ptr(), y.data_ptr(), 3, 4, 16, bias_ptr=bias.data_ptr(),
+                          activation=ACT_GELU, stream_ptr=torch.cuda.current_stream().cuda_stream)
+    torch.cuda.synchronize()
+    got = y.float().cpu().numpy()
+    assert np.all(got[:, 0] == np.inf) and np.all(np.isnan(got[:, 1:3])) and np.all(got[:, 3] == 0.83984375)
