@@ -45,11 +45,13 @@ __device__ __forceinline__ float gelu_erf(float z) {
     return z >= 0.0f ? z * fmaf(-0x1p-9f, c, 1.0f) : z * c * 0x1p-9f;
 }
 
-// z / (1 + e^-t), both parts 2^-8 of themselves: so the reciprocal is a normal
-// number (the hardware's is 0 below) until z = t leaves nothing of it in bf16.
+// z / (1 + e^-t), the sum 2^-15 of itself: so its reciprocal is a normal number (the
+// hardware's is 0 below) as far as t = -97.7, where z = t is the last to leave anything
+// in bf16 (less than half of its least step).  The 2^-15 are taken off in two parts, of
+// z and of the reciprocal, so that neither's product is past fp32.
 __device__ __forceinline__ float z_sigmoid(float z, float t) {
-    return 0x1p-8f * z *
-           __builtin_amdgcn_rcpf(0x1p-8f + __builtin_amdgcn_exp2f(fmaf(-1.44269504f, t, -8.0f)));
+    const float r = __builtin_amdgcn_rcpf(0x1p-15f + __builtin_amdgcn_exp2f(fmaf(-1.44269504f, t, -15.0f)));
+    return 0x1p-8f * z * (0x1p-7f * r);
 }
 
 __device__ __forceinline__ float activate(float z, int act) {

@@ -3,7 +3,7 @@ results are far below their arguments."""
 import numpy as np
 import pytest
 
-from lattice_amd.bindings import ACT_GELU
+from lattice_amd.bindings import ACT_GELU, ACT_GELU_TANH, ACT_SILU
 from tests import e4m3 as E
 from tests.test_gpu_gemm_epi import call
 
@@ -57,3 +57,17 @@ def test_gelu_of_infinities(gpu_lib):
     torch.cuda.synchronize()
     got = y.float().cpu().numpy()
     assert np.all(got[:, 0] == np.inf) and np.all(np.isnan(got[:, 1:3])) and np.all(got[:, 3] == 0.83984375)
+
+
+@pytest.mark.parametrize("act,low,high", [(ACT_SILU, -99, -86), (ACT_GELU_TANH, -10.45, -9.8)])
+def test_results_below_the_normal_numbers(gpu_lib, act, low, high):
+    """z sigmoid(t) of less than 2^-126: bf16 has it down to 2^-133.  Its t is off by
+    at most five roundings of 99 * 2^-24, so y by 2^-15 with eight more of its own."""
+    import torch
+    z = np.unique(E.bf16(np.linspace(low, high, 600))).astype(np.float64)
+    t = z if act == ACT_SILU else np.sqrt(8 / np.pi) * (z + 0.044715 * z ** 3)
+    y = z / (1 + np.exp(-t))
+    assert t.min() > -99.5 and np.abs(y).min() < 2.0 ** -132 and np.abs(y).max() > 2.0 ** -126
+    got = activated(torch, gpu_lib, z, act)
+    assert np.all(np.abs(got - y) <= np.maximum(E.BF16_HALF * np.abs(y), 2.0 ** -134) +
+                  2.0 ** -15 * np.abs(y))
