@@ -33,7 +33,7 @@ enum class Tun {
     kGemmWaves,     // KCMM_GEMM_WAVES (waves per workgroup of unsplit plain / SwiGLU products)
     kGemmHelpers,   // KCMM_GEMM_HELPERS (0: split products without activation-staging helper waves)
     kEpiTile,       // KCMM_EPI_TILE (products with an epilogue: 1.. that tile of the tile
-                    // kernel with KCMM_GEMM_SPLITS K splits, 100 the 256-row tiles)
+                    // kernel, 100 the 256-row tiles; KCMM_GEMM_SPLITS K splits)
     kCount
 };
 // true and *value = atoi(variable) when the variable is set.
@@ -191,7 +191,8 @@ struct GemmWideArgs {
     GemmWidePlan plan;
     uint64_t stream;
 };
-GemmWidePlan gemm_wide_plan(uint32_t m, uint32_t n, uint32_t k, bool swiglu, int max_splits = 8);
+GemmWidePlan gemm_wide_plan(uint32_t m, uint32_t n, uint32_t k, bool swiglu, int max_splits = 8,
+                            bool variables = true);
 bool gemm_wide(const GemmWideArgs& a, std::string* err);
 int gemm_wide_forced();   // the tiling that KCMM_GEMM_TILE forces, less 100; 0: none
 

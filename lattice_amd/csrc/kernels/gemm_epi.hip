@@ -373,7 +373,7 @@ bool run_epi(const EpiParams& p, uint64_t stream, std::string* err) {
     for (int most : {8, 1}) {
         dev::GemmWidePlan wide;
         const bool many = forced == 100 || wide_may_do(p);
-        if (many) wide = dev::gemm_epi_wide_plan(p, most);
+        if (many) wide = dev::gemm_epi_wide_plan(p, most, forced == 100);
         Choice tile;
         if (forced != 100) tile = choose_tile(p, most > 1);
         const bool take_wide = many && (forced == 100 || tile.us < 0 || wide_us(p, wide) < tile.us);

@@ -218,8 +218,10 @@ __device__ __forceinline__ f32x4 mfma_line(const u32x4 (&a)[2], const u32x4 (&b)
 
 namespace dev {
 // The product on 256-row tiles (gemm_epi_wide.hip) and the plan for it; at most
-// max_splits K splits, whose sums the fp32 partials at `part` carry.
-GemmWidePlan gemm_epi_wide_plan(const EpiParams& p, int max_splits);
+// max_splits K splits, whose sums the fp32 partials at `part` carry.  forced: as
+// KCMM_GEMM_TILE and KCMM_GEMM_SPLITS say.  Where there is no such plan: 256-token
+// tiles without K splits, which any product can run on, of infinite time.
+GemmWidePlan gemm_epi_wide_plan(const EpiParams& p, int max_splits, bool forced);
 bool gemm_epi_wide(const EpiParams& p, const GemmWidePlan& plan, float* part, uint64_t stream,
                    std::string* err);
 // The epilogue of the sum of `splits` fp32 partials [splits][M][N].

@@ -11,6 +11,7 @@
 //    splits the sums go through fp32 partials, and a second kernel adds them in
 //    split order and runs it.
 #include <algorithm>
+#include <cmath>
 #include <string>
 #include <type_traits>
 
@@ -323,14 +324,16 @@ bool gemm_epi_sum(const EpiParams& e, const float* part, int splits, uint64_t st
 // either type.  Its K splits are of equal length; from 32 lines on it is asked
 // for a multiple of 8, and the last split is shorter (542 x 3700 x 10928, 171
 // lines: unsplit 174 us).
-GemmWidePlan gemm_epi_wide_plan(const EpiParams& p, int max_splits) {
+GemmWidePlan gemm_epi_wide_plan(const EpiParams& p, int max_splits, bool forced) {
     const uint32_t lines = (p.kb + 127) / 128, round = lines >= 32 ? (lines + 7) / 8 * 8 : lines;
-    GemmWidePlan plan;
-    if (round >= 2)
-        plan = gemm_wide_plan(static_cast<uint32_t>(p.M), static_cast<uint32_t>(p.N), round * 64, false,
-                              max_splits);
-    if (round < 2 || plan.splits < 1) plan = GemmWidePlan{};
-    return plan;
+    if (round >= 2) {
+        const GemmWidePlan plan = gemm_wide_plan(static_cast<uint32_t>(p.M), static_cast<uint32_t>(p.N),
+                                                 round * 64, false, max_splits, forced);
+        if (plan.splits >= 1) return plan;
+    }
+    GemmWidePlan none;
+    none.us = HUGE_VAL;
+    return none;
 }
 
 bool gemm_epi_wide(const EpiParams& e, const GemmWidePlan& c, float* part, uint64_t stream,

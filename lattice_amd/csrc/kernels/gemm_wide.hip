@@ -374,11 +374,13 @@ int gemm_wide_forced() {
 // round on 128-token tiles).  A split counts 5% more than its model, whose
 // error is larger there.  KCMM_GEMM_SPLITS forces the split (0 splits in the
 // result: it cannot be had); KCMM_GEMM_TILE = 100 + fb0 the token tiles'
-// height, 100 + 10 fb1 + fb0 two heights, half of the weight tiles each.
-GemmWidePlan gemm_wide_plan(uint32_t m, uint32_t n, uint32_t k, bool swiglu, int max_splits) {
+// height, 100 + 10 fb1 + fb0 two heights, half of the weight tiles each (both where
+// `variables`).
+GemmWidePlan gemm_wide_plan(uint32_t m, uint32_t n, uint32_t k, bool swiglu, int max_splits,
+                            bool variables) {
     const int M = static_cast<int>(m), N = static_cast<int>(n), K = static_cast<int>(k);
-    const int forced = gemm_wide_forced();
-    const int forced_splits = swiglu ? 1 : tunable_or(Tun::kGemmSplits, 0);
+    const int forced = variables ? gemm_wide_forced() : 0;
+    const int forced_splits = swiglu ? 1 : variables ? tunable_or(Tun::kGemmSplits, 0) : 0;
     const int bn = swiglu ? 128 : 256;
     const int tiles_n = (N + bn - 1) / bn, chunks = K / 64;
     GemmWidePlan best;
