@@ -154,8 +154,21 @@ __device__ __forceinline__ void epi_store(const EpiParams& p, int m, int n, floa
                                           const EpiCols& c, const EpiToken& t) {
     if (m >= p.M || n >= p.N) return;
     if constexpr (F8) {
+        // a sum of codes times a token's scale stays in fp32 for all but the largest
+        // and smallest tokens; those by mantissas and exponents, as the weights' scale
+        // may bring them back
+        if (__builtin_expect(fabsf(t.xs) > 0x1p-100f && fabsf(t.xs) < 0x1p80f, 1)) {
 #pragma unroll
-        for (int r = 0; r < 8; ++r) v[r] = v[r] * t.xs * c.ws[r];
+            for (int r = 0; r < 8; ++r) v[r] = v[r] * t.xs * c.ws[r];
+        } else {
+            int xe, we;
+            const float x = frexpf(t.xs, &xe);
+#pragma unroll
+            for (int r = 0; r < 8; ++r) {
+                const float w = frexpf(c.ws[r], &we);
+                v[r] = ldexpf(v[r] * x * w, xe + we);
+            }
+        }
     }
     if (p.bias != nullptr) {
 #pragma unroll

@@ -1,9 +1,9 @@
 """The ends of the epilogue products' ranges on the GPU: activations whose
-results are far below their arguments."""
+results are far below their arguments, scales near the ends of fp32."""
 import numpy as np
 import pytest
 
-from lattice_amd.bindings import ACT_GELU, ACT_GELU_TANH, ACT_SILU
+from lattice_amd.bindings import ACT_GELU, ACT_GELU_TANH, ACT_NONE, ACT_SILU
 from tests import e4m3 as E
 from tests.test_gpu_gemm_epi import call
 
@@ -71,3 +71,31 @@ def test_results_below_the_normal_numbers(gpu_lib, act, low, high):
     got = activated(torch, gpu_lib, z, act)
     assert np.all(np.abs(got - y) <= np.maximum(E.BF16_HALF * np.abs(y), 2.0 ** -134) +
                   2.0 ** -15 * np.abs(y))
+
+
+@pytest.mark.parametrize("tile,splits", [(None, 1), (9, 1), (9, 2), (100, 1), (100, 2)])
+@pytest.mark.parametrize("m,n,k", [(3, 41, 272), (300, 264, 1024)])
+def test_scales_whose_product_alone_is_ordinary(gpu_lib, tunables, m, n, k, tile, splits):
+    """Tokens of any size (scales 2^-126 .. 2^119, as the row quantisers make them)
+    against weights that bring them back: sum xscale wscale is a whole number
+    times a power of two that fp32 has, sum xscale alone is past it or below it.
+    Bit for bit, as every sum is exact in fp32."""
+    import torch
+    if tile is not None:
+        tunables.setenv("KCMM_EPI_TILE", str(tile))
+        tunables.setenv("KCMM_GEMM_SPLITS", str(splits))
+    rng = np.random.default_rng([m, n, k])
+    for unit, xe, we in ((1.0, rng.integers(100, 120, m), rng.integers(-110, -90, n)),
+                         (2.0 ** -9, rng.integers(-126, -100, m), rng.integers(100, 120, n)),
+                         (1.0, rng.integers(100, 120, m), np.full(n, -149))):
+        x = unit * rng.integers(-3, 4, (m, k)).astype(np.float64)
+        w = unit * rng.integers(-3, 4, (n, k)).astype(np.float64)
+        xs, ws = np.exp2(xe.astype(np.float64)), np.exp2(we.astype(np.float64))
+        bias = E.bf16(rng.integers(-100, 101, n))
+        y, s = E.product(x, w, None, None, None, None, ACT_NONE)
+        assert s.max() < 2 ** 14 * unit * unit
+        y = y * (xs[:, None] * ws)                      # exact: powers of two
+        for b in (None, bias):
+            got = call(torch, gpu_lib, x, w, xs, ws, b)
+            z = E.f32(y) if b is None else E.f32(E.f32(y) + b)
+            assert np.array_equal(got, E.bf16(z)), (unit, b is None)
