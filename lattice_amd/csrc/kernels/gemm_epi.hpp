@@ -31,27 +31,28 @@ typedef int i32x8 __attribute__((ext_vector_type(8)));
 // most of them; a bf16 store's is 2^-8).  A fit of erf alone, of the same absolute
 // error, has no bits of the lower tail: Abramowitz and Stegun 7.1.26 was 0.4% off at
 // z = -6 and 3.7% at -13.  The exponential is 2^8 of itself, so that it is a normal
-// number (the hardware's is 0 below) until nothing of the result is left in bf16.
+// number (the hardware's is 0 below) until nothing of the result is left in bf16; the
+// coefficients take that off again, and half of erfc.
 __device__ __forceinline__ float gelu_erf(float z) {
+    constexpr float s = 0x1p-9f;
     const float t = __builtin_amdgcn_rcpf(fmaf(0.42426407f, fabsf(z), 1.0f));
-    float c = fmaf(-0.0920885652f, t, 0.411972642f);
-    c = fmaf(c, t, -0.64450407f);
-    c = fmaf(c, t, 0.283816934f);
-    c = fmaf(c, t, 0.0733853355f);
-    c = fmaf(c, t, 0.291609466f);
-    c = fmaf(c, t, 0.337247759f);
-    c = fmaf(c, t, 0.338560164f) * t * __builtin_amdgcn_exp2f(fmaf(z * z, -0.72134752f, 8.0f));
-    // one less the upper tail, or the lower tail itself
-    return z >= 0.0f ? z * fmaf(-0x1p-9f, c, 1.0f) : z * c * 0x1p-9f;
+    float c = fmaf(s * -0.0920885652f, t, s * 0.411972642f);
+    c = fmaf(c, t, s * -0.64450407f);
+    c = fmaf(c, t, s * 0.283816934f);
+    c = fmaf(c, t, s * 0.0733853355f);
+    c = fmaf(c, t, s * 0.291609466f);
+    c = fmaf(c, t, s * 0.337247759f);
+    c = fmaf(c, t, s * 0.338560164f) * t * __builtin_amdgcn_exp2f(fmaf(z * z, -0.72134752f, 8.0f));
+    return z * (z >= 0.0f ? 1.0f - c : c);   // one less the upper tail, or the lower tail itself
 }
 
 // z / (1 + e^-t), the sum 2^-15 of itself: so its reciprocal is a normal number (the
 // hardware's is 0 below) as far as t = -97.7, where z = t is the last to leave anything
-// in bf16 (less than half of its least step).  The 2^-15 are taken off in two parts, of
-// z and of the reciprocal, so that neither's product is past fp32.
+// in bf16 (less than half of its least step).  The quotient without z is subnormal from
+// t = -87.3 on, at most 2^-150 off, and z times that nothing to a bf16 step of 2^-133.
 __device__ __forceinline__ float z_sigmoid(float z, float t) {
-    const float r = __builtin_amdgcn_rcpf(0x1p-15f + __builtin_amdgcn_exp2f(fmaf(-1.44269504f, t, -15.0f)));
-    return 0x1p-8f * z * (0x1p-7f * r);
+    return z * (0x1p-15f * __builtin_amdgcn_rcpf(0x1p-15f +
+                                                 __builtin_amdgcn_exp2f(fmaf(-1.44269504f, t, -15.0f))));
 }
 
 __device__ __forceinline__ float activate(float z, int act) {
