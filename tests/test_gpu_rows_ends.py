@@ -1,4 +1,5 @@
-"""SwiGLU rows whose gates are so negative that e^-g is past fp32."""
+"""Rows as e4m3 codes at the ends of their range: SwiGLU gates so negative that e^-g
+is past fp32, norms of nothing."""
 import numpy as np
 import pytest
 
@@ -58,3 +59,20 @@ def test_far_gates_and_ups_that_are_not_finite(gpu_lib):
     v[0, :5] = v[1, :4] = 0
     codes[0, :5] = codes[1, :4] = 0
     check_rows(codes, scales, v, 2.0 ** -17)
+
+
+@pytest.mark.parametrize("cols", [64, 4096, 33000])
+def test_norm_of_zeros_without_eps(gpu_lib, cols):
+    """0 / 0: NaN codes and scale 1 in that row, nothing in the others."""
+    import torch
+    x = E.bf16(np.random.default_rng(cols).standard_normal((3, cols)))
+    x[1] = 0
+    xd, wd = dev16(torch, x), dev16(torch, np.ones(cols))
+    o = Outputs(torch, 3, cols)
+    gpu_lib.add_rmsnorm_fp8(xd.data_ptr(), 0, wd.data_ptr(), 0, o.c.data_ptr(), o.s.data_ptr(), 3, cols,
+                            0.0, torch.cuda.current_stream().cuda_stream)
+    torch.cuda.synchronize()
+    codes, scales = o.get()
+    assert np.all((codes[1] & 0x7f) == 0x7f) and scales[1] == 1
+    _, v = E.add_rmsnorm(x[::2], None, np.ones(cols), 0.0)
+    check_rows(codes[::2], scales[::2], v, 2.0 ** -18 + cols / 1024 * 2.0 ** -24)
