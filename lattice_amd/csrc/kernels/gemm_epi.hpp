@@ -55,31 +55,27 @@ __device__ __forceinline__ float z_sigmoid(float z, float t) {
                                                  __builtin_amdgcn_exp2f(fmaf(-1.44269504f, t, -15.0f))));
 }
 
-__device__ __forceinline__ float activate(float z, int act) {
-    switch (act) {
-        case kActRelu: return z < 0.0f ? 0.0f : z;
-        case kActGelu: return gelu_erf(z);
-        case kActGeluTanh:   // z sigmoid(2 u): the tanh form without its cancellation
-            return z_sigmoid(z, 1.59576912f * z * fmaf(0.044715f * z, z, 1.0f));
-        case kActSilu: return z_sigmoid(z, z);
-        default: return z;
-    }
-}
-
-// The activation of R values, its kind looked at once.
+// The activation of R values, its kind looked at once.  (The code is laid out for every
+// eight outputs of a tile, 180 KB in all: what two kinds share is there once.)
 template <int R>
 __device__ __forceinline__ void activate_all(float (&z)[R], int act) {
-    switch (act) {
-#define KCMM_ACT_CASE(A)                                          \
-    case A:                                                       \
-        _Pragma("unroll") for (int r = 0; r < R; ++r) z[r] = activate(z[r], A); \
-        break;
-        KCMM_ACT_CASE(kActRelu)
-        KCMM_ACT_CASE(kActGelu)
-        KCMM_ACT_CASE(kActGeluTanh)
-        KCMM_ACT_CASE(kActSilu)
-#undef KCMM_ACT_CASE
-        default: break;
+    if (act == kActNone) return;
+    if (act == kActRelu) {
+#pragma unroll
+        for (int r = 0; r < R; ++r) z[r] = z[r] < 0.0f ? 0.0f : z[r];
+    } else if (act == kActGelu) {
+#pragma unroll
+        for (int r = 0; r < R; ++r) z[r] = gelu_erf(z[r]);
+    } else {   // SiLU, or z sigmoid(2 u): the tanh form without its cancellation
+        float t[R];
+#pragma unroll
+        for (int r = 0; r < R; ++r) t[r] = z[r];
+        if (act == kActGeluTanh) {
+#pragma unroll
+            for (int r = 0; r < R; ++r) t[r] = 1.59576912f * z[r] * fmaf(0.044715f * z[r], z[r], 1.0f);
+        }
+#pragma unroll
+        for (int r = 0; r < R; ++r) z[r] = z_sigmoid(z[r], t[r]);
     }
 }
 
@@ -155,21 +151,17 @@ __device__ __forceinline__ void epi_store(const EpiParams& p, int m, int n, floa
                                           const EpiCols& c, const EpiToken& t) {
     if (m >= p.M || n >= p.N) return;
     if constexpr (F8) {
-        // a sum of codes times a token's scale stays in fp32 for all but the largest
-        // and smallest tokens; those by mantissas and exponents, as the weights' scale
-        // may bring them back
-        if (__builtin_expect(fabsf(t.xs) > 0x1p-100f && fabsf(t.xs) < 0x1p80f, 1)) {
+        // A sum of codes times the scale of a very large or small token may leave fp32
+        // where the weights' scale brings it back: such a scale comes in two parts, the
+        // second a power of two after the weights' (1 for any other token).  Nothing is
+        // past fp32 on the way then for weights' scales of 2^-124 .. 2^85.  (A branch
+        // that took such tokens' scales apart cost 2048 x 14336 x 512 e4m3 37.3 -> 40.8 us,
+        // by the length of its code; this 34.5, with the activations' code shared.)
+        const bool large = fabsf(t.xs) >= 0x1p80f, small = fabsf(t.xs) <= 0x1p-80f;
+        const float xs = t.xs * (large ? 0x1p-64f : small ? 0x1p64f : 1.0f);
+        const float after = large ? 0x1p64f : small ? 0x1p-64f : 1.0f;
 #pragma unroll
-            for (int r = 0; r < 8; ++r) v[r] = v[r] * t.xs * c.ws[r];
-        } else {
-            int xe, we;
-            const float x = frexpf(t.xs, &xe);
-#pragma unroll
-            for (int r = 0; r < 8; ++r) {
-                const float w = frexpf(c.ws[r], &we);
-                v[r] = ldexpf(v[r] * x * w, xe + we);
-            }
-        }
+        for (int r = 0; r < 8; ++r) v[r] = v[r] * xs * c.ws[r] * after;
     }
     if (p.bias != nullptr) {
 #pragma unroll
