@@ -162,6 +162,46 @@ int kcmm_paged_attn_decode_f32_on_stream(
     uint32_t kv_heads, uint32_t head_dim, uint32_t block_size,
     uint32_t max_blocks_per_seq, float scale, uint64_t stream_ptr);
 
+/* ---- decode attention of sequences that share a prefix -------------------- */
+
+/**
+ * Decode attention (tensor contract of kcmm_paged_attn_decode_f16, ref
+ * kcmm.h:505; page types and q/out types as kcmm_paged_attn_prefill_on_stream)
+ * for a batch whose sequences share prefixes in groups, each prefix read and
+ * multiplied once for its group.  No counterpart in the reference, whose
+ * sharing manager is a placeholder (ref sharing.rs:24-65); the groups are what
+ * kcmm_share_prefix, kcmm_prefix_attach and kcmm_fork_beams_on_stream make.
+ *
+ * Group g is the sequences group_starts[g] .. group_starts[g + 1] - 1 of the
+ * batch (device int32 [num_groups + 1], ascending, in 0 .. batch; groups may be
+ * empty).  The first shared_lens[b] tokens of sequence b (device int32 [batch],
+ * any number, inside a page too; it may differ within a group) are those of the
+ * group's first sequence, and are read through the first sequence's table
+ * alone: the entries of b's own table for blocks that lie wholly below
+ * shared_lens[b] are not read.  A sequence in no group shares nothing, whatever
+ * its shared_lens.  Sequences with seq_lens <= 0 give zeros.
+ *
+ * scratch_ptr: device memory of the caller's, aligned to 256 bytes, of
+ * scratch_bytes >= kcmm_paged_attn_shared_scratch_bytes; its contents on entry do
+ * not matter.  Calls that may run at the same time need scratch of their own.
+ * Nothing is allocated and no state is kept: a call may be captured into a HIP
+ * graph at once, and the graph reads and writes the buffers it was given.
+ * Enqueue only.  -1 and the pool's error text where an argument does not fit.
+ */
+int kcmm_paged_attn_decode_shared_on_stream(
+    kcmm_pool_t *pool, uint32_t layer_idx, uint64_t query_ptr, uint64_t out_ptr,
+    uint64_t block_tables_ptr, uint64_t seq_lens_ptr, uint64_t shared_lens_ptr,
+    uint64_t group_starts_ptr, uint64_t block_offsets_f16_ptr, uint64_t scratch_ptr,
+    uint64_t scratch_bytes, uint32_t batch, uint32_t num_groups, uint32_t num_q_heads,
+    uint32_t kv_heads, uint32_t head_dim, uint32_t block_size, uint32_t max_blocks_per_seq,
+    float scale, uint64_t stream_ptr);
+
+/** Bytes of scratch that kcmm_paged_attn_decode_shared_on_stream takes for up to
+ *  `batch` sequences in any groups (it grows with batch and with
+ *  max_blocks_per_seq).  0 on error.  Host-only. */
+uint64_t kcmm_paged_attn_shared_scratch_bytes(kcmm_pool_t *pool, uint32_t batch,
+                                              uint32_t num_q_heads, uint32_t max_blocks_per_seq);
+
 /* ---- chunked prefill attention ----------------------------------------- */
 
 /**
@@ -415,6 +455,46 @@ int kcmm_rope_append_bf16_on_stream(kcmm_pool_t *pool, uint32_t layer_idx, uint6
                                     uint32_t num_q_heads, uint32_t max_blocks_per_seq,
                                     uint64_t stream_ptr);
 
+/** Positions of a chunk's tokens, where they are not the places in the cache. */
+typedef struct kcmm_rope_positions {
+    uint64_t positions;         /**< device int32 [axes][total_query_tokens] */
+    uint32_t axes;              /**< 1 .. 4 (time, height, width of an image's patches, ...) */
+    uint8_t axis_of_pair[128];  /**< pair i (< head_dim / 2) turns by axis axis_of_pair[i] */
+} kcmm_rope_positions_t;
+
+/** kcmm_rope_append_bf16_on_stream for the tokens of whole chunks, on every page
+ *  type: what a prompt (or drafted tokens to be verified) needs between its QKV
+ *  projection and kcmm_paged_attn_prefill_on_stream, whose block_tables,
+ *  seq_lens and query_start_loc it takes (the reference prefills a token at a
+ *  time, ref transformer.rs:50-65).  Row query_start_loc[b] + i of qkv_ptr ([q
+ *  heads | k heads | v heads] x head_dim; f16 for f16 pools, fp32 for fp32 pools,
+ *  bf16 otherwise) is the token at place seq_lens[b] - len_b + i of sequence b.
+ *  q goes to the same row of q_out_ptr ([total_query_tokens][num_q_heads]
+ *  [head_dim]), k and v into the token's page row, q and k rotated (pairs i,
+ *  i + head_dim/2) by position * inv_freq[i].  The position is the place, or
+ *  with `positions` (NULL: none) any int32, of the axis that the pair takes.
+ *
+ *  The angle is exact to 2^-22 at any position (the decode form rounds it to
+ *  fp32, which is off by up to 2^-24 of the angle: 2^-9 from position 32768 on),
+ *  and every output is rounded once.  On fp8 pages the rows that the call writes
+ *  into a page are one set, as at the head of this file, but of rotated values
+ *  that have not been rounded to bf16.
+ *
+ *  Left as they were: rows of no sequence (behind query_start_loc[batch]) and
+ *  of places outside 0 .. max_blocks_per_seq * block_size - 1; and the pages of
+ *  table entries that are no block id that the pool had issued at the time of
+ *  the call (their q is written).  Shared pages are made private first, as for
+ *  every append: no two sequences of a call write one page.  head_dim % 8 == 0,
+ *  <= 256; qkv and q_out aligned to 16 bytes and apart.  No workspace; may be
+ *  captured into a HIP graph.  Enqueue only. */
+int kcmm_rope_append_chunk_on_stream(kcmm_pool_t *pool, uint32_t layer_idx, uint64_t qkv_ptr,
+                                     uint64_t q_out_ptr, uint64_t block_tables_ptr,
+                                     uint64_t seq_lens_ptr, uint64_t query_start_loc_ptr,
+                                     uint64_t block_offsets_f16_ptr, uint64_t inv_freq_ptr,
+                                     const kcmm_rope_positions_t *positions, uint32_t batch,
+                                     uint32_t total_query_tokens, uint32_t num_q_heads,
+                                     uint32_t max_blocks_per_seq, uint64_t stream_ptr);
+
 /** The QKV projection of a decode step with RoPE and the KV append in its
  *  store (ref llama_transformer.rs:315-333: q/k/v GEMMs, rope.cu, the cache
  *  write): x_ptr [batch][hidden] times w_qkv_ptr [(Hq + 2 Hkv) head_dim]
@@ -521,6 +601,41 @@ int kcmm_gemm_fp8_on_stream(uint64_t x8_ptr, uint64_t xscale_ptr, uint64_t w8_pt
 int kcmm_gemm_bf16_epi_on_stream(uint64_t x_ptr, uint64_t w_ptr, uint64_t y_ptr,
                                  const kcmm_gemm_epilogue_t *epilogue, uint32_t m, uint32_t n,
                                  uint32_t k, uint64_t stream_ptr);
+
+/* ---- low-rank adapters ----------------------------------------------------- */
+
+/** The adapters of one projection (device addresses; bf16 weights).  A projection
+ *  made of several (q, k and v in one product) has a slice of columns for each:
+ *  slice s ends before column slice_ends[s] and has rows s * rank .. of A. */
+typedef struct kcmm_lora {
+    uint64_t a;              /**< [adapters][slices * rank][k] */
+    uint64_t b;              /**< [adapters][n][rank] */
+    uint64_t scales;         /**< fp32 [adapters], or 0: all 1 */
+    uint32_t adapters, rank; /**< rank: the largest, smaller ones padded with zeros */
+    uint32_t slices;         /**< 1 .. 4 */
+    uint32_t slice_ends[4];  /**< ascending multiples of 16; the last is n */
+} kcmm_lora_t;
+
+/** y[t] = bf16(base[t] + scales[a] (x[t] A_a^T) B_a^T), a = adapter_ids[t]: what
+ *  the tokens' adapters add to the shared projection x W^T that base holds
+ *  (kcmm_gemm_bf16_on_stream and its like).  No counterpart in the reference.
+ *  adapter_ids: device int32 [m], in any order; a token with an id outside 0 ..
+ *  adapters - 1 has no adapter, its y is its base.  Sums are fp32, y is rounded
+ *  once; what one token holds, infinities and NaN too, reaches no other token,
+ *  nor does what an adapter holds reach a token that has another.  y may be
+ *  base.
+ *  low_ptr: device memory of the caller's, fp32 [m][slices * rank], that takes
+ *  the low-rank values x A^T of the tokens with an adapter.  Calls that may run at
+ *  the same time need one each.  1 <= m <= 2^20; n % 16 == 0, <= 2^22; k % 8 ==
+ *  0, <= 2^20; rank % 8 == 0, <= 128; adapters <= 65535.  x, a, b, low, base and y
+ *  aligned to 16 bytes; y (unless it is base) and low overlap nothing else.
+ *  No workspace; may be captured into a HIP graph.  On the calling thread's
+ *  current device, to which pointers and stream belong.  Enqueue only; -1 and a
+ *  line on stderr where an argument does not fit, before any device work. */
+int kcmm_lora_add_bf16_on_stream(uint64_t x_ptr, const kcmm_lora_t *lora,
+                                 uint64_t adapter_ids_ptr, uint64_t low_ptr, uint64_t base_ptr,
+                                 uint64_t y_ptr, uint32_t m, uint32_t n, uint32_t k,
+                                 uint64_t stream_ptr);
 
 /** Device addresses of one layer's weights (bf16, row-major [out][in]). */
 typedef struct kcmm_layer_weights {

@@ -112,6 +112,20 @@ class KcmmGemmEpilogue(C.Structure):
     _fields_ = [("bias", C.c_uint64), ("residual", C.c_uint64), ("activation", C.c_int32)]
 
 
+class KcmmRopePositions(C.Structure):
+    """kcmm_rope_positions_t (include/kcmm_mi355x.h): a chunk's positions on
+    their axes, and the axis of each rotated pair."""
+    _fields_ = [("positions", C.c_uint64), ("axes", C.c_uint32), ("axis_of_pair", C.c_uint8 * 128)]
+
+
+class KcmmLora(C.Structure):
+    """kcmm_lora_t (include/kcmm_mi355x.h): the low-rank adapters of one
+    projection."""
+    _fields_ = [("a", C.c_uint64), ("b", C.c_uint64), ("scales", C.c_uint64),
+                ("adapters", C.c_uint32), ("rank", C.c_uint32), ("slices", C.c_uint32),
+                ("slice_ends", C.c_uint32 * 4)]
+
+
 _P, _U32, _U64, _I32 = C.c_void_p, C.c_uint32, C.c_uint64, C.c_int32
 _ATTN = [_P, _U32, _U64, _U64, _U64, _U64, _U64] + [_U32] * 6 + [C.c_float]
 
@@ -159,6 +173,9 @@ SIGNATURES = {
     "kcmm_paged_attn_prefill_on_stream": ([_P, _U32, _U64, _U64, _U64, _U64, _U64, _U64, _U32,
                                            _U32, _U32, _U32, _U32, _U32, _U32, C.c_float, _U64],
                                           C.c_int),
+    "kcmm_paged_attn_decode_shared_on_stream": ([_P, _U32] + [_U64] * 9 + [_U32] * 7 +
+                                                [C.c_float, _U64], C.c_int),
+    "kcmm_paged_attn_shared_scratch_bytes": ([_P, _U32, _U32, _U32], _U64),
     "kcmm_precompile_paged_attn_decode_f16": ([_P], C.c_int),
     "kcmm_evict_blocks": ([_P, _U32], _U32),
     "kcmm_restore_evicted_block": ([_P, _U32], _U64),
@@ -214,6 +231,10 @@ SIGNATURES = {
                                               C.c_float, _U64], C.c_int),
     "kcmm_qkv_rope_append_bf16_on_stream": ([_P, _U32, _U64, _U64, _U64, _U64, _U64, _U64, _U64,
                                              _U32, _U32, _U32, _U32, _U64], C.c_int),
+    "kcmm_rope_append_chunk_on_stream": ([_P, _U32] + [_U64] * 7 + [C.POINTER(KcmmRopePositions)] +
+                                         [_U32] * 4 + [_U64], C.c_int),
+    "kcmm_lora_add_bf16_on_stream": ([_U64, C.POINTER(KcmmLora)] + [_U64] * 4 + [_U32] * 3 + [_U64],
+                                     C.c_int),
     "kcmm_rope_append_bf16_on_stream": ([_P, _U32, _U64, _U64, _U64, _U64, _U64, _U64, _U32,
                                          _U32, _U32, _U64], C.c_int),
     "kcmm_decode_layer_step_on_stream": ([_P, _U32, C.POINTER(KcmmLayerWeights), _U64, _U64, _U64,
@@ -373,6 +394,18 @@ class KcmmLibrary:
         if self.lib.kcmm_gemm_bf16_epi_on_stream(x_ptr, w_ptr, y_ptr, C.byref(epi), m, n, k,
                                                  stream_ptr) != 0:
             raise KcmmError("kcmm_gemm_bf16_epi_on_stream failed")
+
+    def lora_add_bf16(self, x_ptr, a_ptr, b_ptr, adapter_ids_ptr, low_ptr, base_ptr, y_ptr, m, n, k,
+                      *, adapters, rank, slice_ends=None, scales_ptr=0, stream_ptr=0) -> None:
+        """y[t] = base[t] + scales[a] (x[t] A_a^T) B_a^T, a = adapter_ids[t] (outside 0 ..
+        adapters - 1: y[t] = base[t]); low: fp32 [m][slices * rank] of the caller's; y may be
+        base.  slice_ends: where the columns of the projection's parts end (default: one)."""
+        ends = [n] if slice_ends is None else list(slice_ends)
+        lora = KcmmLora(a_ptr, b_ptr, scales_ptr, adapters, rank, len(ends),
+                        (C.c_uint32 * 4)(*ends[:4]))
+        if self.lib.kcmm_lora_add_bf16_on_stream(x_ptr, C.byref(lora), adapter_ids_ptr, low_ptr,
+                                                 base_ptr, y_ptr, m, n, k, stream_ptr) != 0:
+            raise KcmmError("kcmm_lora_add_bf16_on_stream failed")
 
     def decode_logits_bf16(self, hidden_ptr, norm_w_ptr, lm_head_ptr, logits_ptr, batch,
                            hidden_size, vocab_size, eps, stream_ptr=0) -> None:
@@ -644,7 +677,49 @@ class KcmmPool:
             kv_heads, head_dim, block_size, max_blocks_per_seq, C.c_float(scale), stream_ptr)
         self._check(rc, "paged_attn_prefill")
 
+    def shared_scratch_bytes(self, batch, num_q_heads, max_blocks_per_seq) -> int:
+        """Bytes of scratch that paged_attn_decode_shared takes."""
+        n = self.lib.kcmm_paged_attn_shared_scratch_bytes(self.handle, batch, num_q_heads,
+                                                          max_blocks_per_seq)
+        if n == 0:
+            raise KcmmError(f"kcmm_paged_attn_shared_scratch_bytes failed: {self.last_error()}")
+        return n
+
+    def paged_attn_decode_shared(self, *, layer_idx, query_ptr, out_ptr, block_tables_ptr,
+                                 seq_lens_ptr, shared_lens_ptr, group_starts_ptr,
+                                 block_offsets_f16_ptr, scratch_ptr, scratch_bytes, batch,
+                                 num_groups, num_q_heads, kv_heads, head_dim, block_size,
+                                 max_blocks_per_seq, scale, stream_ptr=0) -> None:
+        """Decode attention of groups of sequences that share a prefix: the first
+        shared_lens[b] tokens of sequence b are those of its group's first sequence (group g:
+        sequences group_starts[g] .. group_starts[g + 1] - 1)."""
+        rc = self.lib.kcmm_paged_attn_decode_shared_on_stream(
+            self.handle, layer_idx, query_ptr, out_ptr, block_tables_ptr, seq_lens_ptr,
+            shared_lens_ptr, group_starts_ptr, block_offsets_f16_ptr, scratch_ptr, scratch_bytes,
+            batch, num_groups, num_q_heads, kv_heads, head_dim, block_size, max_blocks_per_seq,
+            C.c_float(scale), stream_ptr)
+        self._check(rc, "paged_attn_decode_shared")
+
     # -- decode-step glue and the layer step --
+    def rope_append_chunk(self, *, layer_idx, qkv_ptr, q_out_ptr, block_tables_ptr, seq_lens_ptr,
+                          query_start_loc_ptr, block_offsets_f16_ptr, inv_freq_ptr, batch,
+                          total_query_tokens, num_q_heads, max_blocks_per_seq, positions_ptr=0,
+                          num_axes=1, pair_axes=None, stream_ptr=0) -> None:
+        """RoPE of a chunk's q / k, k and v appended to the pages.  positions_ptr: int32
+        [num_axes][total_query_tokens] (0: the places in the cache), pair i turning by axis
+        pair_axes[i] (default: 0)."""
+        pos = None
+        if positions_ptr:
+            pos = KcmmRopePositions(positions_ptr, num_axes)
+            for i, a in enumerate(pair_axes or ()):
+                pos.axis_of_pair[i] = a
+        rc = self.lib.kcmm_rope_append_chunk_on_stream(
+            self.handle, layer_idx, qkv_ptr, q_out_ptr, block_tables_ptr, seq_lens_ptr,
+            query_start_loc_ptr, block_offsets_f16_ptr, inv_freq_ptr,
+            C.byref(pos) if pos is not None else None, batch, total_query_tokens, num_q_heads,
+            max_blocks_per_seq, stream_ptr)
+        self._check(rc, "rope_append_chunk")
+
     def rope_append(self, *, layer_idx, qkv_ptr, q_out_ptr, block_tables_ptr, seq_lens_ptr,
                     block_offsets_f16_ptr, inv_freq_ptr, batch, num_q_heads, max_blocks_per_seq,
                     stream_ptr=0) -> None:

@@ -48,7 +48,8 @@ HIP_SOURCES = ["kernels/backing.hip", "kernels/attn_decode.hip", "kernels/attn_p
                "kernels/page_copy.hip", "kernels/gemm.hip", "kernels/gemm_tiled.hip",
                "kernels/gemm_wide.hip",
                "kernels/glue.hip", "kernels/quant_rows.hip", "kernels/gemm_epi.hip",
-               "kernels/gemm_epi_wide.hip",
+               "kernels/gemm_epi_wide.hip", "kernels/attn_shared.hip", "kernels/rope_chunk.hip",
+               "kernels/lora.hip",
                "kernels/tier_copy.hip"]
 
 

@@ -297,6 +297,47 @@ struct GemmEpiArgs {
 };
 bool gemm_epi(const GemmEpiArgs& a, std::string* err);
 
+// Decode attention of groups of sequences that share a prefix
+// (kernels/attn_shared.hip): the first shared_lens[b] tokens of sequence b are
+// those of its group's first sequence; group g = sequences group_starts[g] ..
+// group_starts[g + 1] - 1.  scratch: the caller's, of at least
+// attn_shared_scratch_bytes.
+struct AttnSharedArgs {
+    int32_t dtype;
+    uint64_t q, out, k_base, v_base, block_tables, seq_lens, shared_lens, group_starts, offsets_f16;
+    uint64_t scratch, scratch_bytes;
+    uint32_t batch, num_groups, num_q_heads, kv_heads, head_dim, block_size, mbps;
+    uint32_t row_bytes, data_bytes;
+    float scale;
+    uint64_t stream;
+};
+uint64_t attn_shared_scratch_bytes(int32_t dtype, uint32_t batch, uint32_t num_q_heads,
+                                   uint32_t kv_heads, uint32_t head_dim, uint32_t block_size,
+                                   uint32_t mbps);
+bool attn_shared(const AttnSharedArgs& a, std::string* err);
+
+// A chunk's rotation and append (kernels/rope_chunk.hip).
+struct RopeChunkArgs {
+    int32_t dtype;
+    uint64_t qkv, q_out, k_base, v_base, block_tables, seq_lens, query_start_loc, offsets_f16;
+    uint64_t inv_freq;      // fp32 [head_dim / 2]
+    uint64_t positions;     // int32 [axes][total_query_tokens], or 0: places in the cache
+    uint8_t axis_of_pair[128];
+    uint32_t batch, total_query_tokens, num_q_heads, kv_heads, head_dim, block_size, mbps;
+    uint32_t row_bytes, data_bytes, n_ids;
+    uint64_t stream;
+};
+bool rope_append_chunk(const RopeChunkArgs& a, std::string* err);
+
+// Low-rank adapters added to a shared projection (kernels/lora.hip).
+struct LoraArgs {
+    uint64_t x, a, b, scales, ids, low, base, y;
+    uint32_t m, n, k, adapters, rank, slices;
+    uint32_t slice_ends[4];
+    uint64_t stream;
+};
+bool lora_add_bf16(const LoraArgs& a, std::string* err);
+
 }  // namespace dev
 
 // Activations of gemm_epi (kcmm_activation_t).

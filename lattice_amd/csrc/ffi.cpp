@@ -671,6 +671,112 @@ int kcmm_paged_attn_prefill_on_stream(kcmm_pool_t* pool, uint32_t layer_idx, uin
     return 0;
 }
 
+extern "C++" {
+namespace {
+// Shapes that the shared-prefix attention takes (kv geometry: the pool's).
+bool shared_shapes_ok(kcmm_pool_t* pool, const char* fn, uint32_t batch, uint32_t hq, uint32_t mbps) {
+    const kcmm::PoolGeometry& g = pool->core->geo();
+    if (batch == 0 || hq == 0 || mbps == 0) {
+        pool->set_error(std::string(fn) + ": shape arguments must be positive");
+        return false;
+    }
+    if (g.head_dim > 256 || hq > 0xFFFF || mbps > 0xFFFF || g.block_size > 0xFFFF ||
+        g.kv_heads > 0xFFFF) {
+        pool->set_error(std::string(fn) + ": head_dim <= 256 and packed shapes <= 65535 required");
+        return false;
+    }
+    if (static_cast<uint64_t>(batch) * hq > 0x7fffffffull ||
+        static_cast<uint64_t>(mbps) * g.block_size > 0x7fffffffull) {
+        pool->set_error(std::string(fn) + ": batch x q heads and the tables' tokens must be below 2^31");
+        return false;
+    }
+    return true;
+}
+}  // namespace
+}  // extern "C++"
+
+uint64_t kcmm_paged_attn_shared_scratch_bytes(kcmm_pool_t* pool, uint32_t batch, uint32_t hq,
+                                              uint32_t mbps) {
+    const char* fn = "kcmm_paged_attn_shared_scratch_bytes";
+    if (pool == nullptr || !shared_shapes_ok(pool, fn, batch, hq, mbps)) return 0;
+    const kcmm::PoolGeometry& g = pool->core->geo();
+    return kcmm::dev::attn_shared_scratch_bytes(
+        g.dtype, batch, hq, static_cast<uint32_t>(g.kv_heads), static_cast<uint32_t>(g.head_dim),
+        static_cast<uint32_t>(g.block_size), mbps);
+}
+
+int kcmm_paged_attn_decode_shared_on_stream(kcmm_pool_t* pool, uint32_t layer_idx, uint64_t q,
+                                            uint64_t out, uint64_t bt, uint64_t sl,
+                                            uint64_t shared_lens, uint64_t group_starts,
+                                            uint64_t offs, uint64_t scratch,
+                                            uint64_t scratch_bytes, uint32_t batch,
+                                            uint32_t num_groups, uint32_t hq, uint32_t hkv,
+                                            uint32_t d, uint32_t bs, uint32_t mbps, float scale,
+                                            uint64_t stream) {
+    const char* fn = "kcmm_paged_attn_decode_shared_on_stream";
+    if (pool == nullptr || q == 0 || out == 0 || bt == 0 || sl == 0 || shared_lens == 0 ||
+        group_starts == 0 || offs == 0 || scratch == 0) {
+        if (pool) pool->set_error(std::string(fn) + ": null pointer argument");
+        return -1;
+    }
+    if (!layer_ok(pool, layer_idx, fn)) return -1;
+    const kcmm::PoolGeometry& g = pool->core->geo();
+    if (hkv != g.kv_heads || d != g.head_dim || bs != g.block_size) {
+        pool->set_error(std::string(fn) +
+                        ": kv_heads/head_dim/block_size differ from the pool's geometry");
+        return -1;
+    }
+    if (!shared_shapes_ok(pool, fn, batch, hq, mbps)) return -1;
+    if (num_groups == 0 || num_groups > batch) {
+        pool->set_error(std::string(fn) + ": needs 1 .. batch groups");
+        return -1;
+    }
+    const uint64_t need = kcmm::dev::attn_shared_scratch_bytes(g.dtype, batch, hq, hkv, d, bs, mbps);
+    if (scratch % 256 != 0 || scratch_bytes < need) {
+        pool->set_error(std::string(fn) + ": scratch must be aligned to 256 bytes and hold " +
+                        std::to_string(need) + " bytes, has " + std::to_string(scratch_bytes));
+        return -1;
+    }
+    if (q % 16 != 0 || out % 16 != 0) {
+        pool->set_error(std::string(fn) + ": q and out must be aligned to 16 bytes");
+        return -1;
+    }
+    std::string err;
+    if (!kcmm::dev::set_device(pool->device, &err)) {
+        pool->set_error(std::string(fn) + ": bind device failed: " + err);
+        return -1;
+    }
+    kcmm::dev::AttnSharedArgs a{};
+    a.dtype = g.dtype;
+    a.q = q;
+    a.out = out;
+    a.k_base = pool->core->va_k(layer_idx);
+    a.v_base = pool->core->va_v(layer_idx);
+    a.block_tables = bt;
+    a.seq_lens = sl;
+    a.shared_lens = shared_lens;
+    a.group_starts = group_starts;
+    a.offsets_f16 = offs;
+    a.scratch = scratch;
+    a.scratch_bytes = scratch_bytes;
+    a.batch = batch;
+    a.num_groups = num_groups;
+    a.num_q_heads = hq;
+    a.kv_heads = hkv;
+    a.head_dim = d;
+    a.block_size = bs;
+    a.mbps = mbps;
+    a.row_bytes = static_cast<uint32_t>(g.row_bytes);
+    a.data_bytes = static_cast<uint32_t>(g.data_bytes);
+    a.scale = scale;
+    a.stream = stream;
+    if (!kcmm::dev::attn_shared(a, &err)) {
+        pool->set_error(std::string(fn) + ": launch failed: " + err);
+        return -1;
+    }
+    return 0;
+}
+
 int kcmm_precompile_paged_attn_decode_f16(kcmm_pool_t* pool) { return pool ? 0 : -1; }
 
 // ---- tiering: HBM <-> host swap (ref tiering.rs, pool.rs:824-1002) ----------------
@@ -1468,6 +1574,143 @@ int kcmm_rope_append_bf16_on_stream(kcmm_pool_t* pool, uint32_t layer_idx, uint6
         return -1;
     }
     return 0;
+}
+
+int kcmm_rope_append_chunk_on_stream(kcmm_pool_t* pool, uint32_t layer_idx, uint64_t qkv,
+                                     uint64_t q_out, uint64_t block_tables, uint64_t seq_lens,
+                                     uint64_t query_start_loc, uint64_t offsets_f16,
+                                     uint64_t inv_freq, const kcmm_rope_positions_t* positions,
+                                     uint32_t batch, uint32_t total, uint32_t num_q_heads,
+                                     uint32_t max_blocks_per_seq, uint64_t stream) {
+    const std::string fn = "kcmm_rope_append_chunk_on_stream";
+    if (pool == nullptr) return -1;
+    auto refuse = [&](const std::string& why) {
+        pool->set_error(fn + ": " + why);
+        return -1;
+    };
+    if (qkv == 0 || q_out == 0 || block_tables == 0 || seq_lens == 0 || query_start_loc == 0 ||
+        offsets_f16 == 0 || inv_freq == 0 || (positions != nullptr && positions->positions == 0))
+        return refuse("null pointer argument");
+    if (!layer_ok(pool, layer_idx, fn.c_str())) return -1;
+    const kcmm::PoolGeometry& g = pool->core->geo();
+    if (batch == 0 || num_q_heads == 0 || max_blocks_per_seq == 0 || num_q_heads % g.kv_heads != 0 ||
+        num_q_heads > 0xFFFF || max_blocks_per_seq > 0xFFFF || batch > 0x7fffffffu)
+        return refuse("batch, q heads (a multiple of kv heads) and max_blocks_per_seq must be positive "
+                      "(q heads and max_blocks_per_seq <= 65535)");
+    if (g.head_dim % 8 != 0 || g.head_dim > 256)
+        return refuse("head_dim must be a multiple of 8, <= 256");
+    const uint64_t heads = num_q_heads + 2 * g.kv_heads, io = g.dtype == kcmm::kF32 ? 4 : 2;
+    if (total * heads * g.head_dim > 0x7fffffffffull || total > 0x7fffffffu ||
+        static_cast<uint64_t>(max_blocks_per_seq) * g.block_size > 0x7fffffffull)
+        return refuse("too many tokens");
+    if (!aligned(16, {qkv, q_out}) || !aligned(8, {offsets_f16}) ||
+        !aligned(4, {block_tables, seq_lens, query_start_loc, inv_freq}))
+        return refuse("qkv and q_out must be aligned to 16 bytes, the others to their elements");
+    if (!apart({qkv, total * heads * g.head_dim * io}, {q_out, total * num_q_heads * g.head_dim * io}))
+        return refuse("q_out overlaps qkv");
+    kcmm::dev::RopeChunkArgs a{};
+    if (positions != nullptr) {
+        if (positions->axes == 0 || positions->axes > 4) return refuse("needs 1 .. 4 axes");
+        if (positions->positions % 4 != 0) return refuse("positions must be aligned to 4 bytes");
+        for (size_t i = 0; i < g.head_dim / 2; ++i) {
+            if (positions->axis_of_pair[i] >= positions->axes)
+                return refuse("pair " + std::to_string(i) + " takes axis " +
+                              std::to_string(positions->axis_of_pair[i]) + " of " +
+                              std::to_string(positions->axes));
+            a.axis_of_pair[i] = positions->axis_of_pair[i];
+        }
+        a.positions = positions->positions;
+    }
+    a.dtype = g.dtype;
+    a.qkv = qkv;
+    a.q_out = q_out;
+    a.k_base = pool->core->va_k(layer_idx);
+    a.v_base = pool->core->va_v(layer_idx);
+    a.block_tables = block_tables;
+    a.seq_lens = seq_lens;
+    a.query_start_loc = query_start_loc;
+    a.offsets_f16 = offsets_f16;
+    a.inv_freq = inv_freq;
+    a.batch = batch;
+    a.total_query_tokens = total;
+    a.num_q_heads = num_q_heads;
+    a.kv_heads = static_cast<uint32_t>(g.kv_heads);
+    a.head_dim = static_cast<uint32_t>(g.head_dim);
+    a.block_size = static_cast<uint32_t>(g.block_size);
+    a.mbps = max_blocks_per_seq;
+    a.row_bytes = static_cast<uint32_t>(g.row_bytes);
+    a.data_bytes = static_cast<uint32_t>(g.data_bytes);
+    a.n_ids = pool->core->total_blocks();
+    a.stream = stream;
+    std::string err;
+    if (!kcmm::dev::set_device(pool->device, &err) || !kcmm::dev::rope_append_chunk(a, &err))
+        return refuse(err);
+    return 0;
+}
+
+int kcmm_lora_add_bf16_on_stream(uint64_t x, const kcmm_lora_t* lora, uint64_t adapter_ids,
+                                 uint64_t low, uint64_t base, uint64_t y, uint32_t m, uint32_t n,
+                                 uint32_t k, uint64_t stream) {
+    return call_without_pool("kcmm_lora_add_bf16_on_stream", [&](std::string* err) {
+        if (lora == nullptr || x == 0 || lora->a == 0 || lora->b == 0 || adapter_ids == 0 || low == 0 ||
+            base == 0 || y == 0) {
+            *err = "null pointer argument";
+            return false;
+        }
+        const uint64_t M = m, N = n, K = k, R = lora->rank, S = lora->slices, A = lora->adapters;
+        if (m == 0 || m > 1u << 20 || n == 0 || n % 16 != 0 || n > 1u << 22 || k == 0 || k % 8 != 0 ||
+            k > 1u << 20) {
+            *err = "needs 1 <= m <= 2^20, n a positive multiple of 16 (<= 2^22), k one of 8 (<= 2^20)";
+            return false;
+        }
+        if (R == 0 || R % 8 != 0 || R > 128 || A == 0 || A > 65535 || S == 0 || S > 4) {
+            *err = "needs a rank that is a multiple of 8 (<= 128), 1 .. 65535 adapters, 1 .. 4 slices";
+            return false;
+        }
+        uint32_t last = 0;
+        for (uint32_t i = 0; i < S; ++i) {
+            if (lora->slice_ends[i] <= last || lora->slice_ends[i] % 16 != 0) {
+                *err = "slice_ends must be ascending multiples of 16";
+                return false;
+            }
+            last = lora->slice_ends[i];
+        }
+        if (last != n) {
+            *err = "the last slice must end at n";
+            return false;
+        }
+        if (!aligned(16, {x, lora->a, lora->b, low, base, y}) || !aligned(4, {lora->scales, adapter_ids})) {
+            *err = "x, a, b, low, base and y must be aligned to 16 bytes, the others to 4";
+            return false;
+        }
+        const Span in[] = {{x, 2 * M * K}, {lora->a, 2 * A * S * R * K}, {lora->b, 2 * A * N * R},
+                           {lora->scales, 4 * A}, {adapter_ids, 4 * M}};
+        const Span lo{low, 4 * M * S * R}, ba{base, 2 * M * N}, out{y, 2 * M * N};
+        bool ok = same_or_apart(out, ba) && apart(out, lo) && apart(lo, ba);
+        for (const Span& s : in) ok = ok && apart(out, s) && apart(lo, s);
+        if (!ok) {
+            *err = "an output overlaps another buffer";
+            return false;
+        }
+        kcmm::dev::LoraArgs a{};
+        a.x = x;
+        a.a = lora->a;
+        a.b = lora->b;
+        a.scales = lora->scales;
+        a.ids = adapter_ids;
+        a.low = low;
+        a.base = base;
+        a.y = y;
+        a.m = m;
+        a.n = n;
+        a.k = k;
+        a.adapters = lora->adapters;
+        a.rank = lora->rank;
+        a.slices = lora->slices;
+        for (uint32_t i = 0; i < S; ++i) a.slice_ends[i] = lora->slice_ends[i];
+        a.stream = stream;
+        return kcmm::dev::lora_add_bf16(a, err);
+    });
 }
 
 int kcmm_qkv_rope_append_bf16_on_stream(kcmm_pool_t* pool, uint32_t layer_idx, uint64_t x,

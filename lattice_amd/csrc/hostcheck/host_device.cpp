@@ -261,6 +261,12 @@ bool silu_mul_fp8(uint64_t, uint64_t, uint64_t, uint32_t, uint32_t, uint64_t, st
     return no_device(err);
 }
 bool gemm_epi(const GemmEpiArgs&, std::string* err) { return no_device(err); }
+uint64_t attn_shared_scratch_bytes(int32_t, uint32_t, uint32_t, uint32_t, uint32_t, uint32_t, uint32_t) {
+    return 4096;
+}
+bool attn_shared(const AttnSharedArgs&, std::string* err) { return no_device(err); }
+bool rope_append_chunk(const RopeChunkArgs&, std::string* err) { return no_device(err); }
+bool lora_add_bf16(const LoraArgs&, std::string* err) { return no_device(err); }
 bool gemm_split_reduce_launch(const float*, uint16_t*, const uint16_t*, int, int, uint64_t,
                               std::string* err) {
     return no_device(err);
