@@ -174,12 +174,13 @@ int kcmm_paged_attn_decode_f32_on_stream(
  *
  * Group g is the sequences group_starts[g] .. group_starts[g + 1] - 1 of the
  * batch (device int32 [num_groups + 1], ascending, in 0 .. batch; groups may be
- * empty).  The first shared_lens[b] tokens of sequence b (device int32 [batch],
- * any number, inside a page too; it may differ within a group) are those of the
- * group's first sequence, and are read through the first sequence's table
- * alone: the entries of b's own table for blocks that lie wholly below
- * shared_lens[b] are not read.  A sequence in no group shares nothing, whatever
- * its shared_lens.  Sequences with seq_lens <= 0 give zeros.
+ * empty).  The whole blocks among the first shared_lens[b] tokens of sequence b
+ * (device int32 [batch], any number; it may differ within a group) are those of
+ * the group's first sequence, and are read through the first sequence's table
+ * alone: the entries of b's own table for them are not read.  The block that a
+ * shared length ends in is read through b's own table, as copy-on-write and
+ * forks leave it.  A sequence in no group shares nothing, whatever its
+ * shared_lens.  Sequences with seq_lens <= 0 give zeros.
  *
  * scratch_ptr: device memory of the caller's, aligned to 256 bytes, of
  * scratch_bytes >= kcmm_paged_attn_shared_scratch_bytes; its contents on entry do

@@ -2,9 +2,8 @@
 (kcmm_paged_attn_decode_shared) on the GPU against fp64.
 
 What a sequence may not read is poisoned: the entries of its own table for
-blocks wholly below its shared length name a page of NaN, and so are NaN every
-slot behind a sequence's end and, of a page that a prefix ends in, the slots of
-the prefix in the sequence's own copy.
+blocks wholly below its shared length name a page of NaN, and so is every slot
+behind a sequence's end.
 
 Tolerance of an output o = sum_t w_t V_t with A = sum_t w_t |V_t| (weights that
 add up to 1): the store rounds by u |o| (u: half a step, eps / 2 of the type);
@@ -53,7 +52,7 @@ class Case:
         need = [max(t, 0) for t in self.totals]
         for s, t, lead in seqs:
             if lead is not None:
-                need[lead] = max(need[lead], min(s, max(t, 0)))
+                need[lead] = max(need[lead], min(s, max(t, 0)) // bs * bs)
         self.mbps = max(1, max(-(-n // bs) for n in need))
         blocks = [-(-n // bs) for n in need]
         cfg = make_config(num_layers=1, kv_heads=hkv, head_dim=d, max_batch=self.batch,
@@ -72,7 +71,7 @@ class Case:
         table = np.full((self.batch, self.mbps), poison, np.int32)
         dense = []
         for b, (s, t, lead) in enumerate(seqs):
-            first = 0 if lead in (None, b) else max(0, min(s, t))     # own tokens from here on
+            first = 0 if lead in (None, b) else max(0, min(s, t)) // bs * bs     # own tokens from here on
             n = need[b]
             kv = []
             for _ in range(2):
