@@ -203,9 +203,8 @@ void launch_generic(const SharedParams& p, hipStream_t s) {
 
 // ---- whole GQA groups of at most 16 heads, head_dim 64 or 128, pages of 8-token groups ----
 
-constexpr int kWaves = 4;          // of a workgroup
-constexpr int kMaxRows = 512;      // sequences of a launch
-constexpr int kRowsPerThread = kMaxRows / (64 * kWaves);
+constexpr int kWaves = 4;              // of a workgroup
+constexpr int kMaxRows = 64 * kWaves;   // sequences of a launch: one a thread in find_items
 
 // What the joining kernel has to know of a sequence: where its parts are.
 struct RowPlan {
@@ -229,37 +228,6 @@ struct FastParams {
 
 __device__ __forceinline__ int tiles_of(int tokens) { return (tokens + 31) >> 5; }
 
-// Exclusive sums over kMaxRows values, kRowsPerThread consecutive ones a thread;
-// *all: their sum.  s_wave: kWaves ints of LDS.
-__device__ __forceinline__ void block_sums(const int (&v)[kRowsPerThread], int (&at)[kRowsPerThread], int* all,
-                                           int* s_wave) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    int sum = 0;
-#pragma unroll
-    for (int i = 0; i < kRowsPerThread; ++i) {
-        at[i] = sum;
-        sum += v[i];
-    }
-    int incl = sum;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const int y = __shfl_up(incl, o);
-        if (lane >= o) incl += y;
-    }
-    if (lane == 63) s_wave[wave] = incl;
-    __syncthreads();
-    int before = incl - sum;
-    *all = 0;
-#pragma unroll
-    for (int w = 0; w < kWaves; ++w) {
-        if (w < wave) before += s_wave[w];
-        *all += s_wave[w];
-    }
-#pragma unroll
-    for (int i = 0; i < kRowsPerThread; ++i) at[i] += before;
-    __syncthreads();
-}
-
 // The items of this launch, in LDS, by sequence (relative to row0).
 struct Items {
     int len[kMaxRows];      // tokens, clamped to what the table holds
@@ -267,106 +235,105 @@ struct Items {
     int lead[kMaxRows];     // whose table these are read through (of the whole batch)
     int common[kMaxRows];   // tokens that the item of the sequence takes in common; 0: none
     int count[kMaxRows];    // sequences of the item that begins here, 0: none does
-    int most[kMaxRows];     // its common tokens
+    int most[kMaxRows];     // the most that one of them shares, then their common tokens
+    int least[kMaxRows];
+    int part[kMaxRows];     // sequences of the item that take part
     int pre[kMaxRows];      // tiles of the items before this sequence, of one kv head
     int own[kMaxRows];      // the same of the sequences' own tokens
-    int pre_all, own_all;
-    int wave[kWaves];
+    uint64_t begins[kWaves];   // bit of a wave's lane: a group begins there
+    int sums[2][kWaves];
     int carry;
 };
 
+// Sum over lanes 0 .. l, by row shifts and row broadcasts.
+__device__ __forceinline__ int wave_sums(int x) {
+#define KCMM_ADD(ctrl, rows) x += __builtin_amdgcn_update_dpp(0, x, ctrl, rows, 0xF, false)
+    KCMM_ADD(0x111, 0xF);   // row_shr:1, 2, 4, 8
+    KCMM_ADD(0x112, 0xF);
+    KCMM_ADD(0x114, 0xF);
+    KCMM_ADD(0x118, 0xF);
+    KCMM_ADD(0x142, 0xA);   // row_bcast:15 into rows 1 and 3
+    KCMM_ADD(0x143, 0xC);   // row_bcast:31 into rows 2 and 3
+#undef KCMM_ADD
+    return x;
+}
+
+// One sequence a thread.  (Every workgroup spends this before its first load, so
+// nothing walks over sequences: an item's members meet in LDS atomics.)
 __device__ __forceinline__ void find_items(const FastParams& f, Items& it) {
     const SharedParams& p = f.p;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    constexpr int N = kRowsPerThread;
-    const int cap = p.mbps * p.block_size, r0 = tid * N;
-    int len[N], want[N], lead[N];
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-        const int r = r0 + i;
-        len[i] = want[i] = 0;
-        if (r < f.rows) {
-            len[i] = max(0, min(p.seq_lens[f.row0 + r], cap));
-            want[i] = p.shared_lens[f.row0 + r];
-        }
-        it.lead[r] = -1;
-        it.common[r] = it.count[r] = 0;
+    const int r = threadIdx.x, lane = r & 63, wave = r >> 6, b = f.row0 + r;
+    int len = 0, shared = 0;
+    if (r < f.rows) {
+        len = max(0, min(p.seq_lens[b], p.mbps * p.block_size));
+        shared = p.shared_lens[b];
     }
-    if (tid == 0) it.carry = -1;
-    __syncthreads();
     const int end = p.group_starts[p.groups];   // sequences from here on lie in no group
-    for (int g = tid; g < p.groups; g += 64 * kWaves) {
+    it.len[r] = len;
+    it.common[r] = it.count[r] = it.most[r] = it.part[r] = 0;
+    it.least[r] = INT_MAX;
+    it.lead[r] = -1;
+    if (r == 0) it.carry = -1;
+    __syncthreads();
+    for (int g = r; g < p.groups; g += kMaxRows) {
         const int start = p.group_starts[g];
-        if (start < 0 || start >= p.batch) continue;
-        if (start >= f.row0 && start < f.row0 + f.rows) atomicMax(&it.lead[start - f.row0], start);
-        else if (start < f.row0) atomicMax(&it.carry, start);
+        if (start < 0 || start >= f.row0 + f.rows) continue;
+        if (start >= f.row0) it.lead[start - f.row0] = start;
+        else atomicMax(&it.carry, start);
     }
     __syncthreads();
-    // the last group start not behind a sequence
-    int top = -1;
-#pragma unroll
-    for (int i = 0; i < N; ++i) lead[i] = top = max(top, it.lead[r0 + i]);
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const int y = __shfl_up(top, o);
-        if (lane >= o) top = max(top, y);
-    }
-    if (lane == 63) it.wave[wave] = top;
-    int before = __shfl_up(top, 1);
-    if (lane == 0) before = -1;
+    const uint64_t mine = __ballot(it.lead[r] >= 0);
+    if (lane == 0) it.begins[wave] = mine;
     __syncthreads();
-    before = max(before, it.carry);
-    for (int w = 0; w < wave; ++w) before = max(before, it.wave[w]);
-    unsigned begins = 0;   // bit i: an item begins at r0 + i
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-        const int r = r0 + i, b = f.row0 + r;
-        lead[i] = max(lead[i], before);
-        const bool in = r < f.rows && lead[i] >= 0 && b < end;
-        it.len[r] = len[i];
-        it.shared[r] = in ? whole_blocks(min(want[i], len[i]), p.block_size) : 0;
-        it.lead[r] = in ? lead[i] : -1;
-        if (in && (b - max(lead[i], f.row0)) % f.seqs == 0) begins |= 1u << i;
+    // the last group start not behind the sequence
+    int lead = it.carry;
+    for (int w = 0; w <= wave; ++w) {
+        const uint64_t m = w < wave ? it.begins[w] : mine & (~0ull >> (63 - lane));
+        if (m) lead = f.row0 + 64 * w + 63 - __clzll(static_cast<long long>(m));
+    }
+    const bool in = r < f.rows && lead >= 0 && b < end;
+    shared = in ? whole_blocks(min(shared, len), p.block_size) : 0;
+    it.shared[r] = shared;
+    it.lead[r] = lead;
+    // the sequence's item begins at `first`
+    const int from = max(lead - f.row0, 0), first = from + (r - from) / f.seqs * f.seqs;
+    if (in) {
+        atomicMax(&it.most[first], shared);
+        atomicAdd(&it.count[first], 1);
     }
     __syncthreads();
-#pragma unroll 1
-    for (int i = 0; i < N; ++i) {
-        if (!(begins >> i & 1)) continue;
-        const int r = r0 + i, mine = it.lead[r];
-        const int last = min(r + f.seqs, f.rows);
-        int most = 0, n = 0;
-        for (; r + n < last && it.lead[r + n] == mine; ++n) most = max(most, it.shared[r + n]);
-        int common = most, part = 0;
-        for (int j = 0; j < n; ++j) {
-            const int s = it.shared[r + j];
-            if (2 * static_cast<long long>(s) < most) continue;
-            common = min(common, s);
-            ++part;
-        }
-        if (common <= 0 || part < 2) continue;   // nothing to gain: each reads its own
-        it.count[r] = n;
-        it.most[r] = common;
-        for (int j = 0; j < n; ++j)
-            if (it.shared[r + j] >= common) it.common[r + j] = common;
+    const bool part = in && shared > 0 && 2ll * shared >= it.most[first];
+    if (part) {
+        atomicMin(&it.least[first], shared);
+        atomicAdd(&it.part[first], 1);
     }
     __syncthreads();
-    int pre[N], own[N], at[N];
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-        const int r = r0 + i;
-        pre[i] = it.count[r] > 0 ? tiles_of(it.most[r]) : 0;   // (the first sequence need not take part)
-        own[i] = tiles_of(it.len[r] - it.common[r]);
+    // (of one sequence alone there is nothing to gain)
+    const int common = part && it.part[first] > 1 ? it.least[first] : 0;
+    const bool begins = in && first == r && it.part[r] > 1;
+    const int pre = begins ? tiles_of(it.least[r]) : 0, own = tiles_of(len - common);
+    it.common[r] = common;
+    if (!begins) it.count[r] = 0;
+    const int pre_to = wave_sums(pre), own_to = wave_sums(own);
+    if (lane == 63) {
+        it.sums[0][wave] = pre_to;
+        it.sums[1][wave] = own_to;
     }
-    int all;
-    block_sums(pre, at, &all, it.wave);
-#pragma unroll
-    for (int i = 0; i < N; ++i) it.pre[r0 + i] = at[i];
-    if (tid == 0) it.pre_all = all;
-    block_sums(own, at, &all, it.wave);
-#pragma unroll
-    for (int i = 0; i < N; ++i) it.own[r0 + i] = at[i];
-    if (tid == 0) it.own_all = all;
     __syncthreads();
+    int before[2] = {0, 0};
+    for (int w = 0; w < wave; ++w) {
+        before[0] += it.sums[0][w];
+        before[1] += it.sums[1][w];
+    }
+    it.pre[r] = before[0] + pre_to - pre;
+    it.own[r] = before[1] + own_to - own;
+    __syncthreads();
+}
+
+// Waves of a SIMD: two where the rings of eight waves fit the LDS and a wave's
+// outputs and Q half of the registers.
+constexpr int waves_of(int dtype, int d, int ncb) {
+    return (dtype == kDtFP8 && ncb < 4) || (dtype != kDtFP8 && d == 64) ? 2 : 1;
 }
 
 // Tiles of a slice: equal parts of all, but none so short that joining the parts
@@ -414,15 +381,42 @@ template <int O>
 __device__ __forceinline__ void lds_write(uint32_t a, u32x4 x) {
     asm volatile("ds_write_b128 %0, %1 offset:%2" :: "v"(a), "v"(x), "i"(O) : "memory");
 }
+// Two fp32 -> one dword of 16-bit elements (round to nearest even).
+template <int DT>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+    if constexpr (DT == kDtF16) {
+        typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+        return __builtin_bit_cast(uint32_t, f16x2{static_cast<_Float16>(lo), static_cast<_Float16>(hi)});
+    } else {
+        typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+        return __builtin_bit_cast(uint32_t, bf16x2{static_cast<__bf16>(lo), static_cast<__bf16>(hi)});
+    }
+}
+// Maximum over the lanes l, l ^ 16, l ^ 32, l ^ 48 that hold a column.
+__device__ __forceinline__ float column_max(float x) {
+    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+// s_waitcnt vmcnt(N) (gfx9 encoding: vmcnt bits 3:0 and 15:14, the others at most).
+template <int N>
+__device__ __forceinline__ void wait_loads() {
+    static_assert(N >= 0 && N < 64, "vmcnt is 6 bits");
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_waitcnt((N & 0xF) | ((N >> 4) << 14) | (0x7 << 4) | (0xF << 8));
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+}
 __device__ __forceinline__ uint32_t lds_address(const void* p) {
     return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) const uint8_t*)p));
 }
 
 template <int DT, int D, int BS, int NCB>
-__global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(NCB == 1 ? 2 : 1)))
+__global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(waves_of(DT, D, NCB))))
 void attn_shared_stream(FastParams f, const int32_t* __restrict__ bt, const uint64_t* __restrict__ offs,
-                        const uint8_t* __restrict__ kreg, const uint8_t* __restrict__ vreg,
-                        const uint8_t* __restrict__ idle) {
+                        const uint8_t* __restrict__ kreg, const uint8_t* __restrict__ vreg) {
     constexpr bool F8 = DT == kDtFP8;
     constexpr int MDT = F8 ? kDtBF16 : DT;     // matrix, q and out element type
     constexpr int EB = F8 ? 1 : 2;
@@ -430,12 +424,10 @@ void attn_shared_stream(FastParams f, const int32_t* __restrict__ bt, const uint
     constexpr int ROWB = D * EB;               // bytes of a token's head row
     constexpr int HALF = 32 * ROWB;            // of a tile's K, and of its V
     constexpr int LOADS = 2 * HALF / 1024;     // of a tile
-    constexpr int ST = ROWB == 256 ? 2 : F8 ? 3 : 4;   // tiles of the ring
-    constexpr int VROW = 2 * D + 32;           // bytes of a padded V row (fp8)
+    constexpr int ST = 2;                      // tiles of the ring
     static_assert(!F8 || D == 128, "fp8 pages take this path at head_dim 128");
     __shared__ Items it;
     __shared__ __attribute__((aligned(1024))) uint8_t s_ring[kWaves][ST * 2 * HALF];
-    __shared__ __attribute__((aligned(16))) uint8_t s_v[F8 ? kWaves : 1][F8 ? 32 * VROW : 16];
     const SharedParams& p = f.p;
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6);
@@ -445,18 +437,23 @@ void attn_shared_stream(FastParams f, const int32_t* __restrict__ bt, const uint
     auto uni = [](int x) { return __builtin_amdgcn_readfirstlane(x); };
 
     find_items(f, it);
-    const int pre_end = uni(it.pre_all) * Hkv, total = pre_end + uni(it.own_all) * Hkv;
+    int pre_all = 0, own_all = 0;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+        pre_all += it.sums[0][w];
+        own_all += it.sums[1][w];
+    }
+    const int pre_end = uni(pre_all) * Hkv, total = pre_end + uni(own_all) * Hkv;
     const int per = slice_tiles(total, f);
     if (blockIdx.x == 0) {
         if (threadIdx.x == 0) *f.per = per;
-        int first = -1;
-        for (int r = threadIdx.x; r < f.rows; r += 64 * kWaves) {
+        const int r = threadIdx.x;
+        if (r < f.rows) {
             RowPlan w{};
             w.own_tile = pre_end + it.own[r] * Hkv;
             w.own_tiles = tiles_of(it.len[r] - it.common[r]);
             if (it.common[r] > 0) {
-                first = r;   // the item that r lies in begins at most seqs - 1 before
-                while (it.count[first] == 0) --first;
+                const int from = max(it.lead[r] - f.row0, 0), first = from + (r - from) / f.seqs * f.seqs;
                 w.first = f.row0 + first;
                 w.pre_tile = it.pre[first] * Hkv;
                 w.pre_tiles = tiles_of(it.common[r]);
@@ -472,7 +469,7 @@ void attn_shared_stream(FastParams f, const int32_t* __restrict__ bt, const uint
     // Cursor over the tile list: tokens begin + 32 t .. of (item, kv head); all of it
     // wave-uniform, so that the tables are read by scalar loads
     struct Cur {
-        int r, own, g, t, nt, begin, end, shared, lead, cols;
+        int r, own, g, t, nt, begin, end, shared, lead, seqs, blocks;
         float ks[F8 ? 4 : 1], vs[F8 ? 4 : 1];   // fp8: page scales of the 8-token groups
     };
     auto locate = [&](int tile) __attribute__((always_inline)) {
@@ -480,16 +477,15 @@ void attn_shared_stream(FastParams f, const int32_t* __restrict__ bt, const uint
         c.own = tile >= pre_end;
         const int* sums = c.own ? it.own : it.pre;
         const int rel = c.own ? tile - pre_end : tile, x = rel / Hkv;
-        int lo = 0, hi = f.rows;   // the last sequence with sums[r] <= x: it has tiles
-        while (hi - lo > 1) {
-            const int mid = (lo + hi) >> 1;
-            if (uni(sums[mid]) <= x) lo = mid;
-            else hi = mid;
-        }
+        // the last sequence with sums[r] <= x: it has tiles
+        int lo = -1;
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w)
+            lo += __popcll(__ballot(sums[64 * w + lane] <= x && 64 * w + lane < f.rows));
         c.r = lo;
-        const int n_seqs = c.own ? 1 : uni(it.count[lo]);
-        const int common = uni(c.own ? it.common[lo] : it.most[lo]);
-        c.cols = n_seqs * G;
+        c.seqs = c.own ? 1 : uni(it.count[lo]);
+        c.blocks = (c.seqs * G + 15) >> 4;
+        const int common = uni(c.own ? it.common[lo] : it.least[lo]);
         c.begin = c.own ? common : 0;
         c.end = c.own ? uni(it.len[lo]) : common;
         c.shared = c.own ? uni(it.shared[lo]) : common;
@@ -507,22 +503,50 @@ void attn_shared_stream(FastParams f, const int32_t* __restrict__ bt, const uint
         c.t = 0;
         if (++c.g == Hkv) c = locate(tile);
     };
-    // Page-relative address of each 8-token group of a tile; groups past the end
-    // re-read the last one (masked).  fp8: also the groups' page scales.
+    // Byte offsets of 64 8-token groups' rows (16 tiles), a lane each, from tile
+    // `from` of (sequence, kind) on; groups past the end repeat the last one
+    // (masked).  They hold for every kv head.  What is loaded here is waited for at
+    // once: a register that a load may still be on its way to would have every later
+    // step wait for all loads in flight.
+    struct {
+        int r, own, from, g;
+        uint64_t row;
+        uint32_t slot;                   // of it, inside its page
+        float ks, vs;                    // fp8: the groups' page scales of kv head g
+    } pages;
+    pages.r = -1;
+    // Where the tile's four groups lie for the tile's kv head (fp8: also their scales)
     auto group_bases = [&](Cur& c, uint64_t* gb) __attribute__((always_inline)) {
-        const int last8 = (c.end - 1) & ~7;
-        const int32_t* mine = bt + static_cast<size_t>(f.row0 + c.r) * p.mbps;
-        const int32_t* theirs = bt + static_cast<size_t>(c.lead) * p.mbps;
+        bool fresh = false;
+        if (pages.r != c.r || pages.own != c.own || (c.t & ~15) != pages.from) {
+            pages.from = c.t & ~15;
+            const int tok = c.begin + min(32 * pages.from + 8 * lane, (c.end - 1 - c.begin) & ~7);
+            const int row = tok < c.shared ? c.lead : f.row0 + c.r, block = tok / bs;
+            const uint64_t page = offs[bt[static_cast<size_t>(row) * p.mbps + block]];
+            pages.slot = static_cast<uint32_t>((tok - block * bs) * p.row_bytes);
+            pages.row = page * 2ull + pages.slot;
+            pages.r = c.r;
+            pages.own = c.own;
+            fresh = true;
+        }
+        if constexpr (F8) {
+            if (fresh || pages.g != c.g) {
+                const uint64_t at = pages.row - pages.slot + static_cast<uint32_t>(p.data_bytes + c.g * 4);
+                pages.ks = *reinterpret_cast<const float*>(kreg + at);
+                pages.vs = *reinterpret_cast<const float*>(vreg + at);
+                pages.g = c.g;
+                wait_loads<0>();
+            }
+        }
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-            const int tok = min(c.begin + c.t * 32 + q * 8, last8);
-            const int lb = tok / bs;
-            const uint64_t page = offs[(tok < c.shared ? theirs : mine)[lb]] * 2ull;
-            gb[q] = page + static_cast<uint32_t>((tok - lb * bs) * p.row_bytes + c.g * D * EB);
+            const int j = min(4 * c.t + q, (c.end - 1 - c.begin) >> 3) - 4 * pages.from;
+            const uint32_t lo = __builtin_amdgcn_readlane(static_cast<uint32_t>(pages.row), j);
+            const uint32_t hi = __builtin_amdgcn_readlane(static_cast<uint32_t>(pages.row >> 32), j);
+            gb[q] = (static_cast<uint64_t>(hi) << 32 | lo) + static_cast<uint32_t>(c.g * D * EB);
             if constexpr (F8) {
-                const uint64_t sc = page + static_cast<uint32_t>(p.data_bytes + c.g * 4);
-                c.ks[q] = *reinterpret_cast<const float*>(kreg + sc);
-                c.vs[q] = *reinterpret_cast<const float*>(vreg + sc);
+                c.ks[q] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(pages.ks), j));
+                c.vs[q] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(pages.vs), j));
             }
         }
     };
@@ -543,27 +567,29 @@ void attn_shared_stream(FastParams f, const int32_t* __restrict__ bt, const uint
         const int piece = ROWB == 256 ? (lane % PIECES) ^ (row & 15) : (lane % PIECES) ^ (row >> 1 & 7);
         src[i] = static_cast<uint32_t>((row & 7) * p.row_bytes + piece * 16);
     }
-    auto issue = [&](int place, bool real, const uint64_t* gb) __attribute__((always_inline)) {
-        const uint8_t* kb = real ? kreg : idle;
-        const uint8_t* vb = real ? vreg : idle;
-        uint8_t* const to = ring + place * 2 * HALF;
+    auto issue = [&](uint32_t place, const uint64_t* gb) __attribute__((always_inline)) {
+        uint8_t* const to = ring + place;
 #pragma unroll
         for (int i = 0; i < 32 / ROWS; ++i) {
-            const uint64_t g = real ? gb[i * ROWS / 8] : 0;
-            load_lds16_nt(kb + g + src[i % STEP], to + i * 1024);
-            load_lds16_nt(vb + g + src[i % STEP], to + HALF + i * 1024);
+            const uint64_t g = gb[i * ROWS / 8];
+            load_lds16_nt(kreg + g + src[i % STEP], to + i * 1024);
+            load_lds16_nt(vreg + g + src[i % STEP], to + HALF + i * 1024);
         }
     };
     // Column c of an item: head c % G of the kv head's, of its sequence c / G.
-    // Columns past the last repeat it; they are computed and never stored.
+    // Columns past the last repeat one; they are computed and never stored.
+    int seq_of[NCB], head_of[NCB];
+#pragma unroll
+    for (int cb = 0; cb < NCB; ++cb) {
+        seq_of[cb] = (cb * 16 + ln) / G;
+        head_of[cb] = cb * 16 + ln - seq_of[cb] * G;
+    }
     u32x4 qf[NCB][KC];
     auto load_q = [&](const Cur& c) __attribute__((always_inline)) {
-        const int cols = c.cols;
 #pragma unroll
         for (int cb = 0; cb < NCB; ++cb) {
-            const int col = min(cb * 16 + ln, cols - 1), s = col / G;
-            const uint8_t* qrow =
-                p.q + (static_cast<size_t>(f.row0 + c.r + s) * Hq + c.g * G + (col - s * G)) * D * 2;
+            const int row = f.row0 + c.r + min(seq_of[cb], c.seqs - 1);
+            const uint8_t* qrow = p.q + (static_cast<size_t>(row) * Hq + c.g * G + head_of[cb]) * D * 2;
 #pragma unroll
             for (int kc = 0; kc < KC; ++kc) {
                 const int e0 = F8 ? (kc >> 1) * 64 + (kc & 1) * 8 + 16 * lg : kc * 32 + lg * 8;
@@ -585,39 +611,27 @@ void attn_shared_stream(FastParams f, const int32_t* __restrict__ bt, const uint
     };
     clear();
 
+    // The part of the (item, kv head) that the wave has been through.  The part where
+    // a (sequence, head) begins has a row of its own; later ones are the slice's, in
+    // the order of the registers, which makes whole lines of the stores.
     auto flush = [&](const Cur& c, bool began_here) __attribute__((always_inline)) {
-        const bool complete = began_here && c.t == c.nt - 1;
-        const int cols = c.cols;
+        float* const to_ml = began_here ? f.ml : f.slice_ml;
 #pragma unroll
         for (int cb = 0; cb < NCB; ++cb) {
+            if (cb >= c.blocks) break;
             const float l = wave_sum_across_groups(l_run[cb]);
-            const int col = cb * 16 + ln;
-            if (col >= cols) continue;
-            const int s = col / G, row = c.r + s, h = c.g * G + (col - s * G);
-            if (complete && c.own && c.begin == 0) {
-                const float inv = 1.0f / l;
-                uint16_t* o = reinterpret_cast<uint16_t*>(p.out) +
-                              (static_cast<size_t>(f.row0 + row) * Hq + h) * D + 4 * lg;
+            const uint32_t row = static_cast<uint32_t>((c.own * f.rows + c.r + seq_of[cb]) * Hq + c.g * G + head_of[cb]);
+            const uint32_t block = static_cast<uint32_t>(slice * NCB + cb);
+            float* pa = began_here ? f.acc + static_cast<size_t>(row) * D + 4 * lg
+                                   : f.slice_acc + static_cast<size_t>(block) * (16 * D) + lane * 4;
+            const int step = began_here ? 16 : 256;
+            if (seq_of[cb] >= c.seqs) continue;
 #pragma unroll
-                for (int db = 0; db < DB; ++db) {
-                    u32x2 w;
-                    w[0] = f32_to_elem<MDT>(acc[cb][db][0] * inv) | (f32_to_elem<MDT>(acc[cb][db][1] * inv) << 16);
-                    w[1] = f32_to_elem<MDT>(acc[cb][db][2] * inv) | (f32_to_elem<MDT>(acc[cb][db][3] * inv) << 16);
-                    *reinterpret_cast<u32x2*>(o + 16 * db) = w;
-                }
-                continue;
-            }
-            // the part where a (sequence, head) begins has a row of its own, later
-            // ones take the slice's
-            const size_t at = began_here ? static_cast<size_t>(c.own * f.rows + row) * Hq + h
-                                         : static_cast<size_t>(slice) * (16 * NCB) + col;
-            float* pa = (began_here ? f.acc : f.slice_acc) + at * D + 4 * lg;
-            float* ml = (began_here ? f.ml : f.slice_ml) + at * 2;
-#pragma unroll
-            for (int db = 0; db < DB; ++db) *reinterpret_cast<f32x4*>(pa + 16 * db) = acc[cb][db];
+            for (int db = 0; db < DB; ++db) *reinterpret_cast<f32x4*>(pa + db * step) = acc[cb][db];
             if (lg == 0) {
-                ml[0] = m_run[cb];
-                ml[1] = l;
+                const size_t at = 2 * static_cast<size_t>(began_here ? row : block * 16 + ln);
+                to_ml[at] = m_run[cb];
+                to_ml[at + 1] = l;
             }
         }
         clear();
@@ -630,54 +644,57 @@ void attn_shared_stream(FastParams f, const int32_t* __restrict__ bt, const uint
     uint32_t k_at[NP], v_at[DB];
 #pragma unroll
     for (int i = 0; i < NP; ++i) k_at[i] = at0 + turned(ln, 4 * i + lg);
-    const uint32_t sv_at = lds_address(s_v[F8 ? wave : 0]);
+    // (V's rows as they are read: 2 D bytes, turned as rows of that length are)
+    auto v_turned = [](int row, int piece) __attribute__((always_inline)) {
+        return row * 2 * D + (D == 128 ? piece ^ (row & 15) : piece ^ (row >> 1 & 7)) * 16;
+    };
 #pragma unroll
     for (int db = 0; db < DB; ++db) {
         const int row = 4 * lg + (ln >> 2);
-        v_at[db] = F8 ? sv_at + row * VROW + db * 32 + (ln & 3) * 8
-                      : at0 + turned(row, 2 * db + ((ln & 3) >> 1)) + (ln & 1) * 8;
+        v_at[db] = at0 + v_turned(row, 2 * db + ((ln & 3) >> 1)) + (ln & 1) * 8;
     }
-    auto compute = [&](auto where, const Cur& c) __attribute__((always_inline)) {
-        constexpr int TK = decltype(where)::value * 2 * HALF, TV = TK + HALF;
+    auto compute = [&](uint32_t place, const Cur& c) __attribute__((always_inline)) {
+        constexpr int TK = 0, TV = HALF;
         const int tbase = c.begin + c.t * 32;
         // rows past the end may hold anything and become zeros
         if (tbase + 32 > c.end)
             for (int row = c.end - tbase + lane / PIECES; row < 32; row += ROWS)
-                lds_write<TV>(at0 + row * ROWB + lane % PIECES * 16, u32x4{0, 0, 0, 0});
+                lds_write<TV>(at0 + place + row * ROWB + lane % PIECES * 16, u32x4{0, 0, 0, 0});
+        uint32_t kp[NP];
+#pragma unroll
+        for (int i = 0; i < NP; ++i) kp[i] = k_at[i] + place;
+        u32x4 x[2][NP];
+        lds_read<TK, TK + 16 * ROWB>(x, kp);
         if constexpr (F8) {
-            // V as bf16 (exactly: the pages' scales go to P)
-            u32x4 x[2][NP];
-            lds_read<TV, TV + 16 * ROWB>(x, k_at);
+            // V as bf16 (exactly: the pages' scales go to P), over the tile's K and V
+            u32x4 y[2][NP];
+            lds_read<TV, TV + 16 * ROWB>(y, kp);
 #pragma unroll
             for (int h = 0; h < 2; ++h)
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                    const uint32_t at = sv_at + (16 * h + ln) * VROW + (4 * e + lg) * 32;
-                    lds_write<0>(at, fp8x8_to_bf16(x[h][e][0], x[h][e][1]));
-                    lds_write<16>(at, fp8x8_to_bf16(x[h][e][2], x[h][e][3]));
+                    const int row = 16 * h + ln, piece = 2 * (4 * e + lg);
+                    lds_write<0>(at0 + place + v_turned(row, piece), fp8x8_to_bf16(y[h][e][0], y[h][e][1]));
+                    lds_write<0>(at0 + place + v_turned(row, piece + 1), fp8x8_to_bf16(y[h][e][2], y[h][e][3]));
                 }
         }
-        f32x4 s[NCB][2];
-        {
-            u32x4 x[2][NP];
-            lds_read<TK, TK + 16 * ROWB>(x, k_at);
+        u32x4 pf[NCB];
+        const bool live = tbase + 32 <= c.end;   // (uniform)
+#pragma unroll
+        for (int cb = 0; cb < NCB; ++cb) {
+            if (cb >= c.blocks) break;   // (uniform: no column of the item lies here)
+            f32x4 s[2];
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-#pragma unroll
-                for (int cb = 0; cb < NCB; ++cb) s[cb][h] = f32x4{0, 0, 0, 0};
+                s[h] = f32x4{0, 0, 0, 0};
 #pragma unroll
                 for (int kc = 0; kc < KC; ++kc) {
                     u32x4 a = x[h][F8 ? kc >> 1 : kc];
                     if constexpr (F8) a = (kc & 1) ? fp8x8_to_bf16(a[2], a[3]) : fp8x8_to_bf16(a[0], a[1]);
-#pragma unroll
-                    for (int cb = 0; cb < NCB; ++cb) s[cb][h] = mfma16x16x32<MDT>(a, qf[cb][kc], s[cb][h]);
+                    s[h] = mfma16x16x32<MDT>(a, qf[cb][kc], s[h]);
                 }
             }
-        }
-        u32x4 pf[NCB];
-#pragma unroll
-        for (int cb = 0; cb < NCB; ++cb) {
-            float v[8];
+            float v[8], sum = 0.0f;
             float mt = -INFINITY;
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
@@ -685,25 +702,27 @@ void attn_shared_stream(FastParams f, const int32_t* __restrict__ bt, const uint
                 if constexpr (F8) sc *= lg < 2 ? c.ks[2 * h] : c.ks[2 * h + 1];
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    const float x = tbase + h * 16 + lg * 4 + r < c.end ? s[cb][h][r] * sc : -INFINITY;
-                    v[h * 4 + r] = x;
-                    mt = fmaxf(mt, x);
+                    const float z = s[h][r] * sc;
+                    v[h * 4 + r] = live || tbase + h * 16 + lg * 4 + r < c.end ? z : -INFINITY;
+                    mt = fmaxf(mt, v[h * 4 + r]);
                 }
             }
-            const float m_new = fmaxf(m_run[cb], wave_max_across_groups(mt));
-            const float corr = __builtin_amdgcn_exp2f(m_run[cb] - m_new);
-            float sum = 0.0f;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                v[i] = __builtin_amdgcn_exp2f(v[i] - m_new);
-                sum += v[i];
-            }
-            l_run[cb] = l_run[cb] * corr + sum;
-            m_run[cb] = m_new;
-            if (__any(corr != 1.0f)) {
+            // the column's reference grows where a score exceeds it by more than 8: until
+            // then weights are at most 2^8, which costs no bits
+            if (__any(mt > m_run[cb] + 8.0f)) {
+                const float m_new = fmaxf(m_run[cb], column_max(mt));
+                const float corr = __builtin_amdgcn_exp2f(m_run[cb] - m_new);
+                l_run[cb] *= corr;
+                m_run[cb] = m_new;
 #pragma unroll
                 for (int i = 0; i < DB; ++i) acc[cb][i] *= corr;
             }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                v[i] = __builtin_amdgcn_exp2f(v[i] - m_run[cb]);
+                sum += v[i];
+            }
+            l_run[cb] += sum;
             if constexpr (F8) {
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
@@ -715,75 +734,72 @@ void attn_shared_stream(FastParams f, const int32_t* __restrict__ bt, const uint
             // slots (lg, i) of the P^T operand: token i < 4 ? 4 lg + i : 16 + 4 lg + i - 4
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-                pf[cb][i] = f32_to_elem<MDT>(v[2 * i]) | (f32_to_elem<MDT>(v[2 * i + 1]) << 16);
+                pf[cb][i] = pack2<MDT>(v[2 * i], v[2 * i + 1]);
         }
 #pragma unroll
         for (int d0 = 0; d0 < DB; d0 += 4) {
             // lane (ln, lg): V[4 lg .. +3][16 db + ln], and of the second half
-            u32x2 x[4][2];
-            const uint32_t at[4] = {v_at[d0], v_at[d0 + 1], v_at[d0 + 2], v_at[d0 + 3]};
-            lds_read_turned<F8 ? 0 : TV, F8 ? 16 * VROW : TV + 16 * ROWB>(x, at);
+            u32x2 t[4][2];
+            const uint32_t at[4] = {v_at[d0] + place, v_at[d0 + 1] + place, v_at[d0 + 2] + place, v_at[d0 + 3] + place};
+            lds_read_turned<F8 ? 0 : TV, (F8 ? 0 : TV) + 32 * D>(t, at);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const u32x4 vt{x[e][0][0], x[e][0][1], x[e][1][0], x[e][1][1]};
+            for (int cb = 0; cb < NCB; ++cb) {
+                if (cb >= c.blocks) break;
 #pragma unroll
-                for (int cb = 0; cb < NCB; ++cb)
+                for (int e = 0; e < 4; ++e) {
+                    const u32x4 vt{t[e][0][0], t[e][0][1], t[e][1][0], t[e][1][1]};
                     acc[cb][d0 + e] = mfma16x16x32<MDT>(vt, pf[cb], acc[cb][d0 + e]);
+                }
             }
         }
     };
 
-    // Tiles i + 1 .. i + ST - 1 are in flight while tile i is consumed, the addresses of
-    // tile i + ST are being fetched.  Past the slice's end loads of `idle` (in L2)
-    // keep the count of loads in flight the same.
-    Cur cq[ST];
+    // Tile i + 1 is in flight while tile i is consumed.
+    Cur cq[ST];   // cursors of tiles i ..
     uint64_t gb[4];
     load_q(ic);
     bool began_here = ic.t == 0;
     group_bases(ic, gb);
-#pragma unroll
-    for (int k = 0; k < ST - 1; ++k) {
-        cq[k] = ic;
-        issue(k, k < n, gb);
-        if (k + 1 < n) {
-            advance(ic, t0 + k + 1);
-            group_bases(ic, gb);
-        }
+    static_assert(ST == 2, "one tile before the loop");
+    cq[0] = ic;
+    issue(0, gb);
+    if (n > 1) {
+        advance(ic, t0 + 1);
+        group_bases(ic, gb);
     }
-    auto step = [&](auto phase, int i) __attribute__((always_inline)) {
-        constexpr int j = decltype(phase)::value, jn = (j + ST - 1) % ST;
-        cq[jn] = ic;
-        issue(jn, i + ST - 1 < n, gb);   // (the place's last reads have returned)
-        if (i + ST < n) {
-            advance(ic, t0 + i + ST);
-            group_bases(ic, gb);
-        }
-        wait_vm_lgkm0<(ST - 1) * LOADS>();   // tile i is there
-        asm volatile("" ::: "memory");
-        __builtin_amdgcn_sched_barrier(0);
-        if (i < n) {
-            compute(phase, cq[j]);
-            if (i == n - 1 || cq[j].t == cq[j].nt - 1) flush(cq[j], began_here);
-            if (i + 1 < n && cq[(j + 1) % ST].t == 0) {
-                load_q(cq[(j + 1) % ST]);
-                began_here = true;
+    // (one copy of the step: a wave runs it some ten times, and code that is not yet in
+    // the instruction cache costs more than the moves)
+    uint32_t place = 0, fill = (ST - 1) * 2 * HALF;
+#pragma unroll 1
+    for (int i = 0; i < n; ++i) {
+        cq[ST - 1] = ic;
+        if (i + ST - 1 < n) {
+            issue(fill, gb);   // (the place's last reads have returned)
+            if (i + ST < n) {
+                advance(ic, t0 + i + ST);
+                group_bases(ic, gb);
             }
+            wait_loads<(ST - 1) * LOADS>();   // tile i is there
+        } else {
+            wait_loads<0>();
         }
-    };
-    for (int i = 0; i < n; i += ST) {
-        step(std::integral_constant<int, 0>{}, i);
-        step(std::integral_constant<int, 1>{}, i + 1);
-        if constexpr (ST > 2) step(std::integral_constant<int, 2>{}, i + 2);
-        if constexpr (ST > 3) step(std::integral_constant<int, 3>{}, i + 3);
+        compute(place, cq[0]);
+        if (i == n - 1 || cq[0].t == cq[0].nt - 1) {
+            flush(cq[0], began_here);
+            if (i + 1 < n) load_q(cq[1]);   // a new (item, kv head)
+            began_here = true;
+        }
+#pragma unroll
+        for (int e = 0; e + 1 < ST; ++e) cq[e] = cq[e + 1];
+        fill = place;
+        place = place + 2 * HALF == ST * 2 * HALF ? 0 : place + 2 * HALF;
     }
-    // no load may land in LDS that the next workgroup has
-    wait_vm_lgkm0<0>();
 }
 
 // Joins the parts of a (sequence, kv head) by their log-sum-exp: weights of up
 // to kJoin parts at a time in LDS, four outputs a thread, the parts dealt to
-// threads that are left over (their sums meet in LDS).  A sequence of one part
-// was stored by the streaming kernel; one without tokens gets zeros here.
+// threads that are left over (their sums meet in LDS).  A sequence without tokens
+// gets zeros here.
 constexpr int kJoin = 64, kJoinThreads = 256;
 template <int DT, int D>
 __global__ __launch_bounds__(kJoinThreads) void attn_shared_join(FastParams f, int slot_cols) {
@@ -805,16 +821,24 @@ __global__ __launch_bounds__(kJoinThreads) void attn_shared_join(FastParams f, i
     const int pre_at = pre0 / per, own_at = own0 / per;
     const int pre_n = w.pre_tiles == 0 ? 0 : (pre0 + w.pre_tiles - 1) / per - pre_at + 1;
     const int own_n = w.own_tiles == 0 ? 0 : (own0 + w.own_tiles - 1) / per - own_at + 1;
-    if (pre_n == 0 && own_n == 1) return;
     const int parts = pre_n + own_n;
     const int shift = (f.row0 + r - w.first) * G;   // its columns in the item's slices
-    // the row of part k's column of head 0: in the first parts' rows, or a slice's
+    // the row of part k's column of head 0: in the first parts' rows, or of a slice
     auto place = [&](int k, bool* first) -> size_t {
         const bool own = k >= pre_n;
         if (own) k -= pre_n;
         *first = k == 0;
         if (k == 0) return static_cast<size_t>(own * f.rows + r) * Hq + g * G;
         return static_cast<size_t>((own ? own_at : pre_at) + k) * slot_cols + (own ? 0 : shift);
+    };
+    // outputs 4 q .. of heads 0 ..: q % (D / 4) of a row's, of a slice by its registers' order
+    auto outputs = [&](int k, int q) {
+        bool first;
+        const size_t row = place(k, &first);
+        if (first) return f.acc + row * D + q * 4;
+        const size_t col = row + q / (D / 4);
+        const int d = q % (D / 4);
+        return f.slice_acc + ((col >> 4) * (D / 16) + (d >> 2)) * 256 + ((d & 3) * 16 + (col & 15)) * 4;
     };
     const int quads = G * D / 4;                       // 16 .. 512
     constexpr int MAXQ = 2;                            // of a thread
@@ -864,9 +888,7 @@ __global__ __launch_bounds__(kJoinThreads) void attn_shared_join(FastParams f, i
                 f32x4 a = acc[i] * s_scale[h];
 #pragma unroll 4
                 for (int k = turn; k < kn; k += deal) {
-                    bool one;
-                    const size_t row = place(k0 + k, &one);
-                    a += s_w[h][k] * *reinterpret_cast<const f32x4*>((one ? f.acc : f.slice_acc) + row * D + q * 4);
+                    a += s_w[h][k] * *reinterpret_cast<const f32x4*>(outputs(k0 + k, q));
                 }
                 acc[i] = a;
             }
@@ -893,13 +915,13 @@ __global__ __launch_bounds__(kJoinThreads) void attn_shared_join(FastParams f, i
 
 // Column blocks of an item: as many as a group's query rows fill, up to 64 columns.
 int column_blocks(long long rows_of_a_group) { return rows_of_a_group <= 16 ? 1 : rows_of_a_group <= 32 ? 2 : 4; }
-int slices_of(int dtype, int ncb) { return dtype == kDtFP8 && ncb == 1 ? 2048 : 1024; }
+int slices_of(int dtype, int d, int ncb) { return 1024 * waves_of(dtype, d, ncb); }
 
 // Where things lie in the scratch of a launch of `rows` sequences.
 struct Layout {
-    size_t idle, per, plan, ml, slice_ml, acc, slice_acc, bytes;
+    size_t per, plan, ml, slice_ml, acc, slice_acc, bytes;
 };
-Layout layout_of(int dtype, int rows, int hq, int d, int row_bytes, int ncb) {
+Layout layout_of(int dtype, int rows, int hq, int d, int ncb) {
     Layout l{};
     size_t at = 0;
     auto take = [&](size_t bytes) {
@@ -907,8 +929,7 @@ Layout layout_of(int dtype, int rows, int hq, int d, int row_bytes, int ncb) {
         at += (bytes + 255) & ~size_t(255);
         return here;
     };
-    const size_t firsts = size_t(2) * rows * hq, later = static_cast<size_t>(slices_of(dtype, ncb)) * 16 * ncb;
-    l.idle = take(static_cast<size_t>(8) * row_bytes + 1024);   // must cover one tile's lane addresses
+    const size_t firsts = size_t(2) * rows * hq, later = static_cast<size_t>(slices_of(dtype, d, ncb)) * 16 * ncb;
     l.per = take(sizeof(int));
     l.plan = take(static_cast<size_t>(rows) * sizeof(RowPlan));
     l.ml = take(firsts * 8);
@@ -932,7 +953,7 @@ bool launch_fast(const SharedParams& p, uint64_t scratch, hipStream_t s, std::st
     f.group = p.num_q_heads / p.kv_heads;
     f.seqs = 16 * NCB / f.group;
     f.scale_log2 = p.scale * 1.4426950408889634f;
-    f.slices = slices_of(DT, NCB);
+    f.slices = slices_of(DT, D, NCB);
     f.least = 1;
     const long long cap = static_cast<long long>(p.mbps) * p.block_size;
     for (int row0 = 0; row0 < p.batch; row0 += kMaxRows) {
@@ -942,7 +963,7 @@ bool launch_fast(const SharedParams& p, uint64_t scratch, hipStream_t s, std::st
             *err = "batch x context too large";
             return false;
         }
-        const Layout l = layout_of(DT, f.rows, p.num_q_heads, D, p.row_bytes, NCB);
+        const Layout l = layout_of(DT, f.rows, p.num_q_heads, D, NCB);
         auto at = [&](size_t o) { return reinterpret_cast<float*>(scratch + o); };
         f.per = reinterpret_cast<int*>(scratch + l.per);
         f.plan = reinterpret_cast<RowPlan*>(scratch + l.plan);
@@ -950,13 +971,12 @@ bool launch_fast(const SharedParams& p, uint64_t scratch, hipStream_t s, std::st
         f.slice_ml = at(l.slice_ml);
         f.acc = at(l.acc);
         f.slice_acc = at(l.slice_acc);
-        const auto* idle = reinterpret_cast<const uint8_t*>(scratch + l.idle);
         // no more workgroups than the tables hold tiles for
         const long long most = 2LL * f.rows * p.kv_heads * ((cap + 31) / 32);
         const unsigned wgs = static_cast<unsigned>(std::min<long long>(f.slices, most) + kWaves - 1) / kWaves;
         auto run = [&](auto bs) {
             hipLaunchKernelGGL((attn_shared_stream<DT, D, decltype(bs)::value, NCB>), dim3(wgs),
-                               dim3(64 * kWaves), 0, s, f, p.block_tables, p.offsets_f16, p.k_base, p.v_base, idle);
+                               dim3(64 * kWaves), 0, s, f, p.block_tables, p.offsets_f16, p.k_base, p.v_base);
         };
         if (p.block_size == 16) run(std::integral_constant<int, 16>{});
         else run(std::integral_constant<int, 0>{});
@@ -986,11 +1006,9 @@ uint64_t attn_shared_scratch_bytes(int32_t dtype, uint32_t batch, uint32_t num_q
                                    uint32_t head_dim, uint32_t block_size, uint32_t) {
     if (!fast_shape(dtype, num_q_heads, kv_heads, head_dim, block_size)) return 256;
     const int rows = static_cast<int>(std::min<uint32_t>(batch, kMaxRows));
-    const int row_bytes = static_cast<int>(kv_heads * head_dim * (dtype == kDtFP8 ? 1 : 2));
     size_t most = 0;
     for (int ncb : {1, 2, 4})
-        most = std::max(most, layout_of(dtype, rows, static_cast<int>(num_q_heads), static_cast<int>(head_dim),
-                                        row_bytes, ncb).bytes);
+        most = std::max(most, layout_of(dtype, rows, static_cast<int>(num_q_heads), static_cast<int>(head_dim), ncb).bytes);
     return most;
 }
 
