@@ -218,7 +218,7 @@ struct FastParams {
     int row0, rows;            // sequences of this launch
     int group, seqs;           // query heads a kv head; sequences of an item
     int slices, least;         // waves; least tiles of one
-    int* per;                  // tiles of a slice, for the joining kernel
+    int* per;                  // tiles of a slice and of all, for the joining kernel
     RowPlan* plan;
     // first parts of (sequence, head): of the common tokens, then of the rest;
     // later parts by slice, a row a column
@@ -226,7 +226,10 @@ struct FastParams {
     float scale_log2;
 };
 
-__device__ __forceinline__ int tiles_of(int tokens) { return (tokens + 31) >> 5; }
+// Tokens of a tile: 8 KiB of K and V, so that two tiles for each of eight waves fit
+// the LDS of a CU.
+constexpr int tile_tokens(int row_bytes) { return row_bytes == 256 ? 16 : 32; }
+__device__ __forceinline__ int tiles_of(int tokens, int tile) { return (tokens + tile - 1) / tile; }
 
 // The items of this launch, in LDS, by sequence (relative to row0).
 struct Items {
@@ -260,6 +263,7 @@ __device__ __forceinline__ int wave_sums(int x) {
 
 // One sequence a thread.  (Every workgroup spends this before its first load, so
 // nothing walks over sequences: an item's members meet in LDS atomics.)
+template <int TILE>
 __device__ __forceinline__ void find_items(const FastParams& f, Items& it) {
     const SharedParams& p = f.p;
     const int r = threadIdx.x, lane = r & 63, wave = r >> 6, b = f.row0 + r;
@@ -311,7 +315,7 @@ __device__ __forceinline__ void find_items(const FastParams& f, Items& it) {
     // (of one sequence alone there is nothing to gain)
     const int common = part && it.part[first] > 1 ? it.least[first] : 0;
     const bool begins = in && first == r && it.part[r] > 1;
-    const int pre = begins ? tiles_of(it.least[r]) : 0, own = tiles_of(len - common);
+    const int pre = begins ? tiles_of(it.least[r], TILE) : 0, own = tiles_of(len - common, TILE);
     it.common[r] = common;
     if (!begins) it.count[r] = 0;
     const int pre_to = wave_sums(pre), own_to = wave_sums(own);
@@ -328,12 +332,6 @@ __device__ __forceinline__ void find_items(const FastParams& f, Items& it) {
     it.pre[r] = before[0] + pre_to - pre;
     it.own[r] = before[1] + own_to - own;
     __syncthreads();
-}
-
-// Waves of a SIMD: two where the rings of eight waves fit the LDS and a wave's
-// outputs and Q half of the registers.
-constexpr int waves_of(int dtype, int d, int ncb) {
-    return (dtype == kDtFP8 && ncb < 4) || (dtype != kDtFP8 && d == 64) ? 2 : 1;
 }
 
 // Tiles of a slice: equal parts of all, but none so short that joining the parts
@@ -353,15 +351,12 @@ __device__ __forceinline__ void lds_read(u32x4 (&x)[2][2], const uint32_t (&a)[2
                  : "=&v"(x[0][0]), "=&v"(x[0][1]), "=&v"(x[1][0]), "=&v"(x[1][1])
                  : "v"(a[0]), "v"(a[1]), "i"(O0), "i"(O1) : "memory");
 }
-template <int O0, int O1>
-__device__ __forceinline__ void lds_read(u32x4 (&x)[2][4], const uint32_t (&a)[4]) {
-    asm volatile("ds_read_b128 %0, %8 offset:%12\n\tds_read_b128 %1, %9 offset:%12\n\t"
-                 "ds_read_b128 %2, %10 offset:%12\n\tds_read_b128 %3, %11 offset:%12\n\t"
-                 "ds_read_b128 %4, %8 offset:%13\n\tds_read_b128 %5, %9 offset:%13\n\t"
-                 "ds_read_b128 %6, %10 offset:%13\n\tds_read_b128 %7, %11 offset:%13\n\ts_waitcnt lgkmcnt(0)"
-                 : "=&v"(x[0][0]), "=&v"(x[0][1]), "=&v"(x[0][2]), "=&v"(x[0][3]), "=&v"(x[1][0]),
-                   "=&v"(x[1][1]), "=&v"(x[1][2]), "=&v"(x[1][3])
-                 : "v"(a[0]), "v"(a[1]), "v"(a[2]), "v"(a[3]), "i"(O0), "i"(O1) : "memory");
+template <int O0, int>
+__device__ __forceinline__ void lds_read(u32x4 (&x)[1][4], const uint32_t (&a)[4]) {
+    asm volatile("ds_read_b128 %0, %4 offset:%8\n\tds_read_b128 %1, %5 offset:%8\n\t"
+                 "ds_read_b128 %2, %6 offset:%8\n\tds_read_b128 %3, %7 offset:%8\n\ts_waitcnt lgkmcnt(0)"
+                 : "=&v"(x[0][0]), "=&v"(x[0][1]), "=&v"(x[0][2]), "=&v"(x[0][3])
+                 : "v"(a[0]), "v"(a[1]), "v"(a[2]), "v"(a[3]), "i"(O0) : "memory");
 }
 // Transposing reads: of a 16-lane group, lane a + 4 s gives the address of four
 // 16-bit elements M[a + 4 s][0 .. 3], lane 4 a + e receives M[a][e], M[a + 4][e],
@@ -377,9 +372,41 @@ __device__ __forceinline__ void lds_read_turned(u32x2 (&x)[4][2], const uint32_t
                    "=&v"(x[2][1]), "=&v"(x[3][0]), "=&v"(x[3][1])
                  : "v"(a[0]), "v"(a[1]), "v"(a[2]), "v"(a[3]), "i"(O0), "i"(O1) : "memory");
 }
+template <int O0, int>
+__device__ __forceinline__ void lds_read_turned(u32x2 (&x)[4][1], const uint32_t (&a)[4]) {
+    asm volatile("ds_read_b64_tr_b16 %0, %4 offset:%8\n\tds_read_b64_tr_b16 %1, %5 offset:%8\n\t"
+                 "ds_read_b64_tr_b16 %2, %6 offset:%8\n\tds_read_b64_tr_b16 %3, %7 offset:%8\n\t"
+                 "s_waitcnt lgkmcnt(0)"
+                 : "=&v"(x[0][0]), "=&v"(x[1][0]), "=&v"(x[2][0]), "=&v"(x[3][0])
+                 : "v"(a[0]), "v"(a[1]), "v"(a[2]), "v"(a[3]), "i"(O0) : "memory");
+}
 template <int O>
 __device__ __forceinline__ void lds_write(uint32_t a, u32x4 x) {
     asm volatile("ds_write_b128 %0, %1 offset:%2" :: "v"(a), "v"(x), "i"(O) : "memory");
+}
+template <int N>
+struct WordsOf;
+template <>
+struct WordsOf<2> {
+    typedef u32x2 type;
+};
+template <>
+struct WordsOf<4> {
+    typedef u32x4 type;
+};
+template <int N>
+using Words = typename WordsOf<N>::type;
+// 16 tokens' product with the weights: four consecutive k a lane group.
+template <int DT>
+__device__ __forceinline__ f32x4 mfma16x16x16(u32x2 a, u32x2 b, f32x4 c) {
+    typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+    typedef short s16x4 __attribute__((ext_vector_type(4)));
+    if constexpr (DT == kDtF16)
+        return __builtin_amdgcn_mfma_f32_16x16x16f16(__builtin_bit_cast(f16x4, a), __builtin_bit_cast(f16x4, b), c, 0,
+                                                     0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(s16x4, a), __builtin_bit_cast(s16x4, b), c,
+                                                         0, 0, 0);
 }
 // Two fp32 -> one dword of 16-bit elements (round to nearest even).
 template <int DT>
@@ -414,7 +441,7 @@ __device__ __forceinline__ uint32_t lds_address(const void* p) {
 }
 
 template <int DT, int D, int BS, int NCB>
-__global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(waves_of(DT, D, NCB))))
+__global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(2)))
 void attn_shared_stream(FastParams f, const int32_t* __restrict__ bt, const uint64_t* __restrict__ offs,
                         const uint8_t* __restrict__ kreg, const uint8_t* __restrict__ vreg) {
     constexpr bool F8 = DT == kDtFP8;
@@ -422,11 +449,15 @@ void attn_shared_stream(FastParams f, const int32_t* __restrict__ bt, const uint
     constexpr int EB = F8 ? 1 : 2;
     constexpr int KC = D / 32, DB = D / 16;
     constexpr int ROWB = D * EB;               // bytes of a token's head row
-    constexpr int HALF = 32 * ROWB;            // of a tile's K, and of its V
+    constexpr int TILE = tile_tokens(ROWB), NH = TILE / 16;   // tokens of a tile, 16-token halves
+    constexpr int GROUPS = TILE / 8;           // 8-token groups, each inside a page
+    constexpr int HALF = TILE * ROWB;          // bytes of a tile's K, and of its V
     constexpr int LOADS = 2 * HALF / 1024;     // of a tile
     constexpr int ST = 2;                      // tiles of the ring
     static_assert(!F8 || D == 128, "fp8 pages take this path at head_dim 128");
     __shared__ Items it;
+    __shared__ int s_key[kWaves], s_began[kWaves];
+    __shared__ float2 s_ml[kWaves][NCB * 16];
     __shared__ __attribute__((aligned(1024))) uint8_t s_ring[kWaves][ST * 2 * HALF];
     const SharedParams& p = f.p;
     const int lane = threadIdx.x & 63;
@@ -436,7 +467,7 @@ void attn_shared_stream(FastParams f, const int32_t* __restrict__ bt, const uint
     const int Hkv = p.kv_heads, Hq = p.num_q_heads, G = f.group;
     auto uni = [](int x) { return __builtin_amdgcn_readfirstlane(x); };
 
-    find_items(f, it);
+    find_items<TILE>(f, it);
     int pre_all = 0, own_all = 0;
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) {
@@ -446,31 +477,34 @@ void attn_shared_stream(FastParams f, const int32_t* __restrict__ bt, const uint
     const int pre_end = uni(pre_all) * Hkv, total = pre_end + uni(own_all) * Hkv;
     const int per = slice_tiles(total, f);
     if (blockIdx.x == 0) {
-        if (threadIdx.x == 0) *f.per = per;
+        if (threadIdx.x == 0) {
+            f.per[0] = per;
+            f.per[1] = total;
+        }
         const int r = threadIdx.x;
         if (r < f.rows) {
             RowPlan w{};
             w.own_tile = pre_end + it.own[r] * Hkv;
-            w.own_tiles = tiles_of(it.len[r] - it.common[r]);
+            w.own_tiles = tiles_of(it.len[r] - it.common[r], TILE);
             if (it.common[r] > 0) {
                 const int from = max(it.lead[r] - f.row0, 0), first = from + (r - from) / f.seqs * f.seqs;
                 w.first = f.row0 + first;
                 w.pre_tile = it.pre[first] * Hkv;
-                w.pre_tiles = tiles_of(it.common[r]);
+                w.pre_tiles = tiles_of(it.common[r], TILE);
             }
             f.plan[r] = w;
         }
     }
     const int slice = static_cast<int>(blockIdx.x) * kWaves + wave;
-    const long long t0l = static_cast<long long>(slice) * per;
-    if (t0l >= total) return;
-    const int t0 = static_cast<int>(t0l), n = min(per, total - t0);
+    if (static_cast<long long>(blockIdx.x) * kWaves * per >= total) return;   // (the whole workgroup)
+    const int t0 = static_cast<int>(min(static_cast<long long>(slice) * per, static_cast<long long>(total)));
+    const int n = min(per, total - t0);   // 0: nothing left for this wave
 
-    // Cursor over the tile list: tokens begin + 32 t .. of (item, kv head); all of it
+    // Cursor over the tile list: tokens begin + TILE t .. of (item, kv head); all of it
     // wave-uniform, so that the tables are read by scalar loads
     struct Cur {
         int r, own, g, t, nt, begin, end, shared, lead, seqs, blocks;
-        float ks[F8 ? 4 : 1], vs[F8 ? 4 : 1];   // fp8: page scales of the 8-token groups
+        float ks[F8 ? GROUPS : 1], vs[F8 ? GROUPS : 1];   // fp8: page scales of the 8-token groups
     };
     auto locate = [&](int tile) __attribute__((always_inline)) {
         Cur c;
@@ -490,20 +524,20 @@ void attn_shared_stream(FastParams f, const int32_t* __restrict__ bt, const uint
         c.end = c.own ? uni(it.len[lo]) : common;
         c.shared = c.own ? uni(it.shared[lo]) : common;
         c.lead = max(uni(it.lead[lo]), 0);
-        c.nt = max(tiles_of(c.end - c.begin), 1);
+        c.nt = max(tiles_of(c.end - c.begin, TILE), 1);
         const int rem = rel - uni(sums[lo]) * Hkv;
         c.g = rem / c.nt;
         c.t = rem - c.g * c.nt;
         return c;
     };
-    Cur ic = locate(t0);
+    Cur ic = locate(min(t0, total - 1));
     // (tile: the cursor's new place in the list)
     auto advance = [&](Cur& c, int tile) __attribute__((always_inline)) {
         if (++c.t < c.nt) return;
         c.t = 0;
         if (++c.g == Hkv) c = locate(tile);
     };
-    // Byte offsets of 64 8-token groups' rows (16 tiles), a lane each, from tile
+    // Byte offsets of 64 8-token groups' rows (512 tokens), a lane each, from tile
     // `from` of (sequence, kind) on; groups past the end repeat the last one
     // (masked).  They hold for every kv head.  What is loaded here is waited for at
     // once: a register that a load may still be on its way to would have every later
@@ -515,12 +549,13 @@ void attn_shared_stream(FastParams f, const int32_t* __restrict__ bt, const uint
         float ks, vs;                    // fp8: the groups' page scales of kv head g
     } pages;
     pages.r = -1;
-    // Where the tile's four groups lie for the tile's kv head (fp8: also their scales)
+    constexpr int AHEAD = 64 / GROUPS;   // tiles of these
+    // Where the tile's groups lie for the tile's kv head (fp8: also their scales)
     auto group_bases = [&](Cur& c, uint64_t* gb) __attribute__((always_inline)) {
         bool fresh = false;
-        if (pages.r != c.r || pages.own != c.own || (c.t & ~15) != pages.from) {
-            pages.from = c.t & ~15;
-            const int tok = c.begin + min(32 * pages.from + 8 * lane, (c.end - 1 - c.begin) & ~7);
+        if (pages.r != c.r || pages.own != c.own || c.t / AHEAD * AHEAD != pages.from) {
+            pages.from = c.t / AHEAD * AHEAD;
+            const int tok = c.begin + min(TILE * pages.from + 8 * lane, (c.end - 1 - c.begin) & ~7);
             const int row = tok < c.shared ? c.lead : f.row0 + c.r, block = tok / bs;
             const uint64_t page = offs[bt[static_cast<size_t>(row) * p.mbps + block]];
             pages.slot = static_cast<uint32_t>((tok - block * bs) * p.row_bytes);
@@ -539,8 +574,8 @@ void attn_shared_stream(FastParams f, const int32_t* __restrict__ bt, const uint
             }
         }
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            const int j = min(4 * c.t + q, (c.end - 1 - c.begin) >> 3) - 4 * pages.from;
+        for (int q = 0; q < GROUPS; ++q) {
+            const int j = min(GROUPS * c.t + q, (c.end - 1 - c.begin) >> 3) - GROUPS * pages.from;
             const uint32_t lo = __builtin_amdgcn_readlane(static_cast<uint32_t>(pages.row), j);
             const uint32_t hi = __builtin_amdgcn_readlane(static_cast<uint32_t>(pages.row >> 32), j);
             gb[q] = (static_cast<uint64_t>(hi) << 32 | lo) + static_cast<uint32_t>(c.g * D * EB);
@@ -570,7 +605,7 @@ void attn_shared_stream(FastParams f, const int32_t* __restrict__ bt, const uint
     auto issue = [&](uint32_t place, const uint64_t* gb) __attribute__((always_inline)) {
         uint8_t* const to = ring + place;
 #pragma unroll
-        for (int i = 0; i < 32 / ROWS; ++i) {
+        for (int i = 0; i < TILE / ROWS; ++i) {
             const uint64_t g = gb[i * ROWS / 8];
             load_lds16_nt(kreg + g + src[i % STEP], to + i * 1024);
             load_lds16_nt(vreg + g + src[i % STEP], to + HALF + i * 1024);
@@ -611,28 +646,29 @@ void attn_shared_stream(FastParams f, const int32_t* __restrict__ bt, const uint
     };
     clear();
 
-    // The part of the (item, kv head) that the wave has been through.  The part where
-    // a (sequence, head) begins has a row of its own; later ones are the slice's, in
-    // the order of the registers, which makes whole lines of the stores.
-    auto flush = [&](const Cur& c, bool began_here) __attribute__((always_inline)) {
-        float* const to_ml = began_here ? f.ml : f.slice_ml;
+    // Where a part's outputs and its (maximum, sum) go: the part where a (sequence,
+    // head) begins has a row of its own; later ones have the slice's place, in the
+    // order of the registers, which makes whole lines of the stores.
+    auto part_acc = [&](const Cur& c, bool begins, int slice, int cb) __attribute__((always_inline)) {
+        const int row = (c.own * f.rows + c.r + seq_of[cb]) * Hq + c.g * G + head_of[cb];
+        return begins ? f.acc + static_cast<size_t>(row) * D + 4 * lg
+                      : f.slice_acc + static_cast<size_t>(slice * NCB + cb) * (16 * D) + lane * 4;
+    };
+    auto part_ml = [&](const Cur& c, bool begins, int slice, int cb) __attribute__((always_inline)) {
+        const int row = (c.own * f.rows + c.r + seq_of[cb]) * Hq + c.g * G + head_of[cb];
+        return reinterpret_cast<float2*>(begins ? f.ml : f.slice_ml) + (begins ? row : (slice * NCB + cb) * 16 + ln);
+    };
+    auto flush = [&](const Cur& c, bool begins) __attribute__((always_inline)) {
 #pragma unroll
         for (int cb = 0; cb < NCB; ++cb) {
             if (cb >= c.blocks) break;
             const float l = wave_sum_across_groups(l_run[cb]);
-            const uint32_t row = static_cast<uint32_t>((c.own * f.rows + c.r + seq_of[cb]) * Hq + c.g * G + head_of[cb]);
-            const uint32_t block = static_cast<uint32_t>(slice * NCB + cb);
-            float* pa = began_here ? f.acc + static_cast<size_t>(row) * D + 4 * lg
-                                   : f.slice_acc + static_cast<size_t>(block) * (16 * D) + lane * 4;
-            const int step = began_here ? 16 : 256;
             if (seq_of[cb] >= c.seqs) continue;
+            float* const to = part_acc(c, begins, slice, cb);
+            const int step = begins ? 16 : 256;
 #pragma unroll
-            for (int db = 0; db < DB; ++db) *reinterpret_cast<f32x4*>(pa + db * step) = acc[cb][db];
-            if (lg == 0) {
-                const size_t at = 2 * static_cast<size_t>(began_here ? row : block * 16 + ln);
-                to_ml[at] = m_run[cb];
-                to_ml[at + 1] = l;
-            }
+            for (int db = 0; db < DB; ++db) *reinterpret_cast<f32x4*>(to + db * step) = acc[cb][db];
+            if (lg == 0) *part_ml(c, begins, slice, cb) = float2{m_run[cb], l};
         }
         clear();
     };
@@ -641,29 +677,24 @@ void attn_shared_stream(FastParams f, const int32_t* __restrict__ bt, const uint
     // and where it writes V's (fp8: as bf16, in padded rows)
     constexpr int NP = F8 ? KC / 2 : KC;
     const uint32_t at0 = lds_address(ring);
-    uint32_t k_at[NP], v_at[DB];
-#pragma unroll
-    for (int i = 0; i < NP; ++i) k_at[i] = at0 + turned(ln, 4 * i + lg);
+    const uint32_t k_at = at0 + turned(ln, lg);   // piece 4 i + lg: 64 i bytes of the turn
     // (V's rows as they are read: 2 D bytes, turned as rows of that length are)
     auto v_turned = [](int row, int piece) __attribute__((always_inline)) {
         return row * 2 * D + (D == 128 ? piece ^ (row & 15) : piece ^ (row >> 1 & 7)) * 16;
     };
-#pragma unroll
-    for (int db = 0; db < DB; ++db) {
-        const int row = 4 * lg + (ln >> 2);
-        v_at[db] = at0 + v_turned(row, 2 * db + ((ln & 3) >> 1)) + (ln & 1) * 8;
-    }
+    // (block db: 32 db bytes of the turn)
+    const uint32_t v_at = at0 + v_turned(4 * lg + (ln >> 2), (ln & 3) >> 1) + (ln & 1) * 8;
     auto compute = [&](uint32_t place, const Cur& c) __attribute__((always_inline)) {
         constexpr int TK = 0, TV = HALF;
-        const int tbase = c.begin + c.t * 32;
+        const int tbase = c.begin + c.t * TILE;
         // rows past the end may hold anything and become zeros
-        if (tbase + 32 > c.end)
-            for (int row = c.end - tbase + lane / PIECES; row < 32; row += ROWS)
+        if (tbase + TILE > c.end)
+            for (int row = c.end - tbase + lane / PIECES; row < TILE; row += ROWS)
                 lds_write<TV>(at0 + place + row * ROWB + lane % PIECES * 16, u32x4{0, 0, 0, 0});
         uint32_t kp[NP];
 #pragma unroll
-        for (int i = 0; i < NP; ++i) kp[i] = k_at[i] + place;
-        u32x4 x[2][NP];
+        for (int i = 0; i < NP; ++i) kp[i] = (k_at + place) ^ (64 * i);
+        u32x4 x[NH][NP];
         lds_read<TK, TK + 16 * ROWB>(x, kp);
         if constexpr (F8) {
             // V as bf16 (exactly: the pages' scales go to P), over the tile's K and V
@@ -678,14 +709,14 @@ void attn_shared_stream(FastParams f, const int32_t* __restrict__ bt, const uint
                     lds_write<0>(at0 + place + v_turned(row, piece + 1), fp8x8_to_bf16(y[h][e][2], y[h][e][3]));
                 }
         }
-        u32x4 pf[NCB];
-        const bool live = tbase + 32 <= c.end;   // (uniform)
+        Words<2 * NH> pf[NCB];
+        const bool live = tbase + TILE <= c.end;   // (uniform)
 #pragma unroll
         for (int cb = 0; cb < NCB; ++cb) {
             if (cb >= c.blocks) break;   // (uniform: no column of the item lies here)
-            f32x4 s[2];
+            f32x4 s[NH];
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
+            for (int h = 0; h < NH; ++h) {
                 s[h] = f32x4{0, 0, 0, 0};
 #pragma unroll
                 for (int kc = 0; kc < KC; ++kc) {
@@ -694,10 +725,10 @@ void attn_shared_stream(FastParams f, const int32_t* __restrict__ bt, const uint
                     s[h] = mfma16x16x32<MDT>(a, qf[cb][kc], s[h]);
                 }
             }
-            float v[8], sum = 0.0f;
+            float v[4 * NH], sum = 0.0f;
             float mt = -INFINITY;
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
+            for (int h = 0; h < NH; ++h) {
                 float sc = f.scale_log2;
                 if constexpr (F8) sc *= lg < 2 ? c.ks[2 * h] : c.ks[2 * h + 1];
 #pragma unroll
@@ -718,14 +749,14 @@ void attn_shared_stream(FastParams f, const int32_t* __restrict__ bt, const uint
                 for (int i = 0; i < DB; ++i) acc[cb][i] *= corr;
             }
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
+            for (int i = 0; i < 4 * NH; ++i) {
                 v[i] = __builtin_amdgcn_exp2f(v[i] - m_run[cb]);
                 sum += v[i];
             }
             l_run[cb] += sum;
             if constexpr (F8) {
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
+                for (int h = 0; h < NH; ++h) {
                     const float vs = lg < 2 ? c.vs[2 * h] : c.vs[2 * h + 1];
 #pragma unroll
                     for (int r = 0; r < 4; ++r) v[h * 4 + r] *= vs;
@@ -733,22 +764,26 @@ void attn_shared_stream(FastParams f, const int32_t* __restrict__ bt, const uint
             }
             // slots (lg, i) of the P^T operand: token i < 4 ? 4 lg + i : 16 + 4 lg + i - 4
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
+            for (int i = 0; i < 2 * NH; ++i)
                 pf[cb][i] = pack2<MDT>(v[2 * i], v[2 * i + 1]);
         }
 #pragma unroll
         for (int d0 = 0; d0 < DB; d0 += 4) {
             // lane (ln, lg): V[4 lg .. +3][16 db + ln], and of the second half
-            u32x2 t[4][2];
-            const uint32_t at[4] = {v_at[d0] + place, v_at[d0 + 1] + place, v_at[d0 + 2] + place, v_at[d0 + 3] + place};
+            u32x2 t[4][NH];
+            const uint32_t v0 = v_at + place;
+            const uint32_t at[4] = {v0 ^ 32 * d0, v0 ^ 32 * (d0 + 1), v0 ^ 32 * (d0 + 2), v0 ^ 32 * (d0 + 3)};
             lds_read_turned<F8 ? 0 : TV, (F8 ? 0 : TV) + 32 * D>(t, at);
 #pragma unroll
             for (int cb = 0; cb < NCB; ++cb) {
                 if (cb >= c.blocks) break;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const u32x4 vt{t[e][0][0], t[e][0][1], t[e][1][0], t[e][1][1]};
-                    acc[cb][d0 + e] = mfma16x16x32<MDT>(vt, pf[cb], acc[cb][d0 + e]);
+                    if constexpr (NH == 2)
+                        acc[cb][d0 + e] = mfma16x16x32<MDT>(u32x4{t[e][0][0], t[e][0][1], t[e][1][0], t[e][1][1]},
+                                                            pf[cb], acc[cb][d0 + e]);
+                    else
+                        acc[cb][d0 + e] = mfma16x16x16<MDT>(t[e][0], pf[cb], acc[cb][d0 + e]);
                 }
             }
         }
@@ -756,20 +791,20 @@ void attn_shared_stream(FastParams f, const int32_t* __restrict__ bt, const uint
 
     // Tile i + 1 is in flight while tile i is consumed.
     Cur cq[ST];   // cursors of tiles i ..
-    uint64_t gb[4];
+    uint64_t gb[GROUPS];
     load_q(ic);
     bool began_here = ic.t == 0;
     group_bases(ic, gb);
     static_assert(ST == 2, "one tile before the loop");
     cq[0] = ic;
-    issue(0, gb);
+    if (n > 0) issue(0, gb);
     if (n > 1) {
         advance(ic, t0 + 1);
         group_bases(ic, gb);
     }
     // (one copy of the step: a wave runs it some ten times, and code that is not yet in
     // the instruction cache costs more than the moves)
-    uint32_t place = 0, fill = (ST - 1) * 2 * HALF;
+    uint32_t place = 0, fill = 2 * HALF;
 #pragma unroll 1
     for (int i = 0; i < n; ++i) {
         cq[ST - 1] = ic;
@@ -784,15 +819,70 @@ void attn_shared_stream(FastParams f, const int32_t* __restrict__ bt, const uint
             wait_loads<0>();
         }
         compute(place, cq[0]);
-        if (i == n - 1 || cq[0].t == cq[0].nt - 1) {
-            flush(cq[0], began_here);
-            if (i + 1 < n) load_q(cq[1]);   // a new (item, kv head)
-            began_here = true;
+        if (i + 1 < n) {
+            if (cq[0].t == cq[0].nt - 1) {
+                flush(cq[0], began_here);
+                load_q(cq[1]);   // a new (item, kv head)
+                began_here = true;
+            }
+            cq[0] = cq[1];
         }
-#pragma unroll
-        for (int e = 0; e + 1 < ST; ++e) cq[e] = cq[e + 1];
         fill = place;
-        place = place + 2 * HALF == ST * 2 * HALF ? 0 : place + 2 * HALF;
+        place ^= 2 * HALF;
+    }
+
+    // Waves whose slices end in the same (item, kv head) -- all but the first lie in it
+    // wholly -- make one part of theirs, in the place of the first's: a quarter of the
+    // parts of a long prefix.
+    const Cur& c = cq[0];
+    const int key = n > 0 ? (c.own * kMaxRows + c.r) * Hkv + c.g : -1;
+    if (lane == 0) {
+        s_key[wave] = key;
+        s_began[wave] = began_here;
+    }
+#pragma unroll
+    for (int cb = 0; cb < NCB; ++cb) {
+        const float l = wave_sum_across_groups(l_run[cb]);
+        if (lg == 0) s_ml[wave][cb * 16 + ln] = float2{m_run[cb], l};
+    }
+    __syncthreads();
+    int head = wave, last = wave;   // of the run of waves
+    while (head > 0 && uni(s_key[head - 1]) == key) --head;
+    while (last + 1 < kWaves && uni(s_key[last + 1]) == key) ++last;
+    const int run = key < 0 ? 0 : last - head + 1;
+    const bool begins = uni(s_began[head]) != 0;
+    constexpr int MOST = ST * 2 * HALF / (DB * 1024);   // column blocks that a ring takes
+    constexpr int PASS = MOST < NCB ? MOST : NCB;
+    static_assert(PASS >= 1 && NCB % PASS == 0, "outputs pass through the rings");
+#pragma unroll
+    for (int p0 = 0; p0 < NCB; p0 += PASS) {
+        f32x4* const mine = reinterpret_cast<f32x4*>(s_ring[wave]) + lane;
+#pragma unroll
+        for (int cb = p0; cb < p0 + PASS; ++cb) {
+            if (run == 0 || cb >= c.blocks) break;
+            float m = -INFINITY, l = 0.0f;
+            for (int w = head; w <= last; ++w) m = fmaxf(m, s_ml[w][cb * 16 + ln].x);
+            for (int w = head; w <= last; ++w)
+                l += s_ml[w][cb * 16 + ln].y * __builtin_amdgcn_exp2f(s_ml[w][cb * 16 + ln].x - m);
+            const float weight = __builtin_amdgcn_exp2f(m_run[cb] - m);
+#pragma unroll
+            for (int db = 0; db < DB; ++db) mine[((cb - p0) * DB + db) * 64] = acc[cb][db] * weight;
+            if (wave == head && lg == 0 && seq_of[cb] < c.seqs) *part_ml(c, begins, slice, cb) = float2{m, l};
+        }
+        __syncthreads();
+#pragma unroll
+        for (int cb = p0; cb < p0 + PASS; ++cb) {
+            if (run == 0 || cb >= c.blocks) break;
+            float* const to = part_acc(c, begins, slice - (wave - head), cb);
+            const int step = begins ? 16 : 256;
+            for (int db = wave - head; db < DB; db += run) {
+                f32x4 sum = f32x4{0, 0, 0, 0};
+                for (int w = head; w <= last; ++w)
+                    sum += reinterpret_cast<const f32x4*>(s_ring[w])[((cb - p0) * DB + db) * 64 + lane];
+                if (seq_of[cb] < c.seqs) *reinterpret_cast<f32x4*>(to + db * step) = sum;
+            }
+        }
+        if (p0 + PASS < NCB) __syncthreads();
     }
 }
 
@@ -810,26 +900,42 @@ __global__ __launch_bounds__(kJoinThreads) void attn_shared_join(FastParams f, i
     const int r = static_cast<int>(blockIdx.x) / p.kv_heads, g = static_cast<int>(blockIdx.x) - r * p.kv_heads;
     const int G = f.group, Hq = p.num_q_heads;
     const RowPlan w = f.plan[r];
-    const int per = *f.per;
+    const int per = f.per[0], total = f.per[1];
     uint16_t* out = reinterpret_cast<uint16_t*>(p.out) + (static_cast<size_t>(f.row0 + r) * Hq + g * G) * D;
     if (w.pre_tiles + w.own_tiles == 0) {
         for (int e = tid; e < G * D; e += kJoinThreads) out[e] = 0;
         return;
     }
-    // first slice and slices of the two kinds of parts
-    const int pre0 = w.pre_tile + g * w.pre_tiles, own0 = w.own_tile + g * w.own_tiles;
-    const int pre_at = pre0 / per, own_at = own0 / per;
-    const int pre_n = w.pre_tiles == 0 ? 0 : (pre0 + w.pre_tiles - 1) / per - pre_at + 1;
-    const int own_n = w.own_tiles == 0 ? 0 : (own0 + w.own_tiles - 1) / per - own_at + 1;
-    const int parts = pre_n + own_n;
+    // The parts of a run of tiles from `first` on: of each workgroup whose slices lie in
+    // it one, by the place of its first such slice (the first of all in the row of its
+    // own), and, where a slice goes on behind the run's end, that slice's.
+    struct Parts {
+        int first, wgs, n, last;
+    };
+    auto parts_of = [&](int first, int tiles) {
+        Parts q{};
+        if (tiles == 0) return q;
+        q.first = first / per;
+        q.last = (first + tiles - 1) / per;
+        const bool on = static_cast<long long>(q.last + 1) * per > first + tiles && first + tiles < total;
+        const int whole = q.last - on;   // the last slice that ends in the run
+        q.wgs = whole >= q.first ? whole / kWaves - q.first / kWaves + 1 : 0;
+        q.n = q.wgs + on;
+        return q;
+    };
+    const Parts pre = parts_of(w.pre_tile + g * w.pre_tiles, w.pre_tiles);
+    const Parts own = parts_of(w.own_tile + g * w.own_tiles, w.own_tiles);
+    const int parts = pre.n + own.n;
     const int shift = (f.row0 + r - w.first) * G;   // its columns in the item's slices
     // the row of part k's column of head 0: in the first parts' rows, or of a slice
     auto place = [&](int k, bool* first) -> size_t {
-        const bool own = k >= pre_n;
-        if (own) k -= pre_n;
+        const bool mine = k >= pre.n;
+        const Parts& q = mine ? own : pre;
+        if (mine) k -= pre.n;
+        const int slice = k >= q.wgs ? q.last : k == 0 ? q.first : (q.first / kWaves + k) * kWaves;
         *first = k == 0;
-        if (k == 0) return static_cast<size_t>(own * f.rows + r) * Hq + g * G;
-        return static_cast<size_t>((own ? own_at : pre_at) + k) * slot_cols + (own ? 0 : shift);
+        if (k == 0) return static_cast<size_t>(mine * f.rows + r) * Hq + g * G;
+        return static_cast<size_t>(slice) * slot_cols + (mine ? 0 : shift);
     };
     // outputs 4 q .. of heads 0 ..: q % (D / 4) of a row's, of a slice by its registers' order
     auto outputs = [&](int k, int q) {
@@ -913,15 +1019,16 @@ __global__ __launch_bounds__(kJoinThreads) void attn_shared_join(FastParams f, i
     }
 }
 
-// Column blocks of an item: as many as a group's query rows fill, up to 64 columns.
-int column_blocks(long long rows_of_a_group) { return rows_of_a_group <= 16 ? 1 : rows_of_a_group <= 32 ? 2 : 4; }
-int slices_of(int dtype, int d, int ncb) { return 1024 * waves_of(dtype, d, ncb); }
+// Column blocks of an item: two of 128 elements, or four of 64, are what half of a
+// SIMD's registers hold; one where a group has few query rows a kv head.
+constexpr int kSlices = 2048;   // two workgroups of four waves a CU
+int column_blocks(int d, long long rows) { return rows <= 8 ? 1 : d == 64 ? 4 : 2; }
 
 // Where things lie in the scratch of a launch of `rows` sequences.
 struct Layout {
     size_t per, plan, ml, slice_ml, acc, slice_acc, bytes;
 };
-Layout layout_of(int dtype, int rows, int hq, int d, int ncb) {
+Layout layout_of(int rows, int hq, int d, int ncb) {
     Layout l{};
     size_t at = 0;
     auto take = [&](size_t bytes) {
@@ -929,8 +1036,8 @@ Layout layout_of(int dtype, int rows, int hq, int d, int ncb) {
         at += (bytes + 255) & ~size_t(255);
         return here;
     };
-    const size_t firsts = size_t(2) * rows * hq, later = static_cast<size_t>(slices_of(dtype, d, ncb)) * 16 * ncb;
-    l.per = take(sizeof(int));
+    const size_t firsts = size_t(2) * rows * hq, later = static_cast<size_t>(kSlices) * 16 * ncb;
+    l.per = take(2 * sizeof(int));
     l.plan = take(static_cast<size_t>(rows) * sizeof(RowPlan));
     l.ml = take(firsts * 8);
     l.slice_ml = take(later * 8);
@@ -953,17 +1060,17 @@ bool launch_fast(const SharedParams& p, uint64_t scratch, hipStream_t s, std::st
     f.group = p.num_q_heads / p.kv_heads;
     f.seqs = 16 * NCB / f.group;
     f.scale_log2 = p.scale * 1.4426950408889634f;
-    f.slices = slices_of(DT, D, NCB);
+    f.slices = kSlices;
     f.least = 1;
     const long long cap = static_cast<long long>(p.mbps) * p.block_size;
     for (int row0 = 0; row0 < p.batch; row0 += kMaxRows) {
         f.row0 = row0;
         f.rows = std::min(kMaxRows, p.batch - row0);
-        if (2LL * f.rows * p.kv_heads * ((cap + 31) / 32) > (1LL << 30)) {
+        if (2LL * f.rows * p.kv_heads * ((cap + 15) / 16) > (1LL << 30)) {
             *err = "batch x context too large";
             return false;
         }
-        const Layout l = layout_of(DT, f.rows, p.num_q_heads, D, NCB);
+        const Layout l = layout_of(f.rows, p.num_q_heads, D, NCB);
         auto at = [&](size_t o) { return reinterpret_cast<float*>(scratch + o); };
         f.per = reinterpret_cast<int*>(scratch + l.per);
         f.plan = reinterpret_cast<RowPlan*>(scratch + l.plan);
@@ -972,7 +1079,7 @@ bool launch_fast(const SharedParams& p, uint64_t scratch, hipStream_t s, std::st
         f.acc = at(l.acc);
         f.slice_acc = at(l.slice_acc);
         // no more workgroups than the tables hold tiles for
-        const long long most = 2LL * f.rows * p.kv_heads * ((cap + 31) / 32);
+        const long long most = 2LL * f.rows * p.kv_heads * ((cap + 15) / 16);
         const unsigned wgs = static_cast<unsigned>(std::min<long long>(f.slices, most) + kWaves - 1) / kWaves;
         auto run = [&](auto bs) {
             hipLaunchKernelGGL((attn_shared_stream<DT, D, decltype(bs)::value, NCB>), dim3(wgs),
@@ -991,11 +1098,8 @@ bool launch_fast(const SharedParams& p, uint64_t scratch, hipStream_t s, std::st
 template <int DT, int D>
 bool launch_columns(const SharedParams& p, uint64_t scratch, hipStream_t s, std::string* err) {
     const long long rows = static_cast<long long>(p.batch) * (p.num_q_heads / p.kv_heads) / p.groups;
-    switch (column_blocks(rows)) {
-        case 1: return launch_fast<DT, D, 1>(p, scratch, s, err);
-        case 2: return launch_fast<DT, D, 2>(p, scratch, s, err);
-        default: return launch_fast<DT, D, 4>(p, scratch, s, err);
-    }
+    return column_blocks(D, rows) == 1 ? launch_fast<DT, D, 1>(p, scratch, s, err)
+                                       : launch_fast<DT, D, D == 64 ? 4 : 2>(p, scratch, s, err);
 }
 
 }  // namespace
@@ -1006,10 +1110,8 @@ uint64_t attn_shared_scratch_bytes(int32_t dtype, uint32_t batch, uint32_t num_q
                                    uint32_t head_dim, uint32_t block_size, uint32_t) {
     if (!fast_shape(dtype, num_q_heads, kv_heads, head_dim, block_size)) return 256;
     const int rows = static_cast<int>(std::min<uint32_t>(batch, kMaxRows));
-    size_t most = 0;
-    for (int ncb : {1, 2, 4})
-        most = std::max(most, layout_of(dtype, rows, static_cast<int>(num_q_heads), static_cast<int>(head_dim), ncb).bytes);
-    return most;
+    const int hq = static_cast<int>(num_q_heads), d = static_cast<int>(head_dim);
+    return std::max(layout_of(rows, hq, d, 1).bytes, layout_of(rows, hq, d, column_blocks(d, INT_MAX)).bytes);
 }
 
 bool attn_shared(const AttnSharedArgs& a, std::string* err) {
