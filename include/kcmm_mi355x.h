@@ -625,8 +625,8 @@ typedef struct kcmm_lora {
  *  once; what one token holds, infinities and NaN too, reaches no other token,
  *  nor does what an adapter holds reach a token that has another.  y may be
  *  base.
- *  low_ptr: device memory of the caller's, fp32 [m][slices * rank], that takes
- *  the low-rank values x A^T of the tokens with an adapter.  Calls that may run at
+ *  low_ptr: scratch memory of the caller's, 4 m slices rank bytes, for the low-rank
+ *  values scales[a] x A_a^T (sums in fp32, kept to 2^-16 of each).  Calls that may run at
  *  the same time need one each.  1 <= m <= 2^20; n % 16 == 0, <= 2^22; k % 8 ==
  *  0, <= 2^20; rank % 8 == 0, <= 128; adapters <= 65535.  x, a, b, low, base and y
  *  aligned to 16 bytes; y (unless it is base) and low overlap nothing else.

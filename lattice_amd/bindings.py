@@ -398,7 +398,7 @@ class KcmmLibrary:
     def lora_add_bf16(self, x_ptr, a_ptr, b_ptr, adapter_ids_ptr, low_ptr, base_ptr, y_ptr, m, n, k,
                       *, adapters, rank, slice_ends=None, scales_ptr=0, stream_ptr=0) -> None:
         """y[t] = base[t] + scales[a] (x[t] A_a^T) B_a^T, a = adapter_ids[t] (outside 0 ..
-        adapters - 1: y[t] = base[t]); low: fp32 [m][slices * rank] of the caller's; y may be
+        adapters - 1: y[t] = base[t]); low: scratch, 4 m slices rank bytes; y may be
         base.  slice_ends: where the columns of the projection's parts end (default: one)."""
         ends = [n] if slice_ends is None else list(slice_ends)
         lora = KcmmLora(a_ptr, b_ptr, scales_ptr, adapters, rank, len(ends),

@@ -1,10 +1,31 @@
 // Low-rank adapters of many requests beside a shared projection (gfx950):
-//   y[t] = bf16(base[t] + scale_a (x[t] A_a^T) B_a^T),  a = adapter_ids[t],
+//   y[t] = bf16(base[t] + (scale_a x[t] A_a^T) B_a^T),  a = adapter_ids[t],
 // A_a [slices * rank][k] and B_a [n][rank] bf16; column n takes the rank values
-// of its slice.  A token without an adapter keeps base.  The low-rank values pass
-// through memory of the caller's, in fp32; y is rounded once.
+// of its slice.  A token without an adapter keeps base.  Two kernels: the low-rank
+// values v = scale x A^T go through memory of the caller's; y is rounded once.
+//
+// Both work on 16 tokens a block, in the order in which they come: a block's
+// tokens may have any adapters, and each of these takes its turn with all 16
+// columns of the matrix instruction, of which only its own tokens' are kept (a
+// column's values come from its own token alone, so what another token or adapter
+// holds, infinities too, goes nowhere).  Prompts have one adapter a block, decode
+// batches up to 16, whose weights are then what has to be read, once a block.
+//  * shrink: k dealt to the waves of a workgroup by lines of 128 bytes, their sums
+//    joined in LDS, in wave order.  A workgroup has 16 rows of A, or 64 where there
+//    are blocks enough, and one of the block's adapters, or several in turn.  Bound by
+//    what one CU loads (64 bytes a cycle).
+//  * expand: bound by base and y in HBM for prompts, by latency for few tokens.  The
+//    matrix instruction has 32 consecutive k and a rank seldom fills them, so the
+//    second parts of the values (below) are nearly free.
+// A CU's load path takes 8 lanes with one line of 128 bytes in 2 cycles but 8 lanes with a
+// line each in 8: operands read from rows straight into the matrix instruction's
+// layout cost 4 times the cycles of whole lines.  Hence the way through LDS in the
+// shrink, the layout of the low-rank values, and tokens as rows in the expand (3001
+// tokens, rank 32, k 4096, n 28672: 36 + 116 us with such reads, 16 + 70 without).
 #include <algorithm>
 #include <climits>
+#include <cmath>
+#include <type_traits>
 
 #include "../device_api.hpp"
 #include "common.hpp"
@@ -22,42 +43,359 @@ struct LoraParams {
     const uint16_t* base;
     uint16_t* y;
     int m, n, k, adapters, rank, slices, rows;   // rows = slices * rank
-    int ends[4];
+    int ends[4];                                 // of the slices' columns
+    int chunks[4];                               // end of the slices' column chunks
 };
 
-// One wave a low-rank value.
-__global__ __launch_bounds__(256) void lora_shrink_simple(LoraParams p) {
-    const int lane = threadIdx.x & 63;
-    const int t = blockIdx.x, r = blockIdx.y * 4 + (threadIdx.x >> 6);
-    const int id = p.ids[t];
-    if (static_cast<uint32_t>(id) >= static_cast<uint32_t>(p.adapters) || r >= p.rows) return;
-    const uint16_t* x = p.x + static_cast<size_t>(t) * p.k;
-    const uint16_t* a = p.a + (static_cast<size_t>(id) * p.rows + r) * p.k;
-    float sum = 0.0f;
-    for (int i = lane; i < p.k; i += 64) sum += bf16_bits_to_f32(x[i]) * bf16_bits_to_f32(a[i]);
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
-    if (lane == 0) p.low[static_cast<size_t>(t) * p.rows + r] = sum;
+__device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c,
+                                                   0, 0, 0);
 }
 
-// One thread an output.
-__global__ __launch_bounds__(256) void lora_expand_simple(LoraParams p) {
-    const int t = blockIdx.x, c = blockIdx.y * 256 + threadIdx.x;
-    if (c >= p.n) return;
-    const size_t at = static_cast<size_t>(t) * p.n + c;
-    const int id = p.ids[t];
-    if (static_cast<uint32_t>(id) >= static_cast<uint32_t>(p.adapters)) {
-        p.y[at] = p.base[at];
-        return;
+// Adapter of token t, or -1.
+__device__ __forceinline__ int adapter_of(const LoraParams& p, int t) {
+    const int id = t < p.m ? p.ids[t] : -1;
+    return static_cast<uint32_t>(id) < static_cast<uint32_t>(p.adapters) ? id : -1;
+}
+
+// Takes the first adapter of the tokens still to be served out of their set: a bit
+// for each of the block's tokens; -1 when none is left.
+__device__ __forceinline__ int next_adapter(int id, uint32_t* left) {
+    if (*left == 0) return -1;
+    const int a = __builtin_amdgcn_readlane(id, __ffs(static_cast<int>(*left)) - 1);
+    *left &= ~static_cast<uint32_t>(__ballot(id == a));
+    return a;
+}
+
+// Rows of 128 bytes of k in LDS, one wave's own: piece j of 16 bytes of row r lies at
+// r * 128 + 16 (j ^ (r & 7)), so that writes of whole rows and reads of one piece of
+// 16 rows both pass all banks.
+__device__ __forceinline__ u32x4* piece_at(u32x4* rows, int row, int piece) {
+    return rows + row * 8 + (piece ^ (row & 7));
+}
+
+// Low-rank values, 4 bytes each, of a block of 16 tokens (`count` of them in the last
+// block), in the order in which the second product reads them: by slices, 2 P pieces
+// of 8 values (P = rank / 8) of all tokens side by side; the first P their bf16
+// values, the others what these leave, bf16 too.  2^-16 of a value is lost so, a 2^-8th
+// of what the rounding of y is.
+struct LowBlock {
+    u32x4* at;
+    int count;
+    __device__ LowBlock(const LoraParams& p, int block, int slice)
+        : at(reinterpret_cast<u32x4*>(p.low + static_cast<size_t>(block) * 16 * p.rows)),
+          count(min(16, p.m - 16 * block)) {
+        at += slice * (p.rank / 4) * count;
     }
-    int s = 0;
-    while (c >= p.ends[s]) ++s;
-    const float* low = p.low + static_cast<size_t>(t) * p.rows + s * p.rank;
-    const uint16_t* b = p.b + (static_cast<size_t>(id) * p.n + c) * p.rank;
-    float sum = 0.0f;
-    for (int r = 0; r < p.rank; ++r) sum += low[r] * bf16_bits_to_f32(b[r]);
-    const float scale = p.scales != nullptr ? p.scales[id] : 1.0f;
-    p.y[at] = static_cast<uint16_t>(f32_to_bf16_bits(bf16_bits_to_f32(p.base[at]) + scale * sum));
+    __device__ u32x4* piece(int q, int token) const { return at + q * count + token; }
+};
+
+// Workgroup (block of 16 tokens, turn, row group): RB * 16 low-rank rows for the
+// turn-th, turn + turns-th ... of the block's adapters.  A wave loads whole lines of 128
+// bytes, 8 lanes a row, U of them before it uses the first.
+template <int RB, int NW, int U>
+__global__ __launch_bounds__(64 * NW) void lora_shrink(LoraParams p, int turns) {
+    constexpr int LOADS = 2 + 2 * RB;   // of 8 rows each: the tokens', the weights'
+    __shared__ u32x4 s_rows[NW][LOADS * 64];
+    const int lane = threadIdx.x & 63, ln = lane & 15, lg = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6);
+    u32x4* const rows = s_rows[wave];
+    const int t0 = blockIdx.x * 16, row0 = blockIdx.z * (RB * 16);
+    const int id = adapter_of(p, t0 + ln);
+    uint32_t left = static_cast<uint32_t>(__ballot(id >= 0)) & 0xffffu;
+    const int pieces = p.k / 8, lines = (pieces + 7) / 8;
+    for (int turn = 0;; ++turn) {
+        const int first = __ffs(static_cast<int>(left)) - 1, a = next_adapter(id, &left);
+        if (a < 0) break;
+        if (turn % turns != static_cast<int>(blockIdx.y)) continue;
+        const bool mine = id == a;
+        const uint32_t ours = static_cast<uint32_t>(__ballot(mine));
+        const uint16_t* src[LOADS];
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) {
+            const int r = 8 * i + (lane >> 3);
+            // a column of no token of this adapter's takes the first one's values along
+            src[i] = i < 2 ? p.x + static_cast<size_t>(t0 + (ours >> r & 1 ? r : first)) * p.k
+                           : p.a + (static_cast<size_t>(a) * p.rows + min(row0 + r - 16, p.rows - 1)) * p.k;
+        }
+        f32x4 sum[RB];
+#pragma unroll
+        for (int i = 0; i < RB; ++i) sum[i] = f32x4{0, 0, 0, 0};
+        // Lines l, l + NW ... l + (U - 1) NW; the last ones may be partial or past the row
+        auto lines_of = [&](int l, auto tail) __attribute__((always_inline)) {
+            u32x4 v[U][LOADS];
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int i = 0; i < LOADS; ++i) {
+                    const int piece = (l + u * NW) * 8 + (lane & 7);
+                    v[u][i] = *reinterpret_cast<const u32x4*>(
+                        src[i] + static_cast<uint32_t>(tail && piece >= pieces ? 0 : piece) * 8);
+                }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const bool in = !tail || (l + u * NW) * 8 + (lane & 7) < pieces;
+#pragma unroll
+                for (int i = 0; i < LOADS; ++i)
+                    *piece_at(rows, 8 * i + (lane >> 3), lane & 7) = in ? v[u][i] : u32x4{0, 0, 0, 0};
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const u32x4 x = *piece_at(rows, ln, 4 * h + lg);
+#pragma unroll
+                    for (int i = 0; i < RB; ++i)
+                        sum[i] = mfma(*piece_at(rows, 16 * (i + 1) + ln, 4 * h + lg), x, sum[i]);
+                }
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            }
+        };
+        int l = wave;
+#pragma clang loop unroll(disable)
+        for (; (l + (U - 1) * NW + 1) * 8 <= pieces; l += NW * U) lines_of(l, std::false_type{});
+        if (l < lines) lines_of(l, std::true_type{});
+        // the waves' sums, each in the place of its lines
+#pragma unroll
+        for (int i = 0; i < RB; ++i) rows[i * 64 + lane] = __builtin_bit_cast(u32x4, sum[i]);
+        __syncthreads();
+        const float scale = p.scales != nullptr ? p.scales[a] : 1.0f;
+        for (int i = wave; i < RB; i += NW) {
+            f32x4 v = {0, 0, 0, 0};
+            for (int j = 0; j < NW; ++j) v += __builtin_bit_cast(f32x4, s_rows[j][i * 64 + lane]);
+            float part[8];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                // (a value that bf16 takes for an infinity leaves nothing)
+                v[e] *= scale;
+                part[e] = bf16_round_hw(v[e]);
+                part[4 + e] = fabsf(part[e]) < INFINITY ? v[e] - part[e] : 0.0f;
+            }
+            // rows 4 lg .. +3 of each 16, of token ln: half a piece
+            const int row = row0 + 16 * i + 4 * lg;
+            if (mine && row < p.rows) {
+                const int slice = row / p.rank, q = (row - slice * p.rank) / 8;
+                const LowBlock low(p, blockIdx.x, slice);
+                const u32x4 o = pack_bf16x8(part);
+                reinterpret_cast<u32x2*>(low.piece(q, ln))[row >> 2 & 1] = u32x2{o[0], o[1]};
+                reinterpret_cast<u32x2*>(low.piece(p.rank / 8 + q, ln))[row >> 2 & 1] = u32x2{o[2], o[3]};
+            }
+        }
+        __syncthreads();
+    }
+}
+
+// The columns of a chunk: `width` of one slice.
+struct Columns {
+    int slice, n0, end;
+    __device__ bool find(const LoraParams& p, int chunk, int width) {
+        slice = 0;
+        while (slice < p.slices && chunk >= p.chunks[slice]) ++slice;
+        if (slice == p.slices) return false;
+        end = p.ends[slice];
+        n0 = (slice > 0 ? p.ends[slice - 1] : 0) + (chunk - (slice > 0 ? p.chunks[slice - 1] : 0)) * width;
+        return true;
+    }
+};
+
+// The piece of a token's values that lane group lg has in step k, and the piece of the
+// weights that goes with it.
+struct Piece {
+    int value, weight;
+    bool in;
+    __device__ Piece(int k, int lg, int P) {
+        in = 4 * k + lg < 2 * P;
+        value = in ? 4 * k + lg : 0;
+        weight = value < P ? value : value - P;
+    }
+};
+
+__device__ __forceinline__ float bf16_half(uint32_t pair, int which) {
+    return __uint_as_float(which ? pair & 0xffff0000u : pair << 16);
+}
+
+// Few tokens: a wave has 16 of them and 16 columns, and the weights of U adapters on
+// their way at once.
+template <int STEPS>
+__global__ __launch_bounds__(256) void lora_expand_few(LoraParams p) {
+    constexpr int U = STEPS <= 2 ? 8 : 4;
+    const int lane = threadIdx.x & 63, ln = lane & 15, lg = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6);
+    Columns columns;
+    if (!columns.find(p, blockIdx.x * 4 + wave, 16)) return;
+    const int t = blockIdx.y * 16 + ln, P = p.rank / 8;
+    const int id = adapter_of(p, t);
+    uint32_t left = static_cast<uint32_t>(__ballot(id >= 0)) & 0xffffu;
+    const size_t at = static_cast<size_t>(min(t, p.m - 1)) * p.n + columns.n0 + 4 * lg;
+    const u32x2 base = *reinterpret_cast<const u32x2*>(p.base + at);
+    const LowBlock low(p, blockIdx.y, columns.slice);
+    const uint16_t* const w = p.b + static_cast<size_t>(columns.n0 + ln) * p.rank;
+    u32x4 vf[STEPS];
+#pragma unroll
+    for (int k = 0; k < STEPS; ++k) {
+        const Piece q(k, lg, P);
+        vf[k] = *low.piece(q.value, min(ln, low.count - 1));
+        if (!q.in) vf[k] = u32x4{0, 0, 0, 0};
+    }
+    f32x4 acc = {0, 0, 0, 0};
+    while (left != 0) {
+        int a[U];
+        u32x4 wf[U][STEPS];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            a[u] = next_adapter(id, &left);
+            if (a[u] < 0) continue;
+#pragma unroll
+            for (int k = 0; k < STEPS; ++k)
+                wf[u][k] = *reinterpret_cast<const u32x4*>(w + static_cast<size_t>(a[u]) * p.n * p.rank +
+                                                          Piece(k, lg, P).weight * 8);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (a[u] < 0) continue;
+            f32x4 d = {0, 0, 0, 0};
+#pragma unroll
+            for (int k = 0; k < STEPS; ++k)
+                d = mfma(Piece(k, lg, P).in ? wf[u][k] : u32x4{0, 0, 0, 0}, vf[k], d);
+            if (id == a[u]) acc = d;
+        }
+    }
+    if (t >= p.m) return;
+    u32x2 out = base;
+    if (id >= 0) {
+        float v[8] = {};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = bf16_half(base[e >> 1], e & 1) + acc[e];
+        const u32x4 o = pack_bf16x8(v);
+        out = u32x2{o[0], o[1]};
+    }
+    *reinterpret_cast<u32x2*>(p.y + at) = out;
+}
+
+// Many tokens: a wave has NB * 16 columns and runs through `per` blocks of 16 tokens.
+// The tokens are the rows of its products, lane ln has the NB columns from ln * NB on, so
+// that 16 lanes read and write whole lines of base and y; the weights stay in registers
+// for as long as the adapter does, the next block's base and values are on their way
+// while one is worked on.
+template <int NB, int STEPS>
+__global__ __launch_bounds__(256) void lora_expand(LoraParams p, int per) {
+    typedef uint32_t Run __attribute__((ext_vector_type(NB / 2)));   // NB columns
+    const int lane = threadIdx.x & 63, ln = lane & 15, lg = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6);
+    Columns columns;
+    if (!columns.find(p, blockIdx.x * 4 + wave, NB * 16)) return;
+    const int P = p.rank / 8, blocks = (p.m + 15) / 16;
+    const int first = blockIdx.y * per, behind = min(first + per, blocks);
+    // past the slice's end its last columns, which are not stored
+    const bool stored = columns.n0 + ln * NB < columns.end;
+    const int column = min(columns.n0 + ln * NB, columns.end - NB);
+    const uint16_t* const w = p.b + static_cast<size_t>(column) * p.rank;
+
+    struct Block {
+        int id;
+        Run base[4];   // of tokens 4 lg .. +3
+        u32x4 v[STEPS];
+    };
+    auto load = [&](int block) __attribute__((always_inline)) {
+        Block r;
+        r.id = adapter_of(p, block * 16 + ln);
+        const LowBlock low(p, block, columns.slice);
+#pragma unroll
+        for (int k = 0; k < STEPS; ++k) r.v[k] = *low.piece(Piece(k, lg, P).value, min(ln, low.count - 1));
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            r.base[i] = __builtin_nontemporal_load(reinterpret_cast<const Run*>(
+                p.base + static_cast<size_t>(min(block * 16 + 4 * lg + i, p.m - 1)) * p.n + column));
+        return r;
+    };
+    int held = -1;
+    u32x4 wf[NB][STEPS];
+    auto finish = [&](int block, const Block& r) __attribute__((always_inline)) {
+        f32x4 acc[NB];
+#pragma unroll
+        for (int b = 0; b < NB; ++b) acc[b] = f32x4{0, 0, 0, 0};
+        const uint32_t any = static_cast<uint32_t>(__ballot(r.id >= 0)) & 0xffffu;
+        uint32_t left = any;
+        for (int a = next_adapter(r.id, &left); a >= 0; a = next_adapter(r.id, &left)) {
+            if (a != held) {
+                held = a;
+#pragma unroll
+                for (int b = 0; b < NB; ++b)
+#pragma unroll
+                    for (int k = 0; k < STEPS; ++k) {
+                        wf[b][k] = *reinterpret_cast<const u32x4*>(
+                            w + (static_cast<size_t>(a) * p.n + b) * p.rank + Piece(k, lg, P).weight * 8);
+                        if (!Piece(k, lg, P).in) wf[b][k] = u32x4{0, 0, 0, 0};
+                    }
+                // (here, and not for all loads after each block)
+                __builtin_amdgcn_s_waitcnt(0x0f70);
+            }
+            const uint32_t ours = static_cast<uint32_t>(__ballot(r.id == a)) >> (4 * lg);
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+                f32x4 d = {0, 0, 0, 0};
+#pragma unroll
+                for (int k = 0; k < STEPS; ++k)
+                    d = mfma(Piece(k, lg, P).in ? r.v[k] : u32x4{0, 0, 0, 0}, wf[b][k], d);
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (ours >> i & 1) acc[b][i] = d[i];
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int t = block * 16 + 4 * lg + i;
+            float v[8] = {};
+#pragma unroll
+            for (int b = 0; b < NB; ++b) v[b] = bf16_half(r.base[i][b >> 1], b & 1) + acc[b][i];
+            const u32x4 o = pack_bf16x8(v);
+            Run out;
+#pragma unroll
+            for (int e = 0; e < NB / 2; ++e) out[e] = any >> (4 * lg + i) & 1 ? o[e] : r.base[i][e];
+            if (t < p.m && stored)
+                __builtin_nontemporal_store(out, reinterpret_cast<Run*>(p.y + static_cast<size_t>(t) * p.n + column));
+        }
+    };
+    Block one = load(first);
+    for (int block = first; block < behind; block += 2) {
+        const Block two = load(min(block + 1, behind - 1));
+        finish(block, one);
+        one = load(min(block + 2, behind - 1));
+        if (block + 1 < behind) finish(block + 1, two);
+    }
+}
+
+template <int RB, int NW, int U>
+void launch_shrink(const LoraParams& p, hipStream_t s) {
+    const int blocks = (p.m + 15) / 16, groups = (p.rows + 16 * RB - 1) / (16 * RB);
+    const int turns = std::max(1, std::min({16, p.adapters, 256 / (blocks * groups)}));
+    hipLaunchKernelGGL((lora_shrink<RB, NW, U>), dim3(blocks, turns, groups), dim3(64 * NW), 0, s, p, turns);
+}
+
+// Chunks of `width` columns; returns their number.
+int deal_columns(LoraParams& p, int width) {
+    int chunks = 0;
+    for (int i = 0; i < p.slices; ++i) {
+        chunks += (p.ends[i] - (i > 0 ? p.ends[i - 1] : 0) + width - 1) / width;
+        p.chunks[i] = chunks;
+    }
+    return chunks;
+}
+
+template <int NB, int STEPS>
+void launch_expand(LoraParams& p, hipStream_t s) {
+    const int chunks = deal_columns(p, 16 * NB);
+    const long long blocks = (p.m + 15) / 16;
+    const int per = static_cast<int>(std::max<long long>(1, std::min<long long>(16, blocks * chunks / 4096)));
+    const dim3 grid((chunks + 3) / 4, static_cast<unsigned>((blocks + per - 1) / per));
+    hipLaunchKernelGGL((lora_expand<NB, STEPS>), grid, dim3(256), 0, s, p, per);
+}
+
+template <int NB, int STEPS>
+void launch_expand_any(LoraParams& p, hipStream_t s) {
+    const long long blocks = (p.m + 15) / 16;
+    if (blocks * ((p.n + 63) / 64) >= 2048) return launch_expand<NB, STEPS>(p, s);
+    const int chunks = deal_columns(p, 16);
+    hipLaunchKernelGGL((lora_expand_few<STEPS>), dim3((chunks + 3) / 4, static_cast<unsigned>(blocks)), dim3(256), 0, s,
+                       p);
 }
 
 }  // namespace
@@ -83,9 +421,15 @@ bool lora_add_bf16(const LoraArgs& a, std::string* err) {
     p.rows = p.rank * p.slices;
     for (int i = 0; i < p.slices; ++i) p.ends[i] = static_cast<int>(a.slice_ends[i]);
     hipStream_t s = reinterpret_cast<hipStream_t>(a.stream);
-    hipLaunchKernelGGL(lora_shrink_simple, dim3(p.m, (p.rows + 3) / 4), dim3(256), 0, s, p);
+    const long long blocks = (p.m + 15) / 16, row_blocks = (p.rows + 15) / 16;
+    if (blocks * row_blocks <= 64) launch_shrink<1, 16, 4>(p, s);
+    else if (row_blocks < 4 || blocks * row_blocks <= 256) launch_shrink<1, 8, 4>(p, s);
+    else launch_shrink<4, 8, 2>(p, s);
     KCMM_HIP_CHECK(hipGetLastError(), err);
-    hipLaunchKernelGGL(lora_expand_simple, dim3(p.m, (p.n + 255) / 256), dim3(256), 0, s, p);
+    if (p.rank <= 16) launch_expand_any<8, 1>(p, s);
+    else if (p.rank <= 32) launch_expand_any<8, 2>(p, s);
+    else if (p.rank <= 64) launch_expand_any<4, 4>(p, s);
+    else launch_expand_any<4, 8>(p, s);
     KCMM_HIP_CHECK(hipGetLastError(), err);
     return true;
 }
