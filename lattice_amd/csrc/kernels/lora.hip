@@ -11,9 +11,9 @@
 // holds, infinities too, goes nowhere).  Prompts have one adapter a block, decode
 // batches up to 16, whose weights are then what has to be read, once a block.
 //  * shrink: k dealt to the waves of a workgroup by lines of 128 bytes, their sums
-//    joined in LDS, in wave order.  A workgroup has 16 rows of A, or 64 where there
-//    are blocks enough, and one of the block's adapters, or several in turn.  Bound by
-//    what one CU loads (64 bytes a cycle).
+//    joined in LDS, in wave order.  A workgroup has 16 or 32 rows of A and one of the
+//    block's adapters, or several in turn.  Bound by what one CU loads (64 bytes a
+//    cycle).
 //  * expand: bound by base and y in HBM for prompts, by latency for few tokens.  The
 //    matrix instruction has 32 consecutive k and a rank seldom fills them, so the
 //    second parts of the values (below) are nearly free.
@@ -21,7 +21,8 @@
 // line each in 8: operands read from rows straight into the matrix instruction's
 // layout cost 4 times the cycles of whole lines.  Hence the way through LDS in the
 // shrink, the layout of the low-rank values, and tokens as rows in the expand (3001
-// tokens, rank 32, k 4096, n 28672: 36 + 116 us with such reads, 16 + 70 without).
+// tokens, rank 32, k 4096, n 28672: 36 + 116 us with such reads, 11 + 70 without; the
+// 70 are 4.9 TB/s of base and y).
 #include <algorithm>
 #include <climits>
 #include <cmath>
@@ -90,74 +91,90 @@ struct LowBlock {
     __device__ u32x4* piece(int q, int token) const { return at + q * count + token; }
 };
 
-// Workgroup (block of 16 tokens, turn, row group): RB * 16 low-rank rows for the
-// turn-th, turn + turns-th ... of the block's adapters.  A wave loads whole lines of 128
-// bytes, 8 lanes a row, U of them before it uses the first.
-template <int RB, int NW, int U>
-__global__ __launch_bounds__(64 * NW) void lora_shrink(LoraParams p, int turns) {
-    constexpr int LOADS = 2 + 2 * RB;   // of 8 rows each: the tokens', the weights'
-    __shared__ u32x4 s_rows[NW][LOADS * 64];
+// Workgroup (block of 16 tokens, turn, row group): R low-rank rows for the turn-th,
+// turn + turns-th ... of the block's adapters.  The adapter's tokens are the first
+// columns, so that up to 8 of them take one load a line.  A wave loads lines of
+// 128 bytes, 8 lanes a row, U of them before it uses the first.
+template <int R, int U>
+__global__ __launch_bounds__(512) void lora_shrink(LoraParams p, int turns) {
+    constexpr int NW = 8, RB = R / 16, WL = R / 8;   // waves; products, loads of weights a line
+    __shared__ u32x4 s_rows[NW][(2 + WL) * 64];
     const int lane = threadIdx.x & 63, ln = lane & 15, lg = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6);
     u32x4* const rows = s_rows[wave];
-    const int t0 = blockIdx.x * 16, row0 = blockIdx.z * (RB * 16);
+    const int t0 = blockIdx.x * 16, row0 = blockIdx.z * R;
     const int id = adapter_of(p, t0 + ln);
     uint32_t left = static_cast<uint32_t>(__ballot(id >= 0)) & 0xffffu;
     const int pieces = p.k / 8, lines = (pieces + 7) / 8;
     for (int turn = 0;; ++turn) {
-        const int first = __ffs(static_cast<int>(left)) - 1, a = next_adapter(id, &left);
+        const int a = next_adapter(id, &left);
         if (a < 0) break;
         if (turn % turns != static_cast<int>(blockIdx.y)) continue;
-        const bool mine = id == a;
-        const uint32_t ours = static_cast<uint32_t>(__ballot(mine));
-        const uint16_t* src[LOADS];
+        // token of the block that column `lane` has; a column behind the last takes the
+        // first one's along
+        const uint32_t ours = static_cast<uint32_t>(__ballot(id == a)) & 0xffffu;
+        const int count = __popc(ours), nth = __popc(ours & ((1u << ln) - 1));
+        const int token = __builtin_amdgcn_ds_permute(4 * (lane < 16 && id == a ? nth : 63), ln);
+        const uint16_t* xs[2];
+        const uint16_t* ws[WL];
 #pragma unroll
-        for (int i = 0; i < LOADS; ++i) {
-            const int r = 8 * i + (lane >> 3);
-            // a column of no token of this adapter's takes the first one's values along
-            src[i] = i < 2 ? p.x + static_cast<size_t>(t0 + (ours >> r & 1 ? r : first)) * p.k
-                           : p.a + (static_cast<size_t>(a) * p.rows + min(row0 + r - 16, p.rows - 1)) * p.k;
+        for (int i = 0; i < 2; ++i) {
+            const int c = 8 * i + (lane >> 3);
+            xs[i] = p.x + static_cast<size_t>(t0 + __shfl(token, c < count ? c : 0)) * p.k;
         }
+#pragma unroll
+        for (int i = 0; i < WL; ++i)
+            ws[i] = p.a + (static_cast<size_t>(a) * p.rows + min(row0 + 8 * i + (lane >> 3), p.rows - 1)) * p.k;
         f32x4 sum[RB];
 #pragma unroll
         for (int i = 0; i < RB; ++i) sum[i] = f32x4{0, 0, 0, 0};
         // Lines l, l + NW ... l + (U - 1) NW; the last ones may be partial or past the row
-        auto lines_of = [&](int l, auto tail) __attribute__((always_inline)) {
-            u32x4 v[U][LOADS];
+        auto lines_of = [&](int l, auto XL, auto tail) __attribute__((always_inline)) {
+            u32x4 x[U][XL], w[U][WL];
 #pragma unroll
-            for (int u = 0; u < U; ++u)
+            for (int u = 0; u < U; ++u) {
+                const int piece = (l + u * NW) * 8 + (lane & 7);
+                const uint32_t at = static_cast<uint32_t>(tail && piece >= pieces ? 0 : piece) * 8;
 #pragma unroll
-                for (int i = 0; i < LOADS; ++i) {
-                    const int piece = (l + u * NW) * 8 + (lane & 7);
-                    v[u][i] = *reinterpret_cast<const u32x4*>(
-                        src[i] + static_cast<uint32_t>(tail && piece >= pieces ? 0 : piece) * 8);
-                }
+                for (int i = 0; i < XL; ++i) x[u][i] = *reinterpret_cast<const u32x4*>(xs[i] + at);
+#pragma unroll
+                for (int i = 0; i < WL; ++i) w[u][i] = *reinterpret_cast<const u32x4*>(ws[i] + at);
+            }
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 const bool in = !tail || (l + u * NW) * 8 + (lane & 7) < pieces;
+                const u32x4 none = {0, 0, 0, 0};
 #pragma unroll
-                for (int i = 0; i < LOADS; ++i)
-                    *piece_at(rows, 8 * i + (lane >> 3), lane & 7) = in ? v[u][i] : u32x4{0, 0, 0, 0};
+                for (int i = 0; i < XL; ++i) *piece_at(rows, 8 * i + (lane >> 3), lane & 7) = in ? x[u][i] : none;
+#pragma unroll
+                for (int i = 0; i < WL; ++i)
+                    *piece_at(rows, 8 * (XL + i) + (lane >> 3), lane & 7) = in ? w[u][i] : none;
                 __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    const u32x4 x = *piece_at(rows, ln, 4 * h + lg);
+                    // (with 8 columns loaded the others are these again)
+                    const u32x4 xf = *piece_at(rows, XL == 1 ? ln & 7 : ln, 4 * h + lg);
 #pragma unroll
                     for (int i = 0; i < RB; ++i)
-                        sum[i] = mfma(*piece_at(rows, 16 * (i + 1) + ln, 4 * h + lg), x, sum[i]);
+                        sum[i] = mfma(*piece_at(rows, 8 * XL + 16 * i + ln, 4 * h + lg), xf, sum[i]);
                 }
                 __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
             }
         };
-        int l = wave;
+        auto all_lines = [&](auto XL) __attribute__((always_inline)) {
+            int l = wave;
 #pragma clang loop unroll(disable)
-        for (; (l + (U - 1) * NW + 1) * 8 <= pieces; l += NW * U) lines_of(l, std::false_type{});
-        if (l < lines) lines_of(l, std::true_type{});
+            for (; (l + (U - 1) * NW + 1) * 8 <= pieces; l += NW * U) lines_of(l, XL, std::false_type{});
+            if (l < lines) lines_of(l, XL, std::true_type{});
+        };
+        if (count <= 8) all_lines(std::integral_constant<int, 1>{});
+        else all_lines(std::integral_constant<int, 2>{});
         // the waves' sums, each in the place of its lines
 #pragma unroll
         for (int i = 0; i < RB; ++i) rows[i * 64 + lane] = __builtin_bit_cast(u32x4, sum[i]);
         __syncthreads();
         const float scale = p.scales != nullptr ? p.scales[a] : 1.0f;
+        const int t = __shfl(token, ln);
         for (int i = wave; i < RB; i += NW) {
             f32x4 v = {0, 0, 0, 0};
             for (int j = 0; j < NW; ++j) v += __builtin_bit_cast(f32x4, s_rows[j][i * 64 + lane]);
@@ -169,14 +186,14 @@ __global__ __launch_bounds__(64 * NW) void lora_shrink(LoraParams p, int turns) 
                 part[e] = bf16_round_hw(v[e]);
                 part[4 + e] = fabsf(part[e]) < INFINITY ? v[e] - part[e] : 0.0f;
             }
-            // rows 4 lg .. +3 of each 16, of token ln: half a piece
+            // rows 4 lg .. +3 of each 16, of column ln: half a piece
             const int row = row0 + 16 * i + 4 * lg;
-            if (mine && row < p.rows) {
+            if (ln < count && row < p.rows) {
                 const int slice = row / p.rank, q = (row - slice * p.rank) / 8;
                 const LowBlock low(p, blockIdx.x, slice);
                 const u32x4 o = pack_bf16x8(part);
-                reinterpret_cast<u32x2*>(low.piece(q, ln))[row >> 2 & 1] = u32x2{o[0], o[1]};
-                reinterpret_cast<u32x2*>(low.piece(p.rank / 8 + q, ln))[row >> 2 & 1] = u32x2{o[2], o[3]};
+                reinterpret_cast<u32x2*>(low.piece(q, t))[row >> 2 & 1] = u32x2{o[0], o[1]};
+                reinterpret_cast<u32x2*>(low.piece(p.rank / 8 + q, t))[row >> 2 & 1] = u32x2{o[2], o[3]};
             }
         }
         __syncthreads();
@@ -363,11 +380,11 @@ __global__ __launch_bounds__(256) void lora_expand(LoraParams p, int per) {
     }
 }
 
-template <int RB, int NW, int U>
+template <int R, int U>
 void launch_shrink(const LoraParams& p, hipStream_t s) {
-    const int blocks = (p.m + 15) / 16, groups = (p.rows + 16 * RB - 1) / (16 * RB);
-    const int turns = std::max(1, std::min({16, p.adapters, 256 / (blocks * groups)}));
-    hipLaunchKernelGGL((lora_shrink<RB, NW, U>), dim3(blocks, turns, groups), dim3(64 * NW), 0, s, p, turns);
+    const int blocks = (p.m + 15) / 16, groups = (p.rows + R - 1) / R;
+    const int turns = std::max(1, std::min({16, p.m, p.adapters, 512 / (blocks * groups)}));
+    hipLaunchKernelGGL((lora_shrink<R, U>), dim3(blocks, turns, groups), dim3(512), 0, s, p, turns);
 }
 
 // Chunks of `width` columns; returns their number.
@@ -391,8 +408,12 @@ void launch_expand(LoraParams& p, hipStream_t s) {
 
 template <int NB, int STEPS>
 void launch_expand_any(LoraParams& p, hipStream_t s) {
+    // Runs of blocks pay once base and y are large: few and many, the whole call, 2048
+    // tokens in runs of an adapter: n 4096 20.0 and 18.9 us, n 6144 64.6 and 51.1; 1024
+    // tokens, n 6144 40.2 and 40.3.  (Where the adapters of 2048 tokens are mixed, weights
+    // are loaded anew for each block: n 4096 33.3 and 47.5.)
     const long long blocks = (p.m + 15) / 16;
-    if (blocks * ((p.n + 63) / 64) >= 2048) return launch_expand<NB, STEPS>(p, s);
+    if (blocks * ((p.n + 63) / 64) >= 8192) return launch_expand<NB, STEPS>(p, s);
     const int chunks = deal_columns(p, 16);
     hipLaunchKernelGGL((lora_expand_few<STEPS>), dim3((chunks + 3) / 4, static_cast<unsigned>(blocks)), dim3(256), 0, s,
                        p);
@@ -421,10 +442,14 @@ bool lora_add_bf16(const LoraArgs& a, std::string* err) {
     p.rows = p.rank * p.slices;
     for (int i = 0; i < p.slices; ++i) p.ends[i] = static_cast<int>(a.slice_ends[i]);
     hipStream_t s = reinterpret_cast<hipStream_t>(a.stream);
+    // Twice the rows a workgroup halve what the tokens cost it, but leave half as many
+    // workgroups.  16 and 32 rows, the whole call: 64 tokens of 16 adapters, 48 rows,
+    // k 4096: 11.7 and 12.9 us; 64 of 8, 64 rows, k 14336: 16.7 and 21.2; 512 (384
+    // products): 22.8 and 24.2; 3001 prompt tokens (752): 85.2 and 83.3; 2048 tokens, 192
+    // rows (1536): 69.1 and 62.7.  8 or 64 rows, or 16 waves, are better nowhere by 1%.
     const long long blocks = (p.m + 15) / 16, row_blocks = (p.rows + 15) / 16;
-    if (blocks * row_blocks <= 64) launch_shrink<1, 16, 4>(p, s);
-    else if (row_blocks < 4 || blocks * row_blocks <= 256) launch_shrink<1, 8, 4>(p, s);
-    else launch_shrink<4, 8, 2>(p, s);
+    if (row_blocks > 1 && blocks * row_blocks >= 512) launch_shrink<32, 2>(p, s);
+    else launch_shrink<16, 4>(p, s);
     KCMM_HIP_CHECK(hipGetLastError(), err);
     if (p.rank <= 16) launch_expand_any<8, 1>(p, s);
     else if (p.rank <= 32) launch_expand_any<8, 2>(p, s);

@@ -122,6 +122,16 @@ def test_shapes(gpu_lib, m, widths, k, rank):
     check(torch, gpu_lib, m, widths, k, rank, 5)
 
 
+@pytest.mark.parametrize("mixed", [True, False])
+@pytest.mark.parametrize("m,widths,k,rank", [(1100, [7680, 16, 528], 72, 16), (2049, [4112], 40, 8),
+                                             (523, [16384, 144], 136, 32), (700, [12800], 64, 64),
+                                             (1001, [8192, 272, 16], 64, 128)])
+def test_many_tokens_and_columns(gpu_lib, m, widths, k, rank, mixed):
+    import torch
+    ids = np.random.default_rng(m).integers(-1, 5, m)
+    check(torch, gpu_lib, m, widths, k, rank, 5, ids=ids if mixed else np.sort(ids), in_place=mixed)
+
+
 @pytest.mark.parametrize("m,widths,k,rank", [(1, [4096], 4096, 16), (64, [4096, 1024, 1024], 4096, 16),
                                              (5, [1024], 14336, 64), (700, [2048], 2048, 32),
                                              (1100, [512, 512], 1024, 128), (2500, [160], 264, 8)])
