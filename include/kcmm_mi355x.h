@@ -475,9 +475,9 @@ typedef struct kcmm_rope_positions {
  *  i + head_dim/2) by position * inv_freq[i].  The position is the place, or
  *  with `positions` (NULL: none) any int32, of the axis that the pair takes.
  *
- *  The angle is exact to 2^-22 at any position (the decode form rounds it to
- *  fp32, which is off by up to 2^-24 of the angle: 2^-9 from position 32768 on),
- *  and every output is rounded once.  On fp8 pages the rows that the call writes
+ *  Cosine and sine are off by at most 2^-21 below position 2^27, 2^-20 at any, with
+ *  frequencies up to 1 (the decode form rounds the angle to fp32, which is off by up
+ *  to 2^-24 of it: 2^-9 from position 32768 on), and every output is rounded once.  On fp8 pages the rows that the call writes
  *  into a page are one set, as at the head of this file, but of rotated values
  *  that have not been rounded to bf16.
  *

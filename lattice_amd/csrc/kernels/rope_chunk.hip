@@ -8,8 +8,8 @@
 // takes (time, height, width of an image's patches).  The angle is reduced in 64
 // bits, in whole turns -- the product p * inv_freq / 2 pi of a 31-bit position has
 // more bits than fp32, and a place of 10^5 would otherwise be off by 0.005 rad --
-// so cos and sin are fp32 values to 2^-22 at any position; each output is rounded
-// once.
+// so cos and sin are off by at most 2^-21 at places below 2^27 (2^-20 at any 32-bit
+// position) with frequencies up to 1; each output is rounded once.
 //
 // Bound by HBM for prompts: each byte of qkv is read once, q and the page rows
 // are written once; by its chain (the sequence of a token, its length, table
@@ -18,10 +18,15 @@
 //    (64 pairs a token against 40 rotated heads), and a part of their heads; the
 //    elements are loaded before the chain begins.
 //  * fp8 pages: the rows that the chunk writes into a page have one scale per kv
-//    head, so a wave takes one (page, kv head, K or V): rotated values stay in
-//    registers in 32 bits while their maximum is found, and are encoded from
-//    there, without a rounding to bf16 between.  q heads are rows as above, in
-//    the same launch.
+//    head, so a wave takes one (page, kv head, K or V), or 2 or 4 waves do where the
+//    page has more than they hold: rotated values stay in registers in 32 bits while
+//    their maximum is found, and are encoded from there, without a rounding to bf16
+//    between.  q heads are rows as above, in the same launch, behind the pages, whose
+//    chain is longer (rows first: 35 for 32 us).  32 values a lane: with
+//    64 the registers leave too few waves for the rows (32 for 26.6 us).
+// Ragged prompts (32 q, 8 kv heads x 128): 4150 tokens 24 us in bf16, 4.2 TB/s
+// read and written; 4507 into fp8 pages 24-26 us; 8 sequences of a few drafted tokens 7.4 us,
+// a launch and the chain.
 #include <algorithm>
 #include <climits>
 #include <cstring>
@@ -47,7 +52,8 @@ struct ChunkParams {
     uint32_t axis_bits[8];      // two bits per pair
     int batch, total, num_q_heads, kv_heads, head_dim, block_size, mbps, row_bytes, data_bytes;
     uint32_t n_ids;
-    int row_wgs;                // workgroups of the rows, in front of the page waves
+    int page_wgs;               // workgroups of the pages, in front of the rows
+    int page_waves;             // waves of a page, kv head and K or V: 1, 2, 4
     int row_parts;              // of a tile of tokens' heads
 };
 
@@ -55,7 +61,7 @@ constexpr int kTokens = 4;      // of a workgroup of rows (a wave finds each)
 constexpr int kUnits = 2;       // 8-pair pieces of a thread
 
 // cos and sin of p * f, p any 32-bit integer: whole turns are dropped in 64 bits
-// (31 + 24 bits of the product, 2^-53 of at most 2^31 turns: 2^-22 of a turn).
+// (two roundings of 2^-53 of fewer than 2^29 turns; the rest is rounded to 2^-26).
 __device__ __forceinline__ void turn(int p, float f, float* c, float* s) {
     const double turns = static_cast<double>(p) * static_cast<double>(f) * 0.15915494309189535;
     sincospif(2.0f * static_cast<float>(turns - rint(turns)), s, c);
@@ -158,7 +164,7 @@ struct Pairs {
 };
 
 // Rows: tokens wg / parts * kTokens .. and a part of their heads (Q_ONLY: the q
-// heads; k and v go through page_wave).
+// heads; k and v go through page_waves).
 template <int DT, int C, bool Q_ONLY>
 __device__ __forceinline__ void rows(const ChunkParams& p, int wg) {
     constexpr int IO = DT == kDtFP8 ? kDtBF16 : DT;   // type of qkv and q
@@ -275,12 +281,15 @@ __device__ __forceinline__ void put_codes(uint8_t* at, const float (&v)[C], floa
     else *reinterpret_cast<uint32_t*>(at) = w[0];
 }
 
-// One wave: the chunk's rows of one (page, kv head, K or V), job = unit * 2 Hkv +
-// 2 kvh + is_v over the pages that the sequences' chunks touch, in order.  The
-// scale: as fp8_write_page_head has it.
+// `waves` waves of a workgroup: the chunk's rows of one (page, kv head, K or V), job =
+// unit * 2 Hkv + 2 kvh + is_v over the pages that the sequences' chunks touch, in
+// order.  The scale: as fp8_write_page_head has it.
 template <int C>
-__device__ __forceinline__ void page_wave(const ChunkParams& p, int job) {
-    const int lane = threadIdx.x & 63;
+__device__ __forceinline__ void page_waves(const ChunkParams& p, int wg) {
+    __shared__ float s_amax[4];
+    const int lane = threadIdx.x & 63, W = p.page_waves;
+    const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6);
+    const int job = wg * (4 / W) + wave / W, sub = wave % W;
     const int unit = job / (2 * p.kv_heads), j = job - unit * 2 * p.kv_heads;
     const int kvh = j >> 1;
     const bool is_v = j & 1;
@@ -307,23 +316,24 @@ __device__ __forceinline__ void page_wave(const ChunkParams& p, int job) {
         }
         base += __shfl(end, 63);
     }
-    if (b < 0) return;
-    const int id = block_id(p, b, block);
-    if (id < 0) return;
+    int id = b < 0 ? -1 : block_id(p, b, block);
+    if (id < 0 && W == 1) return;
+    const bool none = id < 0;   // (its waves go on to the barrier)
+    if (none) b = block = id = 0;
     const Places at = places_of(p, b);
     const int D = p.head_dim, half = D / 2, per = half / C;
     const int s0 = max(at.lo - block * p.block_size, 0);
-    const int s1 = min(at.hi - block * p.block_size, p.block_size);
+    const int s1 = none ? s0 : min(at.hi - block * p.block_size, p.block_size);
     // token of slot 0 (a row of qkv), place of slot 0
     const int place0 = block * p.block_size, tok0 = p.qsl[b] + place0 - at.first;
     const int all = p.num_q_heads + 2 * p.kv_heads;
     const int head = p.num_q_heads + (is_v ? p.kv_heads : 0) + kvh;
     uint8_t* page = (is_v ? p.v_base : p.k_base) + p.offsets_f16[id] * 2ull;
     float* const scale_at = reinterpret_cast<float*>(page + p.data_bytes) + kvh;
-    const float old = *scale_at;
+    const float old = none ? 0.0f : *scale_at;
 
-    constexpr int PASS = 32 / C;        // pieces of a lane held at a time (64 values)
-    const int pieces = (s1 - s0) * per;
+    constexpr int PASS = 16 / C;        // pieces of a lane held at a time (32 values)
+    const int pieces = (s1 - s0) * per, mine = sub * 64 * PASS, step = W * 64 * PASS;
     float y1[PASS][C], y2[PASS][C];
     bool nan = false;
     float amax = 0.0f;
@@ -354,7 +364,7 @@ __device__ __forceinline__ void page_wave(const ChunkParams& p, int job) {
             }
         }
     };
-    for (int q0 = 0; q0 < pieces; q0 += 64 * PASS) {
+    for (int q0 = mine; q0 < pieces; q0 += step) {
         take(q0);
 #pragma unroll
         for (int i = 0; i < PASS; ++i) {
@@ -368,6 +378,12 @@ __device__ __forceinline__ void page_wave(const ChunkParams& p, int job) {
     }
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor(amax, o));
+    if (W > 1) {
+        if (lane == 0) s_amax[wave] = amax;
+        __syncthreads();
+        for (int i = 0; i < W; ++i) amax = fmaxf(amax, s_amax[wave - sub + i]);
+        if (none) return;
+    }
     const bool fresh = s0 == 0 || !(old > 0.0f && old <= 3.40282347e38f);
     float scale = old;
     if (fresh) {
@@ -376,7 +392,7 @@ __device__ __forceinline__ void page_wave(const ChunkParams& p, int job) {
         scale = amax / 448.0f;
         // the slots that the chunk does not write, from the old scale to the new
         const int words = D / 8, rest = p.block_size - (s1 - s0);
-        for (int q = lane; q < rest * words; q += 64) {
+        for (int q = sub * 64 + lane; q < rest * words; q += W * 64) {
             int s = q / words;
             if (s >= s0) s += s1 - s0;
             u32x2* const w = reinterpret_cast<u32x2*>(page + static_cast<size_t>(s) * p.row_bytes +
@@ -395,8 +411,8 @@ __device__ __forceinline__ void page_wave(const ChunkParams& p, int job) {
     }
     const bool fast = !__any(nan) && scale >= kFp8QuotientMin && scale <= kFp8QuotientMax;
     const float r = 1.0f / scale;
-    for (int q0 = 0; q0 < pieces; q0 += 64 * PASS) {
-        if (pieces > 64 * PASS) take(q0);
+    for (int q0 = mine; q0 < pieces; q0 += step) {
+        if (pieces > step) take(q0);
 #pragma unroll
         for (int i = 0; i < PASS; ++i) {
             const int q = q0 + i * 64 + lane;
@@ -407,20 +423,19 @@ __device__ __forceinline__ void page_wave(const ChunkParams& p, int job) {
             put_codes<C>(row + half, y2[i], scale, r, fast);
         }
     }
-    if (lane == 0) *scale_at = scale;
+    if (sub == 0 && lane == 0) *scale_at = scale;
 }
 
 template <int DT, int C>
 __global__ __launch_bounds__(256) void rope_chunk(ChunkParams p) {
     const int wg = static_cast<int>(blockIdx.x);
     if constexpr (DT == kDtFP8) {
-        if (wg >= p.row_wgs) {
-            const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6);
-            page_wave<C>(p, (wg - p.row_wgs) * 4 + wave);
+        if (wg < p.page_wgs) {
+            page_waves<C>(p, wg);
             return;
         }
     }
-    rows<DT, C, DT == kDtFP8>(p, wg);
+    rows<DT, C, DT == kDtFP8>(p, wg - p.page_wgs);
 }
 
 template <int DT>
@@ -436,14 +451,17 @@ bool launch_chunk(ChunkParams& p, hipStream_t s, std::string* err) {
         // a chunk of n tokens touches at most (n - 1) / block_size + 2 pages
         const long long seqs = std::min(p.batch, p.total);
         const long long pages = std::min<long long>(p.total, (p.total - seqs) / p.block_size + 2 * seqs);
-        page_wgs = (pages * 2 * p.kv_heads + 3) / 4;
+        // a wave for every 128 pieces of a full page, which it holds
+        const int pieces = p.block_size * (p.head_dim / 2 / C), each = 64 * (16 / C);
+        p.page_waves = pieces <= each ? 1 : pieces <= 2 * each ? 2 : 4;
+        page_wgs = (pages * 2 * p.kv_heads * p.page_waves + 3) / 4;
     }
     if (wgs + page_wgs > INT_MAX) {
         *err = "too many tokens x heads";
         return false;
     }
     p.row_parts = static_cast<int>(parts);
-    p.row_wgs = static_cast<int>(wgs);
+    p.page_wgs = static_cast<int>(page_wgs);
     const dim3 grid(static_cast<unsigned>(wgs + page_wgs));
     if (C == 8) hipLaunchKernelGGL((rope_chunk<DT, DT == kDtF32 ? 4 : 8>), grid, dim3(256), 0, s, p);
     else hipLaunchKernelGGL((rope_chunk<DT, 4>), grid, dim3(256), 0, s, p);
