@@ -390,3 +390,36 @@ def test_scratch_is_enough(gpu_lib):
             c.check()
         finally:
             c.close()
+
+
+@pytest.mark.parametrize("dtype,hq,hkv,d", [(KV_BF16, 8, 2, 128), (KV_FP8, 4, 4, 128), (KV_F16, 4, 2, 64),
+                                            (KV_BF16, 2, 2, 80)])
+def test_large_batches(gpu_lib, dtype, hq, hkv, d):
+    """More sequences than one launch takes: groups that go on into the next,
+    or over more than one, with sequences of no group around them."""
+    import torch
+    rng = np.random.default_rng(9)
+
+    def some(n, s):
+        return [(s, int(s + t)) for t in rng.integers(-s // 2, 40, n)]
+
+    check(torch, gpu_lib, dtype, hq, hkv, d, 16, [some(120, 100), some(250, 170), [], some(180, 33)],
+          before=(5, 0, 40), behind=(17,) * 20)
+    check(torch, gpu_lib, dtype, hq, hkv, d, 16, [some(600, 130)])
+    check(torch, gpu_lib, dtype, hq, hkv, d, 16, [some(256, 64), some(1, 90), some(255, 64), some(2, 64)])
+
+
+def test_scratch_of_large_batches(gpu_lib):
+    """As many bytes as the size call names are enough, for any number of
+    sequences."""
+    import torch
+    c = Case(torch, gpu_lib, KV_BF16, 16, 1, 128, 16, [[(64, 64 + i % 50) for i in range(520)]])
+    try:
+        n = c.scratch.numel()
+        whole = torch.full((n + 4096,), 0x5A, dtype=torch.uint8, device="cuda")
+        c.run(scratch=whole[:n])
+        torch.cuda.synchronize()
+        assert bool((whole[n:] == 0x5A).all())
+        c.check()
+    finally:
+        c.close()
