@@ -186,7 +186,8 @@ int kcmm_paged_attn_decode_f32_on_stream(
  * scratch_bytes >= kcmm_paged_attn_shared_scratch_bytes; its contents on entry do
  * not matter.  Calls that may run at the same time need scratch of their own.
  * Nothing is allocated and no state is kept: a call may be captured into a HIP
- * graph at once, and the graph reads and writes the buffers it was given.
+ * graph at once, and the graph reads and writes the buffers it was given.  An
+ * infinity in V that a sequence reads may come out as NaN.
  * Enqueue only.  -1 and the pool's error text where an argument does not fit.
  */
 int kcmm_paged_attn_decode_shared_on_stream(
@@ -198,8 +199,8 @@ int kcmm_paged_attn_decode_shared_on_stream(
     float scale, uint64_t stream_ptr);
 
 /** Bytes of scratch that kcmm_paged_attn_decode_shared_on_stream takes for up to
- *  `batch` sequences in any groups (it grows with batch and with
- *  max_blocks_per_seq).  0 on error.  Host-only. */
+ *  `batch` sequences in any groups (it grows with batch, up to 256 sequences, and
+ *  with heads and head_dim).  0 on error.  Host-only. */
 uint64_t kcmm_paged_attn_shared_scratch_bytes(kcmm_pool_t *pool, uint32_t batch,
                                               uint32_t num_q_heads, uint32_t max_blocks_per_seq);
 

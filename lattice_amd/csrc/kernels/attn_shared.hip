@@ -6,24 +6,31 @@
 // table they are read; the rest is read through b's own table.  L_b <= 0 writes
 // zeros.  Sums, maxima and outputs are fp32 up to the store.
 //
-// Bound by HBM: a page that a group shares is read once for up to 64 / G of its
-// sequences (G query heads a kv head), instead of once for each.
+// Bound by HBM: a page that a group shares is read once for several of its
+// sequences, instead of once for each.
 //  * An item is a run of sequences of one group with the tokens that they have in
-//    common, or one sequence with the tokens behind those.  16 NCB columns of the
-//    matrix products are (sequence of the item, query head) pairs, so a K/V byte
-//    in registers serves up to 64 query rows, as one of a single sequence serves
-//    G.  No column of an item is masked: a sequence that shares less than half of
-//    what the others do is left to read its tokens by itself.
-//  * The work is the list of 32-token tiles of all (item, kv head), common tokens
-//    first; every wave takes an equal, contiguous slice of it and streams its
-//    pages through registers, the next tile's loads in flight.  Each workgroup
-//    works out items and slices for itself, from lengths and group starts, in LDS
-//    (a kernel in front would cost more than that).
+//    common, or one sequence with the tokens behind those.  The 16 NCB columns of
+//    the matrix products are (sequence of the item, query head) pairs, so a K/V byte
+//    serves up to 64 query rows, as one of a single sequence serves G (query heads a
+//    kv head).  No column of an item is masked: a sequence that shares less than half
+//    of what the others do is left to read its tokens by itself.
+//  * The work is the list of 8 KiB tiles (16 or 32 tokens) of all (item, kv head),
+//    common tokens first; every wave takes an equal, contiguous slice of it.  Two
+//    tiles a wave, one on its way, by direct loads into LDS, and two waves a SIMD: one
+//    wave with larger tiles has a quarter of its time without loads in flight.
+//    Each workgroup works out items and slices for itself, from lengths and group
+//    starts, in LDS (a kernel in front would cost more than that).
 //  * S^T = K Q^T and O^T += V^T P^T on 16x16x32 matrix instructions, softmax with a
 //    running maximum in the log2 domain; V is turned by the transposing LDS read,
 //    through LDS of the wave's own (no barrier in the loop).
 //  * Parts of a (sequence, head) -- slices of the common tokens, slices of the rest
-//    -- are joined by their log-sum-exp in a second kernel.
+//    -- are joined by their log-sum-exp in a second kernel.  The waves of a workgroup
+//    that end in the same (item, kv head) make one part of theirs in LDS first.
+// 64 sequences over one prompt of 2048 with 64 to 512 tokens of their own (32 q, 8 kv
+// heads x 128, bf16): 41 us, 2.2 TB/s of what has to be read once; 32 requests of four
+// beams over 1 to 8 thousand tokens, fp8 pages: 96 us, 3.4 TB/s.  The launch and the
+// chain length, table, offset, page in front of the first tile are 6 us of each, the
+// joining kernel 6 more.
 #include <algorithm>
 #include <climits>
 #include <cmath>
@@ -384,30 +391,6 @@ template <int O>
 __device__ __forceinline__ void lds_write(uint32_t a, u32x4 x) {
     asm volatile("ds_write_b128 %0, %1 offset:%2" :: "v"(a), "v"(x), "i"(O) : "memory");
 }
-template <int N>
-struct WordsOf;
-template <>
-struct WordsOf<2> {
-    typedef u32x2 type;
-};
-template <>
-struct WordsOf<4> {
-    typedef u32x4 type;
-};
-template <int N>
-using Words = typename WordsOf<N>::type;
-// 16 tokens' product with the weights: four consecutive k a lane group.
-template <int DT>
-__device__ __forceinline__ f32x4 mfma16x16x16(u32x2 a, u32x2 b, f32x4 c) {
-    typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
-    typedef short s16x4 __attribute__((ext_vector_type(4)));
-    if constexpr (DT == kDtF16)
-        return __builtin_amdgcn_mfma_f32_16x16x16f16(__builtin_bit_cast(f16x4, a), __builtin_bit_cast(f16x4, b), c, 0,
-                                                     0, 0);
-    else
-        return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(s16x4, a), __builtin_bit_cast(s16x4, b), c,
-                                                         0, 0, 0);
-}
 // Two fp32 -> one dword of 16-bit elements (round to nearest even).
 template <int DT>
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
@@ -418,6 +401,11 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
         typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
         return __builtin_bit_cast(uint32_t, bf16x2{static_cast<__bf16>(lo), static_cast<__bf16>(hi)});
     }
+}
+// What the elements of `packed` = pack2(lo, hi) leave of the values.
+template <int DT>
+__device__ __forceinline__ uint32_t pack2_rest(float lo, float hi, uint32_t packed) {
+    return pack2<DT>(lo - elem_to_f32<DT>(packed & 0xffffu), hi - elem_to_f32<DT>(packed >> 16));
 }
 // Maximum over the lanes l, l ^ 16, l ^ 32, l ^ 48 that hold a column.
 __device__ __forceinline__ float column_max(float x) {
@@ -709,7 +697,7 @@ void attn_shared_stream(FastParams f, const int32_t* __restrict__ bt, const uint
                     lds_write<0>(at0 + place + v_turned(row, piece + 1), fp8x8_to_bf16(y[h][e][2], y[h][e][3]));
                 }
         }
-        Words<2 * NH> pf[NCB];
+        u32x4 pf[NCB][NH];
         const bool live = tbase + TILE <= c.end;   // (uniform)
 #pragma unroll
         for (int cb = 0; cb < NCB; ++cb) {
@@ -762,10 +750,15 @@ void attn_shared_stream(FastParams f, const int32_t* __restrict__ bt, const uint
                     for (int r = 0; r < 4; ++r) v[h * 4 + r] *= vs;
                 }
             }
-            // slots (lg, i) of the P^T operand: token i < 4 ? 4 lg + i : 16 + 4 lg + i - 4
+            // slots (lg, i) of a half's P^T operand: token 4 lg + i % 4, its weight and what
+            // that leaves (one part alone, 2^-9 of a weight, would be as large an error as
+            // the store's; 16 tokens would leave half the slots empty anyway)
 #pragma unroll
-            for (int i = 0; i < 2 * NH; ++i)
-                pf[cb][i] = pack2<MDT>(v[2 * i], v[2 * i + 1]);
+            for (int h = 0; h < NH; ++h) {
+                const float* w = v + 4 * h;
+                const uint32_t a = pack2<MDT>(w[0], w[1]), b = pack2<MDT>(w[2], w[3]);
+                pf[cb][h] = u32x4{a, b, pack2_rest<MDT>(w[0], w[1], a), pack2_rest<MDT>(w[2], w[3], b)};
+            }
         }
 #pragma unroll
         for (int d0 = 0; d0 < DB; d0 += 4) {
@@ -778,13 +771,11 @@ void attn_shared_stream(FastParams f, const int32_t* __restrict__ bt, const uint
             for (int cb = 0; cb < NCB; ++cb) {
                 if (cb >= c.blocks) break;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    if constexpr (NH == 2)
-                        acc[cb][d0 + e] = mfma16x16x32<MDT>(u32x4{t[e][0][0], t[e][0][1], t[e][1][0], t[e][1][1]},
-                                                            pf[cb], acc[cb][d0 + e]);
-                    else
-                        acc[cb][d0 + e] = mfma16x16x16<MDT>(t[e][0], pf[cb], acc[cb][d0 + e]);
-                }
+                for (int e = 0; e < 4; ++e)
+#pragma unroll
+                    for (int h = 0; h < NH; ++h)
+                        acc[cb][d0 + e] = mfma16x16x32<MDT>(
+                            u32x4{t[e][h][0], t[e][h][1], t[e][h][0], t[e][h][1]}, pf[cb][h], acc[cb][d0 + e]);
             }
         }
     };
