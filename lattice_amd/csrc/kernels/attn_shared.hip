@@ -27,8 +27,8 @@
 //    -- are joined by their log-sum-exp in a second kernel.  The waves of a workgroup
 //    that end in the same (item, kv head) make one part of theirs in LDS first.
 // 64 sequences over one prompt of 2048 with 64 to 512 tokens of their own (32 q, 8 kv
-// heads x 128, bf16): 41 us, 2.2 TB/s of what has to be read once; 32 requests of four
-// beams over 1 to 8 thousand tokens, fp8 pages: 96 us, 3.4 TB/s.  The launch and the
+// heads x 128, bf16): 35 us, 2.5 TB/s of what has to be read once; 32 requests of four
+// beams over 1 to 8 thousand tokens, fp8 pages: 95 us, 3.5 TB/s.  The launch and the
 // chain length, table, offset, page in front of the first tile are 6 us of each, the
 // joining kernel 6 more.
 #include <algorithm>
@@ -215,7 +215,7 @@ constexpr int kMaxRows = 64 * kWaves;   // sequences of a launch: one a thread i
 
 // What the joining kernel has to know of a sequence: where its parts are.
 struct RowPlan {
-    int pre_tile, pre_tiles;   // first tile of the item's common tokens (kv head 0), tiles a kv head; 0: none
+    int pre_tile, pre_tiles;   // first tile of the item's common tokens (kv head 0), their number; 0: none
     int first;                 // first sequence of the item
     int own_tile, own_tiles;   // the same of the tokens behind them
 };
@@ -225,7 +225,7 @@ struct FastParams {
     int row0, rows;            // sequences of this launch
     int group, seqs;           // query heads a kv head; sequences of an item
     int slices, least;         // waves; least tiles of one
-    int* per;                  // tiles of a slice and of all, for the joining kernel
+    int* per;                  // tiles of a slice, of all, and common ones a kv head: for the joining kernel
     RowPlan* plan;
     // first parts of (sequence, head): of the common tokens, then of the rest;
     // later parts by slice, a row a column
@@ -462,12 +462,13 @@ void attn_shared_stream(FastParams f, const int32_t* __restrict__ bt, const uint
         pre_all += it.sums[0][w];
         own_all += it.sums[1][w];
     }
-    const int pre_end = uni(pre_all) * Hkv, total = pre_end + uni(own_all) * Hkv;
+    const int pre_head = max(uni(pre_all), 1), pre_end = uni(pre_all) * Hkv, total = pre_end + uni(own_all) * Hkv;
     const int per = slice_tiles(total, f);
     if (blockIdx.x == 0) {
         if (threadIdx.x == 0) {
             f.per[0] = per;
             f.per[1] = total;
+            f.per[2] = uni(pre_all);
         }
         const int r = threadIdx.x;
         if (r < f.rows) {
@@ -477,28 +478,36 @@ void attn_shared_stream(FastParams f, const int32_t* __restrict__ bt, const uint
             if (it.common[r] > 0) {
                 const int from = max(it.lead[r] - f.row0, 0), first = from + (r - from) / f.seqs * f.seqs;
                 w.first = f.row0 + first;
-                w.pre_tile = it.pre[first] * Hkv;
+                w.pre_tile = it.pre[first];
                 w.pre_tiles = tiles_of(it.common[r], TILE);
             }
             f.plan[r] = w;
         }
     }
-    const int slice = static_cast<int>(blockIdx.x) * kWaves + wave;
-    if (static_cast<long long>(blockIdx.x) * kWaves * per >= total) return;   // (the whole workgroup)
+    // The common tokens' tiles are listed by kv head, and an XCD (every eighth workgroup)
+    // takes an eighth of them side by side: the items of a long prefix, which has more
+    // sequences than one item holds, find its pages in that XCD's L2 (64 sequences of 4
+    // heads over 2048 tokens, eight items: 40.6 -> 38.1 us).
+    int wg = blockIdx.x;
+    const int eighth = pre_end / (kWaves * per) / 8;
+    if (wg < 8 * eighth) wg = wg % 8 * eighth + wg / 8;
+    const int slice = wg * kWaves + wave;
+    if (static_cast<long long>(wg) * kWaves * per >= total) return;   // (the whole workgroup)
     const int t0 = static_cast<int>(min(static_cast<long long>(slice) * per, static_cast<long long>(total)));
     const int n = min(per, total - t0);   // 0: nothing left for this wave
 
     // Cursor over the tile list: tokens begin + TILE t .. of (item, kv head); all of it
     // wave-uniform, so that the tables are read by scalar loads
     struct Cur {
-        int r, own, g, t, nt, begin, end, shared, lead, seqs, blocks;
+        int r, own, g, t, nt, begin, end, shared, lead, seqs, blocks, again;
         float ks[F8 ? GROUPS : 1], vs[F8 ? GROUPS : 1];   // fp8: page scales of the 8-token groups
     };
     auto locate = [&](int tile) __attribute__((always_inline)) {
         Cur c;
         c.own = tile >= pre_end;
         const int* sums = c.own ? it.own : it.pre;
-        const int rel = c.own ? tile - pre_end : tile, x = rel / Hkv;
+        // (own tokens by sequence, then kv head: a table's entries serve all its heads)
+        const int rel = c.own ? tile - pre_end : tile % pre_head, x = c.own ? rel / Hkv : rel;
         // the last sequence with sums[r] <= x: it has tiles
         int lo = -1;
 #pragma unroll
@@ -513,9 +522,13 @@ void attn_shared_stream(FastParams f, const int32_t* __restrict__ bt, const uint
         c.shared = c.own ? uni(it.shared[lo]) : common;
         c.lead = max(uni(it.lead[lo]), 0);
         c.nt = max(tiles_of(c.end - c.begin, TILE), 1);
-        const int rem = rel - uni(sums[lo]) * Hkv;
-        c.g = rem / c.nt;
-        c.t = rem - c.g * c.nt;
+        // whether another item reads these tokens too
+        const int next = min(lo + max(c.seqs, 1), f.rows - 1);
+        c.again = !c.own && ((lo > 0 && uni(it.lead[lo - 1]) == uni(it.lead[lo])) ||
+                             (next > lo && uni(it.lead[next]) == uni(it.lead[lo]) && next == lo + c.seqs));
+        const int rem = rel - uni(sums[lo]) * (c.own ? Hkv : 1);
+        c.g = c.own ? rem / c.nt : tile / pre_head;
+        c.t = c.own ? rem - c.g * c.nt : rem;
         return c;
     };
     Cur ic = locate(min(t0, total - 1));
@@ -523,7 +536,7 @@ void attn_shared_stream(FastParams f, const int32_t* __restrict__ bt, const uint
     auto advance = [&](Cur& c, int tile) __attribute__((always_inline)) {
         if (++c.t < c.nt) return;
         c.t = 0;
-        if (++c.g == Hkv) c = locate(tile);
+        if (!c.own || ++c.g == Hkv) c = locate(tile);
     };
     // Byte offsets of 64 8-token groups' rows (512 tokens), a lane each, from tile
     // `from` of (sequence, kind) on; groups past the end repeat the last one
@@ -590,13 +603,25 @@ void attn_shared_stream(FastParams f, const int32_t* __restrict__ bt, const uint
         const int piece = ROWB == 256 ? (lane % PIECES) ^ (row & 15) : (lane % PIECES) ^ (row >> 1 & 7);
         src[i] = static_cast<uint32_t>((row & 7) * p.row_bytes + piece * 16);
     }
-    auto issue = [&](uint32_t place, const uint64_t* gb) __attribute__((always_inline)) {
+    // (What is read once does not push out of the caches what is not: 332 MB of beams'
+    // pages take 95 us so and 100 without; a prompt of eight items 35 us with its pages
+    // left in the caches, 38 without.)
+    auto issue = [&](uint32_t place, const uint64_t* gb, bool again) __attribute__((always_inline)) {
         uint8_t* const to = ring + place;
+        if (again) {
 #pragma unroll
-        for (int i = 0; i < TILE / ROWS; ++i) {
-            const uint64_t g = gb[i * ROWS / 8];
-            load_lds16_nt(kreg + g + src[i % STEP], to + i * 1024);
-            load_lds16_nt(vreg + g + src[i % STEP], to + HALF + i * 1024);
+            for (int i = 0; i < TILE / ROWS; ++i) {
+                const uint64_t g = gb[i * ROWS / 8];
+                load_lds16(kreg + g + src[i % STEP], to + i * 1024);
+                load_lds16(vreg + g + src[i % STEP], to + HALF + i * 1024);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < TILE / ROWS; ++i) {
+                const uint64_t g = gb[i * ROWS / 8];
+                load_lds16_nt(kreg + g + src[i % STEP], to + i * 1024);
+                load_lds16_nt(vreg + g + src[i % STEP], to + HALF + i * 1024);
+            }
         }
     };
     // Column c of an item: head c % G of the kv head's, of its sequence c / G.
@@ -788,7 +813,7 @@ void attn_shared_stream(FastParams f, const int32_t* __restrict__ bt, const uint
     group_bases(ic, gb);
     static_assert(ST == 2, "one tile before the loop");
     cq[0] = ic;
-    if (n > 0) issue(0, gb);
+    if (n > 0) issue(0, gb, ic.again);
     if (n > 1) {
         advance(ic, t0 + 1);
         group_bases(ic, gb);
@@ -800,7 +825,7 @@ void attn_shared_stream(FastParams f, const int32_t* __restrict__ bt, const uint
     for (int i = 0; i < n; ++i) {
         cq[ST - 1] = ic;
         if (i + ST - 1 < n) {
-            issue(fill, gb);   // (the place's last reads have returned)
+            issue(fill, gb, ic.again);   // (the place's last reads have returned)
             if (i + ST < n) {
                 advance(ic, t0 + i + ST);
                 group_bases(ic, gb);
@@ -914,7 +939,7 @@ __global__ __launch_bounds__(kJoinThreads) void attn_shared_join(FastParams f, i
         q.n = q.wgs + on;
         return q;
     };
-    const Parts pre = parts_of(w.pre_tile + g * w.pre_tiles, w.pre_tiles);
+    const Parts pre = parts_of(w.pre_tile + g * f.per[2], w.pre_tiles);
     const Parts own = parts_of(w.own_tile + g * w.own_tiles, w.own_tiles);
     const int parts = pre.n + own.n;
     const int shift = (f.row0 + r - w.first) * G;   // its columns in the item's slices
@@ -1028,7 +1053,7 @@ Layout layout_of(int rows, int hq, int d, int ncb) {
         return here;
     };
     const size_t firsts = size_t(2) * rows * hq, later = static_cast<size_t>(kSlices) * 16 * ncb;
-    l.per = take(2 * sizeof(int));
+    l.per = take(3 * sizeof(int));
     l.plan = take(static_cast<size_t>(rows) * sizeof(RowPlan));
     l.ml = take(firsts * 8);
     l.slice_ml = take(later * 8);
