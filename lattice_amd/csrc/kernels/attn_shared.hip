@@ -1036,9 +1036,15 @@ __global__ __launch_bounds__(kJoinThreads) void attn_shared_join(FastParams f, i
 }
 
 // Column blocks of an item: two of 128 elements, or four of 64, are what half of a
-// SIMD's registers hold; one where a group has few query rows a kv head.
+// SIMD's registers hold; one where a group has few query rows a kv head (in the mean
+// over groups).  One and two, 128 elements, prompts of 1 to 4 thousand: 4 rows 136
+// and 140 us, 8 rows 89 and 84 (fp8 64 and 62; two sequences alone 14.1 and 14.8),
+// 16 rows 106 and 89; one and four, 64 elements: 8 rows 31.3 and 32.9.
 constexpr int kSlices = 2048;   // two workgroups of four waves a CU
-int column_blocks(int d, long long rows) { return rows <= 8 ? 1 : d == 64 ? 4 : 2; }
+int column_blocks(int d, long long rows, int batch) {
+    const bool few = rows < 8 || (rows == 8 && (d == 64 || batch < 16));
+    return few ? 1 : d == 64 ? 4 : 2;
+}
 
 // Where things lie in the scratch of a launch of `rows` sequences.
 struct Layout {
@@ -1114,7 +1120,7 @@ bool launch_fast(const SharedParams& p, uint64_t scratch, hipStream_t s, std::st
 template <int DT, int D>
 bool launch_columns(const SharedParams& p, uint64_t scratch, hipStream_t s, std::string* err) {
     const long long rows = static_cast<long long>(p.batch) * (p.num_q_heads / p.kv_heads) / p.groups;
-    return column_blocks(D, rows) == 1 ? launch_fast<DT, D, 1>(p, scratch, s, err)
+    return column_blocks(D, rows, p.batch) == 1 ? launch_fast<DT, D, 1>(p, scratch, s, err)
                                        : launch_fast<DT, D, D == 64 ? 4 : 2>(p, scratch, s, err);
 }
 
@@ -1127,7 +1133,7 @@ uint64_t attn_shared_scratch_bytes(int32_t dtype, uint32_t batch, uint32_t num_q
     if (!fast_shape(dtype, num_q_heads, kv_heads, head_dim, block_size)) return 256;
     const int rows = static_cast<int>(std::min<uint32_t>(batch, kMaxRows));
     const int hq = static_cast<int>(num_q_heads), d = static_cast<int>(head_dim);
-    return std::max(layout_of(rows, hq, d, 1).bytes, layout_of(rows, hq, d, column_blocks(d, INT_MAX)).bytes);
+    return std::max(layout_of(rows, hq, d, 1).bytes, layout_of(rows, hq, d, column_blocks(d, INT_MAX, INT_MAX)).bytes);
 }
 
 bool attn_shared(const AttnSharedArgs& a, std::string* err) {
