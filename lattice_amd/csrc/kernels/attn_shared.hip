@@ -1124,6 +1124,13 @@ bool launch_columns(const SharedParams& p, uint64_t scratch, hipStream_t s, std:
                                        : launch_fast<DT, D, D == 64 ? 4 : 2>(p, scratch, s, err);
 }
 
+// Enough for either number of column blocks.
+uint64_t fast_scratch(uint32_t batch, uint32_t num_q_heads, uint32_t head_dim) {
+    const int rows = static_cast<int>(std::min<uint32_t>(batch, kMaxRows));
+    const int hq = static_cast<int>(num_q_heads), d = static_cast<int>(head_dim);
+    return std::max(layout_of(rows, hq, d, 1).bytes, layout_of(rows, hq, d, column_blocks(d, INT_MAX, INT_MAX)).bytes);
+}
+
 }  // namespace
 
 namespace dev {
@@ -1131,9 +1138,7 @@ namespace dev {
 uint64_t attn_shared_scratch_bytes(int32_t dtype, uint32_t batch, uint32_t num_q_heads, uint32_t kv_heads,
                                    uint32_t head_dim, uint32_t block_size, uint32_t) {
     if (!fast_shape(dtype, num_q_heads, kv_heads, head_dim, block_size)) return 256;
-    const int rows = static_cast<int>(std::min<uint32_t>(batch, kMaxRows));
-    const int hq = static_cast<int>(num_q_heads), d = static_cast<int>(head_dim);
-    return std::max(layout_of(rows, hq, d, 1).bytes, layout_of(rows, hq, d, column_blocks(d, INT_MAX, INT_MAX)).bytes);
+    return fast_scratch(batch, num_q_heads, head_dim);
 }
 
 bool attn_shared(const AttnSharedArgs& a, std::string* err) {
@@ -1159,6 +1164,11 @@ bool attn_shared(const AttnSharedArgs& a, std::string* err) {
     p.scale = a.scale;
     hipStream_t s = reinterpret_cast<hipStream_t>(a.stream);
     if (fast_shape(a.dtype, a.num_q_heads, a.kv_heads, a.head_dim, a.block_size)) {
+        // (again: the caller's check may have been of another choice of kernels)
+        if (a.scratch_bytes < fast_scratch(a.batch, a.num_q_heads, a.head_dim)) {
+            *err = "scratch is too small";
+            return false;
+        }
         if (a.dtype == kDtFP8) return launch_columns<kDtFP8, 128>(p, a.scratch, s, err);
         if (a.dtype == kDtF16)
             return a.head_dim == 64 ? launch_columns<kDtF16, 64>(p, a.scratch, s, err)

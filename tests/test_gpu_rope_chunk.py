@@ -226,6 +226,16 @@ def test_lengths(gpu_lib, dtype, chunks, pad, mbps):
     check(torch, gpu_lib, dtype, 4, 2, 64, 16, chunks, pad=pad, mbps=mbps)
 
 
+@pytest.mark.parametrize("hkv,d,bs", [(1, 128, 32), (3, 128, 64), (2, 128, 128), (2, 64, 48), (1, 256, 33), (3, 72, 100)])
+def test_fp8_pages_of_several_waves(gpu_lib, hkv, d, bs):
+    """Chunks that begin and end inside large pages, whose rows several waves
+    share; whole pages, single rows, and growth of a page that has rows already."""
+    import torch
+    check(torch, gpu_lib, KV_FP8, 2 * hkv, hkv, d, bs, [(2 * bs + 5, 3 * bs), (1, bs + 1), (bs, bs), (3, 2 * bs + 2),
+                                                       (bs - 1, 2 * bs - 1), (0, 7), (bs // 2, bs // 2 + 9)], seed=bs)
+    check(torch, gpu_lib, KV_FP8, 2 * hkv, hkv, d, bs, [(5 * bs + 1, 6 * bs - 3), (9, 9)], mbps=4, seed=d)
+
+
 @pytest.mark.parametrize("dtype", ALL)
 @pytest.mark.parametrize("n_axes,deal", [(1, None), (2, "turn"), (3, "sections"), (4, "turn")])
 def test_axes(gpu_lib, dtype, n_axes, deal):
