@@ -228,3 +228,27 @@ def test_two_streams_at_once(gpu_lib):
     torch.cuda.synchronize()
     for c in cs:
         c.check()
+
+
+def test_graph_of_many_tokens_and_columns(gpu_lib):
+    """The form for many tokens, in place, captured without a call before and
+    replayed with another order of adapters than it was captured with."""
+    import torch
+    c = Case(torch, 1030, [8192, 64], 136, 24, 5)
+    graph, stream = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=stream):
+        c.run(gpu_lib, stream=torch.cuda.current_stream().cuda_stream)
+    for turn in range(3):
+        c.ids = np.roll(c.ids, 7 * turn)
+        c.dev["ids"].copy_(torch.from_numpy(c.ids))
+        c.y[:c.m * c.n].fill_(7.0)
+        c.low.fill_(-5.0)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        c.check()
+        first = c.y.clone()
+        c.run(gpu_lib)
+        torch.cuda.synchronize()
+        assert torch.equal(c.y, first)

@@ -297,6 +297,22 @@ def test_foreign_blocks(gpu_lib, dtype):
         c.close()
 
 
+@pytest.mark.parametrize("bs", [32, 64, 128])
+def test_fp8_foreign_blocks_of_several_waves(gpu_lib, bs):
+    """The same where waves of a workgroup meet for a page's maximum."""
+    import torch
+    c = Case(torch, gpu_lib, KV_FP8, 3, 1, 128, bs, [(3 * bs, 4 * bs - 5), (20, 20), (0, 4), (bs, bs)])
+    try:
+        c.bt[0, 1], c.bt[1, 0], c.bt[0, 3] = -1, len(c.offs), 2147483647
+        c.dev["bt"].copy_(torch.from_numpy(c.bt))
+        torch.cuda.synchronize()
+        c.run()
+        torch.cuda.synchronize()
+        c.check()
+    finally:
+        c.close()
+
+
 @pytest.mark.parametrize("value", [0.0, 3e38, 1e-38, 1e-30])
 def test_fp8_ends_of_the_range(gpu_lib, value):
     """Rows of zeros, and of values at the ends of bf16's range."""
