@@ -132,6 +132,15 @@ def test_many_tokens_and_columns(gpu_lib, m, widths, k, rank, mixed):
     check(torch, gpu_lib, m, widths, k, rank, 5, ids=ids if mixed else np.sort(ids), in_place=mixed)
 
 
+@pytest.mark.parametrize("adapters", [2, 5, 70])
+@pytest.mark.parametrize("m,widths,k,rank", [(600, [4096, 16], 72, 16), (257, [8192], 40, 8), (1000, [2064], 136, 32),
+                                             (449, [4608], 64, 64), (385, [5008, 48], 64, 128)])
+def test_hundreds_of_mixed_tokens(gpu_lib, m, widths, k, rank, adapters):
+    import torch
+    ids = np.random.default_rng(m + adapters).integers(-2, adapters + 1, m)
+    check(torch, gpu_lib, m, widths, k, rank, adapters, ids=ids, in_place=adapters == 5)
+
+
 @pytest.mark.parametrize("m,widths,k,rank", [(1, [4096], 4096, 16), (64, [4096, 1024, 1024], 4096, 16),
                                              (5, [1024], 14336, 64), (700, [2048], 2048, 32),
                                              (1100, [512, 512], 1024, 128), (2500, [160], 264, 8)])
