@@ -1020,9 +1020,10 @@ __global__ __launch_bounds__(kJoinThreads) void attn_shared_join(FastParams f, i
     if (deal > 1) {
         s_red[tid] = acc[0];
         __syncthreads();
-        if (turn > 0) return;
-        for (int i = 1; i < deal; ++i) acc[0] += s_red[i * threads + lane_q];
+        if (turn == 0)
+            for (int i = 1; i < deal; ++i) acc[0] += s_red[i * threads + lane_q];
     }
+    if (turn > 0) return;   // (and where threads are left over that took no part)
 #pragma unroll
     for (int i = 0; i < MAXQ; ++i) {
         const int q = lane_q + i * kJoinThreads;
