@@ -79,6 +79,10 @@ __device__ __forceinline__ int leader_of(const SharedParams& p, int b, int lane)
 // scales) of kChunk positions are staged in LDS before they are walked.
 constexpr int kThreads = 512, kChunk = 1024, kUnroll = 4;
 
+// Where a running maximum begins: finite, so that scores of -inf in front of every
+// other leave 0 (and no NaN), and tokens of such scores alone 0 / 0.
+constexpr float kLowest = -3.402823466e38f;
+
 template <int DT>
 __global__ __launch_bounds__(kThreads) void attn_shared_generic(SharedParams p, int tlog2) {
     constexpr bool F8 = DT == kDtFP8;
@@ -118,7 +122,7 @@ __global__ __launch_bounds__(kThreads) void attn_shared_generic(SharedParams p, 
             else x[i] = elem_to_f32<DT>(reinterpret_cast<const uint16_t*>(row)[d]);
         }
     };
-    float m = -INFINITY, s = 0.0f;
+    float m = kLowest, s = 0.0f;
     for (int end = 0, c0 = 0; c0 < L; c0 = end) {
         // up to kChunk positions of one table
         const int32_t* table = p.block_tables + static_cast<size_t>(c0 < shared ? lead : b) * p.mbps;
@@ -153,7 +157,7 @@ __global__ __launch_bounds__(kThreads) void attn_shared_generic(SharedParams p, 
                 dot[u] = pos + u * teams < end ? dot[u] * p.scale : -INFINITY;
                 top = fmaxf(top, dot[u]);
             }
-            const float corr = m == -INFINITY ? 0.0f : kexp<DT>(m - top);
+            const float corr = kexp<DT>(m - top);
             s *= corr;
 #pragma unroll
             for (int i = 0; i < 4; ++i) acc[i] *= corr;
@@ -170,7 +174,7 @@ __global__ __launch_bounds__(kThreads) void attn_shared_generic(SharedParams p, 
     }
     float M = m;
     for (int o = T; o < 64; o <<= 1) M = fmaxf(M, __shfl_xor(M, o));
-    const float f = m == -INFINITY ? 0.0f : kexp<DT>(m - M);
+    const float f = kexp<DT>(m - M);
     s *= f;
 #pragma unroll
     for (int i = 0; i < 4; ++i) acc[i] *= f;
@@ -189,10 +193,10 @@ __global__ __launch_bounds__(kThreads) void attn_shared_generic(SharedParams p, 
     }
     __syncthreads();
     for (int d = tid; d < D; d += kThreads) {
-        float top = -INFINITY, S = 0.0f, o = 0.0f;
+        float top = kLowest, S = 0.0f, o = 0.0f;
         for (int w = 0; w < kThreads / 64; ++w) top = fmaxf(top, s_m[w]);
         for (int w = 0; w < kThreads / 64; ++w) {
-            const float e = s_m[w] == -INFINITY ? 0.0f : kexp<DT>(s_m[w] - top);
+            const float e = kexp<DT>(s_m[w] - top);
             S += s_s[w] * e;
             o += s_acc[w * 256 + d] * e;
         }
@@ -651,7 +655,7 @@ void attn_shared_stream(FastParams f, const int32_t* __restrict__ bt, const uint
     auto clear = [&]() __attribute__((always_inline)) {
 #pragma unroll
         for (int cb = 0; cb < NCB; ++cb) {
-            m_run[cb] = -3.402823466e38f;   // (finite: a first tile of scores -inf leaves 0, no NaN)
+            m_run[cb] = kLowest;
             l_run[cb] = 0.0f;
 #pragma unroll
             for (int i = 0; i < DB; ++i) acc[cb][i] = f32x4{0, 0, 0, 0};

@@ -1,10 +1,12 @@
 """Decode attention of groups that share a prefix (kcmm_paged_attn_decode_shared):
 the parts of a long prefix and their join, for every number of query heads a kv
 head, against fp64 under the tolerance of test_gpu_attn_shared."""
+import numpy as np
 import pytest
 
-from lattice_amd.bindings import KV_BF16, KV_F16, KV_FP8
-from tests.test_gpu_attn_shared import check
+from lattice_amd.bindings import KV_BF16, KV_F16, KV_F32, KV_FP8, memcpy_dtoh, memcpy_htod
+from lattice_amd.workload import SB
+from tests.test_gpu_attn_shared import Case, check
 
 pytestmark = pytest.mark.gpu
 
@@ -22,3 +24,40 @@ def test_heads_of_a_kv_head(gpu_lib, dtype, group, d):
     check(torch, gpu_lib, dtype, 2 * group, 2, d, 16, [[(100, 133), (100, 101), (100, 164)], [(37, 70)]],
           seed=group)
     check(torch, gpu_lib, dtype, group, 1, d, 16, [[(2100, 2100 + 40 * i) for i in range(3)], [(0, 5)]], seed=group)
+
+
+@pytest.mark.parametrize("dtype,hq,hkv,d,bs", [
+    (KV_BF16, 8, 2, 128, 16), (KV_F16, 16, 4, 64, 16), (KV_BF16, 6, 3, 80, 16), (KV_F16, 40, 2, 64, 8),
+    (KV_F32, 8, 2, 128, 16), (KV_F32, 4, 4, 36, 4)])
+@pytest.mark.parametrize("rows", [[0], [0, 1, 2, 3], list(range(200)), list(range(1, 700)), [299], [5, 640]])
+def test_scores_of_minus_infinity(gpu_lib, dtype, hq, hkv, d, bs, rows):
+    """Tokens whose K holds an infinity that makes their scores -inf weigh
+    nothing, wherever they stand: the others' softmax is left."""
+    import torch
+    c = Case(torch, gpu_lib, dtype, hq, hkv, d, bs,
+             [[(640, 700), (640, 641), (640, 900)], [(0, 5), (0, 1024)]], seed=d)
+    try:
+        c.dev["q"][:, :, 0] = 1.0
+        c.q[:, :, 0] = 1.0
+        code = np.frombuffer({KV_BF16: b"\x80\xff", KV_F16: b"\x00\xfc", KV_F32: b"\x00\x00\x80\xff"}[dtype], np.uint8)
+        keys = memcpy_dtoh(c.pool.va_k(0), c.pool.stats()["superblock_count"] * SB)
+        offs, bt = np.asarray(c.pool.all_block_offsets_f16(), np.int64) * 2, c.dev["bt"].cpu().numpy()
+        lead = np.repeat(c.starts[:-1], np.diff(c.starts))
+        for b in range(c.batch):
+            hit = [t for t in rows if t < c.totals[b]]
+            if len(hit) == c.totals[b]:
+                hit = hit[:-1]       # (one token is left)
+            for t in hit:
+                r = lead[b] if t < c.shared[b] // bs * bs else b
+                at = int(offs[bt[r, t // bs]]) + t % bs * hkv * d * len(code)
+                for h in range(hkv):
+                    keys[at + h * d * len(code):][:len(code)] = code
+            gone = np.isin(np.arange(c.totals[b]), hit)
+            c.dense[b] = [x[:c.totals[b]][~gone] for x in c.dense[b]]
+            c.totals[b] = int((~gone).sum())
+        memcpy_htod(c.pool.va_k(0), keys)
+        c.run()
+        torch.cuda.synchronize()
+        c.check()
+    finally:
+        c.close()
