@@ -756,9 +756,12 @@ void attn_shared_stream(FastParams f, const int32_t* __restrict__ bt, const uint
                 }
             }
             // the column's reference grows where a score exceeds it by more than 8: until
-            // then weights are at most 2^8, which costs no bits
-            if (__any(mt > m_run[cb] + 8.0f)) {
-                const float m_new = fmaxf(m_run[cb], column_max(mt));
+            // then weights are at most 2^8 of the greatest, which costs no bits.  f16 weights
+            // are 2^7 times as large, up to 2^15: below 2^-25 f16 has nothing, and a tile of
+            // weights of 2^-26 beside one of 1 would be lost
+            constexpr float UP = DT == kDtF16 ? 7.0f : 0.0f;
+            if (__any(mt > m_run[cb] + (8.0f + UP))) {
+                const float m_new = fmaxf(m_run[cb], column_max(mt) - UP);
                 const float corr = __builtin_amdgcn_exp2f(m_run[cb] - m_new);
                 l_run[cb] *= corr;
                 m_run[cb] = m_new;

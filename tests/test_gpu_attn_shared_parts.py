@@ -4,11 +4,33 @@ head, against fp64 under the tolerance of test_gpu_attn_shared."""
 import numpy as np
 import pytest
 
+import oracle as O
 from lattice_amd.bindings import KV_BF16, KV_F16, KV_F32, KV_FP8, memcpy_dtoh, memcpy_htod
 from lattice_amd.workload import SB
-from tests.test_gpu_attn_shared import Case, check
+from tests.test_gpu_attn_shared import HALF_STEP, Case, check
 
 pytestmark = pytest.mark.gpu
+
+
+def tight(c):
+    got = c.out.double().cpu().numpy()
+    f16, u = c.dtype == KV_F16, HALF_STEP[c.dtype]
+    for b, n in enumerate(c.totals):
+        k, v = (x[:n] for x in c.dense[b])
+        for h in range(c.hq):
+            g = h * c.hkv // c.hq
+            z = k[:, g] @ c.q[b, h] * c.scale
+            size = np.abs(k[:, g]) @ np.abs(c.q[b, h]) * abs(c.scale)
+            w = np.exp(z - z.max())
+            w /= w.sum()
+            o, a = w @ v[:, g], w @ np.abs(v[:, g])
+            assert np.abs(z - z.max())[w > 2.0 ** -60].max() <= 64
+            delta = 2 * ((c.d + 2) * 2.0 ** -24 * size.max() + 2.0 ** -18)
+            tol = u * np.abs(o) + (u * u + delta + (n + 64) * 2.0 ** -24) * a
+            if f16:
+                tol += 2.0 ** -32 * np.abs(v[:, g]).sum(0) + 2.0 ** -25
+            off = np.abs(got[b, h] - o)
+            assert np.all(off <= tol), (b, h, n, float(np.max(off / tol)))
 
 
 # the page types and head widths whose parts are joined
@@ -59,5 +81,43 @@ def test_scores_of_minus_infinity(gpu_lib, dtype, hq, hkv, d, bs, rows):
         c.run()
         torch.cuda.synchronize()
         c.check()
+    finally:
+        c.close()
+
+
+@pytest.mark.parametrize("dtype,hq,hkv,d", [(KV_BF16, 8, 2, 128), (KV_F16, 8, 2, 128), (KV_F16, 8, 2, 64),
+                                            (KV_F16, 16, 1, 64)])
+@pytest.mark.parametrize("heavy", [0, 9, 15, 90])
+@pytest.mark.parametrize("nats", [12, 18, 20])
+def test_small_weights_beside_a_large_one(gpu_lib, dtype, hq, hkv, d, heavy, nats):
+    """One token of nearly all the weight, whose V is 0, beside tokens of e^-nats
+    each: their values are the output."""
+    import torch
+    c = Case(torch, gpu_lib, dtype, hq, hkv, d, 16, [[(90, 100), (90, 99)], [(0, 16)]], scale=1.0, seed=nats)
+    try:
+        c.dev["q"].fill_(1.0)
+        c.q[:] = 1.0
+        offs, bt = np.asarray(c.pool.all_block_offsets_f16(), np.int64) * 2, c.dev["bt"].cpu().numpy()
+        nbytes = c.pool.stats()["superblock_count"] * SB
+        code = {KV_BF16: O.BF16, KV_F16: O.F16}[dtype]
+        k, v = np.zeros(nbytes // 2, np.uint16), np.zeros(nbytes // 2, np.uint16)
+        big = O.encode(code, np.full(hkv * d, nats / d, np.float32))
+        some = O.encode(code, np.random.default_rng(nats).uniform(800, 1000, hkv * d).astype(np.float32))
+        assert np.all(O.decode(code, big) * d == nats)
+        for b, n in enumerate(c.totals):
+            heavy_b = min(heavy, n - 1)
+            for t in range(n):
+                at = int(offs[bt[0 if b == 1 and t < 80 else b, t // 16]]) // 2 + t % 16 * hkv * d
+                k[at:at + hkv * d] = big if t == heavy_b else 0
+                v[at:at + hkv * d] = 0 if t == heavy_b else some
+            c.dense[b][0][:] = 0
+            c.dense[b][0][heavy_b] = nats / d
+            c.dense[b][1][:] = O.decode(code, some).reshape(hkv, d)
+            c.dense[b][1][heavy_b] = 0
+        memcpy_htod(c.pool.va_k(0), k)
+        memcpy_htod(c.pool.va_v(0), v)
+        c.run()
+        torch.cuda.synchronize()
+        tight(c)
     finally:
         c.close()
