@@ -12,8 +12,9 @@
 //    common, or one sequence with the tokens behind those.  The 16 NCB columns of
 //    the matrix products are (sequence of the item, query head) pairs, so a K/V byte
 //    serves up to 64 query rows, as one of a single sequence serves G (query heads a
-//    kv head).  No column of an item is masked: a sequence that shares less than half
-//    of what the others do is left to read its tokens by itself.
+//    kv head).  No column of an item is masked: where its sequences share different
+//    lengths, the cut that saves most reads is taken, and those that share less than that
+//    are left to read their tokens by themselves.
 //  * The work is the list of 8 KiB tiles (16 or 32 tokens) of all (item, kv head),
 //    common tokens first; every wave takes an equal, contiguous slice of it.  Two
 //    tiles a wave, one on its way, by direct loads into LDS, and two waves a SIMD: one
@@ -249,9 +250,9 @@ struct Items {
     int lead[kMaxRows];     // whose table these are read through (of the whole batch)
     int common[kMaxRows];   // tokens that the item of the sequence takes in common; 0: none
     int count[kMaxRows];    // sequences of the item that begins here, 0: none does
-    int most[kMaxRows];     // the most that one of them shares, then their common tokens
-    int least[kMaxRows];
-    int part[kMaxRows];     // sequences of the item that take part
+    int most[kMaxRows];     // the most and the least that one of them shares; then
+    int least[kMaxRows];    // least: their common tokens
+    unsigned long long best[kMaxRows];   // what the best cut saves, and that cut
     int pre[kMaxRows];      // tiles of the items before this sequence, of one kv head
     int own[kMaxRows];      // the same of the sequences' own tokens
     uint64_t begins[kWaves];   // bit of a wave's lane: a group begins there
@@ -285,7 +286,8 @@ __device__ __forceinline__ void find_items(const FastParams& f, Items& it) {
     }
     const int end = p.group_starts[p.groups];   // sequences from here on lie in no group
     it.len[r] = len;
-    it.common[r] = it.count[r] = it.most[r] = it.part[r] = 0;
+    it.common[r] = it.count[r] = it.most[r] = 0;
+    it.best[r] = 0;
     it.least[r] = INT_MAX;
     it.lead[r] = -1;
     if (r == 0) it.carry = -1;
@@ -314,20 +316,30 @@ __device__ __forceinline__ void find_items(const FastParams& f, Items& it) {
     const int from = max(lead - f.row0, 0), first = from + (r - from) / f.seqs * f.seqs;
     if (in) {
         atomicMax(&it.most[first], shared);
+        atomicMin(&it.least[first], shared);
         atomicAdd(&it.count[first], 1);
     }
     __syncthreads();
-    const bool part = in && shared > 0 && 2ll * shared >= it.most[first];
-    if (part) {
-        atomicMin(&it.least[first], shared);
-        atomicAdd(&it.part[first], 1);
+    // The common tokens: of the lengths that the item's sequences share, the c with the most
+    // (k - 1) c saved, k of them sharing c or more (both in units of 8 tokens, below 2^34
+    // and 2^28); the others read all of theirs by themselves.  Where all share the same
+    // there is nothing to choose.
+    const int count = in ? it.count[first] : 0, most = in ? it.most[first] : 0;
+    const bool unequal = in && it.least[first] < most;
+    if (unequal && shared > 0) {
+        int others = -1;
+        for (int i = 0; i < count; ++i) others += it.shared[first + i] >= shared;
+        const unsigned long long c = static_cast<unsigned>(shared) / 8;
+        atomicMax(&it.best[first], others * c << 28 | (others > 0 ? c : 0));
     }
     __syncthreads();
     // (of one sequence alone there is nothing to gain)
-    const int common = part && it.part[first] > 1 ? it.least[first] : 0;
-    const bool begins = in && first == r && it.part[r] > 1;
-    const int pre = begins ? tiles_of(it.least[r], TILE) : 0, own = tiles_of(len - common, TILE);
+    const int cut = unequal ? static_cast<int>(it.best[first] & 0xfffffff) * 8 : count > 1 ? most : 0;
+    const int common = cut > 0 && shared >= cut ? cut : 0;
+    const bool begins = in && first == r && cut > 0;
+    const int pre = begins ? tiles_of(cut, TILE) : 0, own = tiles_of(len - common, TILE);
     it.common[r] = common;
+    it.least[r] = cut;
     if (!begins) it.count[r] = 0;
     const int pre_to = wave_sums(pre), own_to = wave_sums(own);
     if (lane == 63) {

@@ -121,3 +121,38 @@ def test_small_weights_beside_a_large_one(gpu_lib, dtype, hq, hkv, d, heavy, nat
         tight(c)
     finally:
         c.close()
+
+
+def reads(shared, totals, bs):
+    """The fewest tokens that sequences read with one common length: c + what each
+    has behind it, all of it for who shares less."""
+    blocks = [max(0, min(s, t)) // bs * bs for s, t in zip(shared, totals)]
+    return min(c + sum(t - (c if s >= c else 0) for s, t in zip(blocks, totals)) for c in {0, *blocks})
+
+
+@pytest.mark.parametrize("dtype,d", SPLIT)
+@pytest.mark.parametrize("lengths", [
+    [4200] + [2048] * 7,                       # the first sequence states all that is its own
+    [2048] * 7 + [1040],                       # one shares half of it
+    [2048] * 7 + [16], [2048] * 7 + [0],
+    [3000] * 4 + [1500] * 4, [3000] * 2 + [1000] * 6,
+    [500, 1000, 1500, 2000, 2500, 3000, 3500, 4000], [64] * 7 + [2000],
+])
+@pytest.mark.parametrize("order", [1, -1])
+def test_lengths_that_differ(gpu_lib, dtype, d, lengths, order):
+    """However the lengths of a group differ, its common tokens are read once, as
+    few tokens in all as one common length allows.  (The second word of the
+    scratch: tiles of all kv heads.)"""
+    import torch
+    lengths = lengths[::order]
+    group = [(s, max(s + 30, 2100) + 7 * i) for i, s in enumerate(lengths)]
+    c = Case(torch, gpu_lib, dtype, 8, 2, d, 16, [group], seed=len(set(lengths)))
+    try:
+        c.run()
+        torch.cuda.synchronize()
+        c.check()
+        tile = 16 if d == 128 and dtype != KV_FP8 else 32
+        tiles = int(c.scratch[:12].view(torch.int32)[1]) // 2
+        assert tiles <= reads(lengths, c.totals, 16) // tile + 1 + len(lengths)
+    finally:
+        c.close()
