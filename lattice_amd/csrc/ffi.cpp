@@ -685,9 +685,11 @@ bool shared_shapes_ok(kcmm_pool_t* pool, const char* fn, uint32_t batch, uint32_
         pool->set_error(std::string(fn) + ": head_dim <= 256 and packed shapes <= 65535 required");
         return false;
     }
+    // (kernels step up to 1024 tokens past a sequence's end, in 32 bits)
     if (static_cast<uint64_t>(batch) * hq > 0x7fffffffull ||
-        static_cast<uint64_t>(mbps) * g.block_size > 0x7fffffffull) {
-        pool->set_error(std::string(fn) + ": batch x q heads and the tables' tokens must be below 2^31");
+        static_cast<uint64_t>(mbps) * g.block_size > 0x7fffffffull - 4096) {
+        pool->set_error(std::string(fn) +
+                        ": batch x q heads must be below 2^31, the tables' tokens below 2^31 - 4096");
         return false;
     }
     return true;

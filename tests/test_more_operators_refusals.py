@@ -132,3 +132,16 @@ def test_null_structs(hostcheck_lib, capfd):
         None, 0, *[at(i) for i in range(9)], 1, 1, 1, 1, 64, 16, 1, C.c_float(1), 0) == -1
     assert C.sizeof(KcmmLora) == 56 and KcmmLora.slice_ends.offset == 36
     assert C.sizeof(KcmmRopePositions) == 144 and KcmmRopePositions.axis_of_pair.offset == 12
+
+
+def test_shared_attention_of_tables_near_2_to_31(hostcheck_lib):
+    """Token numbers are 32 bits, and a kernel's loop steps past the last one."""
+    with hostcheck_lib.create_pool(make_config(num_layers=1, kv_heads=1, head_dim=8, max_batch=1,
+                                               max_seq_len=42966, block_size=42966), KV_FP8) as pool:
+        call = dict(SHARED, batch=1, num_groups=1, num_q_heads=1, kv_heads=1, head_dim=8, block_size=42966)
+        for blocks, why in ((49981, "2\\^31"), (49980, "no device"), (1, "no device")):   # 2^31 - 2, and 42966 less
+            with pytest.raises(KcmmError, match=why):
+                pool.paged_attn_decode_shared(**{**call, "max_blocks_per_seq": blocks})
+        with pytest.raises(KcmmError, match="2\\^31"):
+            pool.shared_scratch_bytes(1, 1, 49981)
+        assert pool.shared_scratch_bytes(1, 1, 49980) > 0
