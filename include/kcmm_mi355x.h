@@ -485,7 +485,8 @@ typedef struct kcmm_rope_positions {
  *  Left as they were: rows of no sequence (behind query_start_loc[batch]) and
  *  of places outside 0 .. max_blocks_per_seq * block_size - 1; and the pages of
  *  table entries that are no block id that the pool had issued at the time of
- *  the call (their q is written).  Shared pages are made private first, as for
+ *  the call, or in a graph by the time it runs (their q is written); the offset table
+ *  covers every id that it had.  Shared pages are made private first, as for
  *  every append: no two sequences of a call write one page.  head_dim % 8 == 0,
  *  <= 256; qkv and q_out aligned to 16 bytes and apart.  No workspace; may be
  *  captured into a HIP graph.  Enqueue only. */

@@ -325,6 +325,7 @@ struct RopeChunkArgs {
     uint8_t axis_of_pair[128];
     uint32_t batch, total_query_tokens, num_q_heads, kv_heads, head_dim, block_size, mbps;
     uint32_t row_bytes, data_bytes, n_ids;
+    uint64_t issued_word;   // page-locked: n_ids as it is when a captured graph runs
     uint64_t stream;
 };
 bool rope_append_chunk(const RopeChunkArgs& a, std::string* err);

@@ -3,6 +3,7 @@
 // (ref src/kcmm/ffi.rs); bookkeeping is PoolCore, device work goes through
 // device_api.hpp.  This file has no HIP dependency.
 #include <algorithm>
+#include <atomic>
 #include <cctype>
 #include <cmath>
 #include <cstdio>
@@ -12,6 +13,7 @@
 #include <initializer_list>
 #include <memory>
 #include <mutex>
+#include <new>
 #include <string>
 #include <type_traits>
 #include <vector>
@@ -33,6 +35,7 @@ struct kcmm_pool_t {
     static constexpr size_t kSwapChunkBlocks = 64;
     std::vector<uint8_t*> swap_chunks;
     size_t swap_slot_bytes = 0;
+    void* issued_word = nullptr;   // the number of ids issued, page-locked: PoolCore::set_issued_word
     std::mutex tier_mu;   // one evict / restore data move at a time
 
     void set_error(const std::string& s) {
@@ -53,6 +56,8 @@ struct kcmm_pool_t {
     }
     ~kcmm_pool_t() {
         for (uint8_t* c : swap_chunks) kcmm::dev::host_pinned_free(c);
+        core.reset();
+        kcmm::dev::host_pinned_free(issued_word);
     }
 };
 
@@ -245,8 +250,15 @@ kcmm_pool_t* kcmm_pool_create_typed(const kcmm_config_t* cfg, int32_t kv_dtype) 
         g_create_error = "kcmm_pool_create: " + err;
         return nullptr;
     }
+    void* word = nullptr;
+    if (!kcmm::dev::host_pinned_alloc(sizeof(std::atomic<uint32_t>), &word, &err)) {
+        g_create_error = "kcmm_pool_create: " + err;
+        return nullptr;
+    }
     auto* p = new kcmm_pool_t;
+    p->issued_word = word;
     p->core.reset(new kcmm::PoolCore(g, std::move(backing)));
+    p->core->set_issued_word(new (word) std::atomic<uint32_t>(0));
     p->device = device;
     if (cfg->tiering != 0) {
         // ref ffi.rs:480-497 defaults, tiering.rs:723-770 swap sizing (max_blocks
@@ -1643,6 +1655,7 @@ int kcmm_rope_append_chunk_on_stream(kcmm_pool_t* pool, uint32_t layer_idx, uint
     a.row_bytes = static_cast<uint32_t>(g.row_bytes);
     a.data_bytes = static_cast<uint32_t>(g.data_bytes);
     a.n_ids = pool->core->total_blocks();
+    a.issued_word = reinterpret_cast<uint64_t>(pool->issued_word);
     a.stream = stream;
     std::string err;
     if (!kcmm::dev::set_device(pool->device, &err) || !kcmm::dev::rope_append_chunk(a, &err))

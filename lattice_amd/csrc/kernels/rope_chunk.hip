@@ -52,6 +52,7 @@ struct ChunkParams {
     uint32_t axis_bits[8];      // two bits per pair
     int batch, total, num_q_heads, kv_heads, head_dim, block_size, mbps, row_bytes, data_bytes;
     uint32_t n_ids;
+    const uint32_t* issued;     // in a graph: the ids issued by now; or null
     int page_wgs;               // workgroups of the pages, in front of the rows
     int page_waves;             // waves of a page, kv head and K or V: 1, 2, 4
     int row_parts;              // of a tile of tokens' heads
@@ -87,10 +88,14 @@ __device__ __forceinline__ Places places_of(const ChunkParams& p, int b) {
     return r;
 }
 
-// Block id of a sequence's block, or -1 for one that the pool has not issued.
+// Block id of a sequence's block, or -1 for one that the pool has not issued.  A graph
+// runs when the pool may have issued more ids than at its capture: their number is read
+// from host memory, only for an id that was none then.
 __device__ __forceinline__ int block_id(const ChunkParams& p, int b, int block) {
     const int32_t id = p.block_tables[static_cast<size_t>(b) * p.mbps + block];
-    return static_cast<uint32_t>(id) < p.n_ids ? id : -1;
+    if (static_cast<uint32_t>(id) < p.n_ids) return id;
+    if (p.issued == nullptr || id < 0) return -1;
+    return static_cast<uint32_t>(id) < __hip_atomic_load(p.issued, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM) ? id : -1;
 }
 
 // C pairs of a row: elements e .. e+C-1 and e + D/2 .. of a head.
@@ -499,6 +504,10 @@ bool rope_append_chunk(const RopeChunkArgs& a, std::string* err) {
     p.data_bytes = static_cast<int>(a.data_bytes);
     p.n_ids = a.n_ids;
     hipStream_t s = reinterpret_cast<hipStream_t>(a.stream);
+    hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
+    if (s != nullptr && hipStreamIsCapturing(s, &capture) != hipSuccess)
+        (void)hipGetLastError();   // (a stream that is never captured, while another one is)
+    if (capture != hipStreamCaptureStatusNone) p.issued = reinterpret_cast<const uint32_t*>(a.issued_word);
     switch (a.dtype) {
         case kDtF16: return launch_chunk<kDtF16>(p, s, err);
         case kDtBF16: return launch_chunk<kDtBF16>(p, s, err);

@@ -111,6 +111,7 @@ bool PoolCore::alloc_one_locked(uint32_t* id_out, std::string* err) {
         blocks_.push_back(bi);
         rc_.push_back(0);
         in_base_.push_back(0);
+        count_issued_locked();
     }
     rc_[id] = 1;
     ++epoch_;
@@ -133,6 +134,7 @@ bool PoolCore::alloc_blocks(uint32_t n, uint32_t* out, std::string* err) {
                     blocks_.pop_back();
                     rc_.pop_back();
                     in_base_.pop_back();
+                    count_issued_locked();
                 } else {
                     bi = BlockInfo{};
                     free_ids_.push_back(out[j]);
@@ -1094,6 +1096,12 @@ uint32_t PoolCore::blocks_in_use() {
 uint32_t PoolCore::total_blocks() {
     std::lock_guard<std::mutex> lk(mu_);
     return static_cast<uint32_t>(blocks_.size());
+}
+
+void PoolCore::set_issued_word(std::atomic<uint32_t>* word) {
+    std::lock_guard<std::mutex> lk(mu_);
+    issued_word_ = word;
+    count_issued_locked();
 }
 
 uint32_t PoolCore::free_physical_blocks() {

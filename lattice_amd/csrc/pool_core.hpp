@@ -22,6 +22,7 @@
 //   sequence ids       len(sequences), never reused      (ref pool.rs:551-572)
 #pragma once
 
+#include <atomic>
 #include <cstddef>
 #include <cstdint>
 #include <memory>
@@ -247,6 +248,9 @@ public:
     bool has_free_blocks();
     uint32_t blocks_in_use();
     uint32_t total_blocks();
+    // Where total_blocks() is kept up to date for kernels of captured graphs, which
+    // run when more ids have been issued than at their capture.
+    void set_issued_word(std::atomic<uint32_t>* word);
     uint32_t free_physical_blocks();
     uint32_t active_sequences();
     uint64_t epoch();
@@ -270,6 +274,10 @@ private:
     // the fork and release passes over a table touch 4 bytes per entry).
     std::vector<uint32_t> rc_;
     std::vector<uint32_t> free_ids_;
+    std::atomic<uint32_t>* issued_word_ = nullptr;   // (page-locked, of the pool's owner)
+    void count_issued_locked() {
+        if (issued_word_) issued_word_->store(static_cast<uint32_t>(blocks_.size()), std::memory_order_release);
+    }
     // Sequence indices are never reused, so a serving loop that forks keeps
     // appending; a deque never moves the sequences it already holds.
     std::deque<SequenceState> seqs_;

@@ -412,3 +412,68 @@ def test_graph_replays(gpu_lib, dtype):
             assert all(np.array_equal(x, y) for x, y in zip(got[0][1:], got[1][1:]))
     finally:
         c.close()
+
+
+@pytest.mark.parametrize("dtype", ALL)
+def test_blocks_issued_after_a_capture(gpu_lib, dtype):
+    """A graph whose tables, updated in place, name a block that the pool issued
+    after the capture writes its rows; ids that it has not issued are no blocks."""
+    import torch
+    hq, hkv, d, bs = 4, 2, 64, 16
+    cfg = make_config(num_layers=1, kv_heads=hkv, head_dim=d, max_batch=2, max_seq_len=512, block_size=bs)
+    pool = gpu_lib.create_pool(cfg, dtype)
+    try:
+        most = 12
+        mine = pool.alloc_blocks(2)
+        i32 = lambda v: torch.tensor(np.asarray(v), dtype=torch.int32, device="cuda")  # noqa: E731
+        bt, sl, qsl = i32([[mine[0], 0, 0], [mine[1], 0, 0]]), i32([5, 9]), i32([0, 1, 2])
+        offs = torch.zeros(most, dtype=torch.int64, device="cuda")
+        offs[:pool.total_blocks()] = torch.tensor(pool.all_block_offsets_f16(), device="cuda")
+        qkv = torch.ones(2, (hq + 2 * hkv) * d, dtype=torch_io_dtype(dtype), device="cuda")
+        q = torch.zeros(2, hq, d, dtype=qkv.dtype, device="cuda")
+        inv = torch.from_numpy(rope_inv_freq(10000.0, d)).cuda()
+        nbytes = pool.stats()["superblock_count"] * SB
+        memcpy_htod(pool.va_v(0), np.zeros(nbytes, np.uint8))
+
+        def call():
+            pool.rope_append_chunk(
+                layer_idx=0, qkv_ptr=qkv.data_ptr(), q_out_ptr=q.data_ptr(), block_tables_ptr=bt.data_ptr(),
+                seq_lens_ptr=sl.data_ptr(), query_start_loc_ptr=qsl.data_ptr(),
+                block_offsets_f16_ptr=offs.data_ptr(), inv_freq_ptr=inv.data_ptr(), batch=2,
+                total_query_tokens=2, num_q_heads=hq, max_blocks_per_seq=3,
+                stream_ptr=torch.cuda.current_stream().cuda_stream)
+
+        def capture():
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=torch.cuda.Stream()):
+                call()
+            return graph
+
+        def written(graph, block, row):
+            q.zero_()
+            torch.cuda.synchronize()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert bool((q[:, 0, 0] != 0).all())
+            at = int(pool.all_block_offsets_f16()[block]) * 2 + row * hkv * d * {KV_FP8: 1, KV_F32: 4}.get(dtype, 2)
+            return bool(memcpy_dtoh(pool.va_v(0), nbytes)[at:at + 64].any())
+
+        torch.cuda.synchronize()
+        graph = capture()
+        assert written(graph, mine[0], 4) and written(graph, mine[1], 8)
+        for n in range(3):
+            # the next block of the first sequence, in the place of the table that the graph reads
+            new = pool.alloc_blocks(1)[0]
+            assert pool.total_blocks() == new + 1 == 3 + n
+            offs[:new + 1] = torch.tensor(pool.all_block_offsets_f16(), device="cuda")
+            bt[0, 1], bt[1, 0] = new, new + 1
+            sl[0] = 18
+            before = memcpy_dtoh(pool.va_v(0), nbytes)
+            assert written(graph, new, 1)
+            after = memcpy_dtoh(pool.va_v(0), nbytes)
+            page = int(offs[new]) * 2
+            assert np.array_equal(before[:page], after[:page])          # (nothing else: id new + 1 is none)
+            rest = page + pool.stats()["block_bytes"]
+            assert np.array_equal(before[rest:], after[rest:])
+    finally:
+        pool.destroy()
