@@ -156,3 +156,57 @@ def test_lengths_that_differ(gpu_lib, dtype, d, lengths, order):
         assert tiles <= reads(lengths, c.totals, 16) // tile + 1 + len(lengths)
     finally:
         c.close()
+
+
+@pytest.mark.parametrize("dtype,d", SPLIT)
+@pytest.mark.parametrize("hq,hkv,bs", [(8, 2, 16), (4, 4, 8), (16, 1, 32), (14, 2, 16), (20, 2, 16)])
+def test_weights_of_two_parts(gpu_lib, dtype, d, hq, hkv, bs):
+    """As near as weights of two 16-bit parts are, not of one."""
+    import torch
+    for groups in ([[(100, 133), (100, 101), (100, 164), (100, 100)], [(37, 70)], [(0, 1)]],
+                   [[(1500, 1500 + 33 * i) for i in range(5)]]):
+        for q_scale in (1.0, 3.0):
+            c = Case(torch, gpu_lib, dtype, hq, hkv, d, bs, groups, seed=hq + d, q_scale=q_scale)
+            try:
+                c.run()
+                torch.cuda.synchronize()
+                tight(c)
+            finally:
+                c.close()
+
+
+@pytest.mark.parametrize("dtype,d", SPLIT)
+def test_a_page_that_counts(gpu_lib, dtype, d):
+    """One page's values are 64 times the others', each in turn: taken twice or not
+    at all it would change outputs by several times their size.  4 items of two
+    tiles or more a wave."""
+    import torch
+    c = Case(torch, gpu_lib, dtype, 8, 4, d, 16, [[(4100, 4100 + 21 * i) for i in range(17)]], seed=d)
+    try:
+        offs, bt = np.asarray(c.pool.all_block_offsets_f16(), np.int64) * 2, c.dev["bt"].cpu().numpy()
+        row, nbytes = 4 * d * (1 if dtype == KV_FP8 else 2), c.pool.stats()["superblock_count"] * SB
+        plain, dense = memcpy_dtoh(c.pool.va_v(0), nbytes), c.dense
+        for seq, block in [(0, 0), (0, 1), (0, 131), (0, 255), (16, 256), (16, 275), (5, 261)]:
+            last = min((block + 1) * 16, c.totals[seq])
+            values = plain.copy()
+            page = int(offs[bt[seq, block]])
+            if dtype == KV_FP8:
+                values[page + 16 * row:page + 16 * row + 16].view(np.float32)[:] *= 64
+            else:
+                n = (last - block * 16) * row
+                code = {KV_BF16: O.BF16, KV_F16: O.F16}[dtype]
+                raw = values[page:page + n].view(np.uint16)
+                raw[:] = O.encode(code, (O.decode(code, raw) * 64).astype(np.float32))
+            memcpy_htod(c.pool.va_v(0), values)
+            c.dense = []
+            for b, (k, v) in enumerate(dense):
+                if b == seq or block < 256:
+                    v = v.copy()
+                    v[block * 16:last] *= 64
+                c.dense.append([k, v])
+            c.out.fill_(float("nan"))
+            c.run()
+            torch.cuda.synchronize()
+            tight(c)
+    finally:
+        c.close()
