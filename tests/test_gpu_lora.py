@@ -261,3 +261,48 @@ def test_graph_of_many_tokens_and_columns(gpu_lib):
         c.run(gpu_lib)
         torch.cuda.synchronize()
         assert torch.equal(c.y, first)
+
+
+# a shape for each form of the expand, the last three with 32 rows a workgroup of the shrink
+FORMS = [(40, [4096, 16], 264, 16), (600, [4096, 16], 72, 16), (449, [4592, 16], 64, 64), (1100, [8192, 32], 72, 16),
+         (1100, [4112, 16, 16, 4096], 40, 32), (2049, [4096, 16], 72, 64), (700, [32, 12800], 64, 128)]
+
+
+@pytest.mark.parametrize("m,widths,k,rank", FORMS)
+@pytest.mark.parametrize("order", ["mixed", "runs"])
+@pytest.mark.parametrize("in_place", [False, True])
+def test_infinities_and_nan_in_every_form(gpu_lib, m, widths, k, rank, order, in_place):
+    """What a token or an adapter holds reaches no other, tokens side by side or in
+    runs; adapters that no token has hold NaN."""
+    import torch
+    ids = np.arange(m) % 4 - 1
+    ids = ids if order == "mixed" else np.sort(ids)
+    c = Case(torch, m, widths, k, rank, 5, ids=ids, in_place=in_place, poison=True)
+    base = c.dev["base"].clone()
+
+    def run():
+        c.y[:m * c.n] = base.reshape(-1) if in_place else 0
+        c.low.fill_(-5.0)
+        torch.cuda.synchronize()
+        c.run(gpu_lib)
+        torch.cuda.synchronize()
+        return c.get().copy()
+
+    run()
+    c.check()
+    good = c.get().copy()
+    none, first, two = (np.nonzero(ids == a)[0] for a in (-1, 0, 2))
+    bad = first[[0, len(first) // 2, -1]]
+    c.dev["x"][int(none[0]), 5] = float("nan")
+    c.dev["x"][int(none[-1])] = float("inf")
+    c.dev["x"][torch.from_numpy(bad).cuda(), 7] = float("inf")
+    c.dev["b"][2, 3, 1] = float("inf")                    # column 3 of adapter 2
+    c.dev["a"][2, rank + 1, 0] = float("nan")             # its second slice
+    got = run()
+    cut = slice(widths[0], widths[0] + widths[1])
+    same = np.ones((m, c.n), bool)
+    same[bad] = False
+    same[np.ix_(two, [3])] = same[two, cut] = False
+    assert np.array_equal(got[same], good[same])
+    assert not np.isfinite(got[bad]).any() and np.isnan(got[two, cut]).all()
+    assert not np.isfinite(got[two, 3]).any()
