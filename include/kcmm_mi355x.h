@@ -625,8 +625,8 @@ typedef struct kcmm_lora {
  *  adapter_ids: device int32 [m], in any order; a token with an id outside 0 ..
  *  adapters - 1 has no adapter, its y is its base.  Sums are fp32, y is rounded
  *  once; what one token holds, infinities and NaN too, reaches no other token,
- *  nor does what an adapter holds reach a token that has another.  y may be
- *  base.
+ *  nor does what an adapter holds reach a token that has another.  An infinity in an
+ *  adapter's B may come out as NaN.  y may be base.
  *  low_ptr: scratch memory of the caller's, 4 m slices rank bytes, for the low-rank
  *  values scales[a] x A_a^T (sums in fp32, kept to 2^-16 of each).  Calls that may run at
  *  the same time need one each.  1 <= m <= 2^20; n % 16 == 0, <= 2^22; k % 8 ==

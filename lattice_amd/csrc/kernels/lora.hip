@@ -4,12 +4,14 @@
 // of its slice.  A token without an adapter keeps base.  Two kernels: the low-rank
 // values v = scale x A^T go through memory of the caller's; y is rounded once.
 //
-// Both work on 16 tokens a block, in the order in which they come: a block's
-// tokens may have any adapters, and each of these takes its turn with all 16
-// columns of the matrix instruction, of which only its own tokens' are kept (a
-// column's values come from its own token alone, so what another token or adapter
-// holds, infinities too, goes nowhere).  Prompts have one adapter a block, decode
-// batches up to 16, whose weights are then what has to be read, once a block.
+// The first works on 16 tokens a block, in the order in which they come, and so does
+// the second for few tokens and for large prompts: a block's tokens may have any
+// adapters, and each of these takes its turn with all 16 columns of the matrix
+// instruction, of which only its own tokens' are kept (a column's values come from its own
+// token alone, so what another token or adapter holds, infinities too, goes nowhere).
+// Prompts have one adapter a block, decode batches up to 16, whose weights are then what
+// has to be read, once a block.  Hundreds of tokens go through the second product by
+// units: up to 16 tokens of one adapter out of 64.
 //  * shrink: k dealt to the waves of a workgroup by lines of 128 bytes, their sums
 //    joined in LDS, in wave order.  A workgroup has 16 or 32 rows of A and one of the
 //    block's adapters, or several in turn.  Bound by what one CU loads (64 bytes a
@@ -74,7 +76,7 @@ struct Units {
     int id;          // this lane's token's adapter
     uint64_t left;   // tokens whose adapter's turn has not come
     uint64_t ours = 0;   // those of the adapter that has it
-    int a = -1, from = 0, token = 0, count = 0;
+    int a = -1, from = 0, count = 0;
     __device__ Units(const LoraParams& p, int t0, int lane) : id(adapter_of(p, t0 + lane)) {
         left = __ballot(id >= 0);
     }
@@ -319,8 +321,9 @@ __global__ __launch_bounds__(256) void lora_expand_few(LoraParams p) {
     *reinterpret_cast<u32x2*>(p.y + at) = out;
 }
 
-// Decode batches of mixed adapters: a wave has 16 columns and the units of 64 tokens, so
-// that an adapter's weights are loaded once for its tokens among these.
+// Hundreds of tokens: a wave has 16 columns and the units of 64 tokens, one after the
+// other, each with a load of its adapter's weights: mixed adapters load them for 16 of their
+// tokens at a time, not for each block of 16 tokens that holds one.
 template <int STEPS>
 __global__ __launch_bounds__(256) void lora_expand_units(LoraParams p) {
     const int lane = threadIdx.x & 63, ln = lane & 15, lg = lane >> 4;
@@ -490,16 +493,21 @@ void launch_expand(LoraParams& p, hipStream_t s) {
 
 template <int NB, int STEPS>
 void launch_expand_any(LoraParams& p, hipStream_t s) {
-    // Runs of blocks pay once base and y are large: few and many, the whole call, 2048
-    // tokens in runs of an adapter: n 4096 20.0 and 18.9 us, n 6144 64.6 and 51.1; 1024
-    // tokens, n 6144 40.2 and 40.3.  (Where the adapters of 2048 tokens are mixed, weights
-    // are loaded anew for each block: n 4096 33.3 and 47.5.)
+    // Runs of blocks pay once base and y are large.  Units and this, the whole call, k 4096,
+    // tokens in runs of 8 adapters, ranks 16 / 64: 1024 tokens, n 6144 21.5 and 21.6 us /
+    // 40.4 and 41.6; from 2048 tokens, n 4096 20.5 and 19.8 / 42.3 and 33.2 on, to 4096
+    // tokens, n 28672 240 and 102 / 430 and 145.  (Where adapters are mixed, weights are
+    // loaded anew for each block: 2048 tokens, n 4096 32.4 and 48.9 / 82.9 and 149.  Ids
+    // lie on the device, so no rule can tell.)
     const long long blocks = (p.m + 15) / 16;
     if (blocks * ((p.n + 63) / 64) >= 8192) return launch_expand<NB, STEPS>(p, s);
     const int chunks = deal_columns(p, 16);
-    // Units where there are waves enough without the latencies that the other form hides:
-    // hundreds of tokens of mixed adapters 42.7 -> 27 us; 64 tokens of 16 adapters, n 6144
-    // (384 waves), would take 17 for 12.
+    // Units where there are waves enough without the latencies that the other form hides.
+    // Few and units, as above, mixed: 512 tokens, n 4096 13.3 and 14.0 us / 45.2 and 28.5,
+    // 1024 20.5 and 19.0 / 81.1 and 48.4; in runs of an adapter 10.0 and 10.7 / 16.9 and 17.0,
+    // 14.9 and 14.1 / 26.1 and 25.8.  With fewer waves, 256 tokens, n 4096: mixed 10.8 and 12.6
+    // / 26.8 and 19.4, runs 8.9 and 10.3 / 12.5 and 13.7; 64 tokens of 16 adapters, n 6144 12
+    // and 17.
     const long long tiles = (p.m + 63) / 64;
     if (chunks * tiles >= 2048) {
         hipLaunchKernelGGL((lora_expand_units<STEPS>), dim3((chunks + 3) / 4, static_cast<unsigned>(tiles)), dim3(256), 0,
