@@ -229,7 +229,7 @@ struct FastParams {
     SharedParams p;
     int row0, rows;            // sequences of this launch
     int group, seqs;           // query heads a kv head; sequences of an item
-    int slices, least;         // waves; least tiles of one
+    int slices;                // waves
     int* per;                  // tiles of a slice, of all, and common ones a kv head: for the joining kernel
     RowPlan* plan;
     // first parts of (sequence, head): of the common tokens, then of the rest;
@@ -357,10 +357,9 @@ __device__ __forceinline__ void find_items(const FastParams& f, Items& it) {
     __syncthreads();
 }
 
-// Tiles of a slice: equal parts of all, but none so short that joining the parts
-// costs more than the shorter slices save.
+// Tiles of a slice: equal parts of all.
 __device__ __forceinline__ int slice_tiles(int total, const FastParams& f) {
-    return max((total + f.slices - 1) / f.slices, f.least);
+    return max((total + f.slices - 1) / f.slices, 1);
 }
 
 // LDS accesses of the streaming loop, at byte addresses and constant offsets, each
@@ -1103,7 +1102,6 @@ bool launch_fast(const SharedParams& p, uint64_t scratch, hipStream_t s, std::st
     f.seqs = 16 * NCB / f.group;
     f.scale_log2 = p.scale * 1.4426950408889634f;
     f.slices = kSlices;
-    f.least = 1;
     const long long cap = static_cast<long long>(p.mbps) * p.block_size;
     for (int row0 = 0; row0 < p.batch; row0 += kMaxRows) {
         f.row0 = row0;
