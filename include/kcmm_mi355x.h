@@ -167,8 +167,8 @@ int kcmm_paged_attn_decode_f32_on_stream(
 /**
  * Decode attention (tensor contract of kcmm_paged_attn_decode_f16, ref
  * kcmm.h:505; page types and q/out types as kcmm_paged_attn_prefill_on_stream)
- * for a batch whose sequences share prefixes in groups, each prefix read and
- * multiplied once for its group.  No counterpart in the reference, whose
+ * for a batch whose sequences share prefixes in groups, a prefix read once for
+ * several of its sequences.  No counterpart in the reference, whose
  * sharing manager is a placeholder (ref sharing.rs:24-65); the groups are what
  * kcmm_share_prefix, kcmm_prefix_attach and kcmm_fork_beams_on_stream make.
  *
@@ -181,6 +181,16 @@ int kcmm_paged_attn_decode_f32_on_stream(
  * shared length ends in is read through b's own table, as copy-on-write and
  * forks leave it.  A sequence in no group shares nothing, whatever its
  * shared_lens.  Sequences with seq_lens <= 0 give zeros.
+ *
+ * What is read once: with head_dim 64 or 128 (fp8 pages: 128), at most 16 query heads a
+ * kv head, a block_size that 8 divides and 16-bit or fp8 pages, up to 32 query rows a kv
+ * head (head_dim 64: 64; groups of few rows: 16), which are that many sequences of a
+ * group times their heads, take their common tokens together; a group of more does so
+ * several times.  Common is one length: where shared lengths differ, the one that saves
+ * most reads; what a sequence shares beyond it, or all if it shares less, it reads by
+ * itself.  Every other shape reads all of every sequence by itself, 1.2 to 3.6 times as
+ * long as kcmm_paged_attn_decode_*_on_stream: use that where the tables of all sequences
+ * hold their shared blocks.
  *
  * scratch_ptr: device memory of the caller's, aligned to 256 bytes, of
  * scratch_bytes >= kcmm_paged_attn_shared_scratch_bytes; its contents on entry do
