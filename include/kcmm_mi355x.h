@@ -186,8 +186,8 @@ int kcmm_paged_attn_decode_f32_on_stream(
  * kv head, a block_size that 8 divides and 16-bit or fp8 pages, up to 32 query rows a kv
  * head (head_dim 64: 64; groups of few rows: 16), which are that many sequences of a
  * group times their heads, take their common tokens together; a group of more does so
- * several times.  Common is one length: where shared lengths differ, the one that saves
- * most reads; what a sequence shares beyond it, or all if it shares less, it reads by
+ * several times.  Common is one length: the least, or where shared lengths differ by
+ * more than an eighth, the one that saves most reads; what a sequence shares beyond it, or all if it shares less, it reads by
  * itself.  Every other shape reads all of every sequence by itself, 1.2 to 3.6 times as
  * long as kcmm_paged_attn_decode_*_on_stream: use that where the tables of all sequences
  * hold their shared blocks.

@@ -13,8 +13,8 @@
 //    the matrix products are (sequence of the item, query head) pairs, so a K/V byte
 //    serves up to 64 query rows, as one of a single sequence serves G (query heads a
 //    kv head).  No column of an item is masked: where its sequences share different
-//    lengths, the cut that saves most reads is taken, and those that share less than that
-//    are left to read their tokens by themselves.
+//    lengths, the cut that saves most reads (or the least length, where that is near) is
+//    taken, and those that share less are left to read their tokens by themselves.
 //  * The work is the list of 8 KiB tiles (16 or 32 tokens) of all (item, kv head),
 //    common tokens first; every wave takes an equal, contiguous slice of it.  Two
 //    tiles a wave, one on its way, by direct loads into LDS, and two waves a SIMD: one
@@ -322,10 +322,10 @@ __device__ __forceinline__ void find_items(const FastParams& f, Items& it) {
     __syncthreads();
     // The common tokens: of the lengths that the item's sequences share, the c with the most
     // (k - 1) c saved, k of them sharing c or more (both in units of 8 tokens, below 2^34
-    // and 2^28); the others read all of theirs by themselves.  Where all share the same
-    // there is nothing to choose.
-    const int count = in ? it.count[first] : 0, most = in ? it.most[first] : 0;
-    const bool unequal = in && it.least[first] < most;
+    // and 2^28); the others read all of theirs by themselves.  Where all share nearly the
+    // same it is the least: the search takes 1 to 2 us, and could save an eighth at most.
+    const int count = in ? it.count[first] : 0, least = in ? it.least[first] : 0;
+    const bool unequal = in && 8ll * least < 7ll * it.most[first];
     if (unequal && shared > 0) {
         int others = -1;
         for (int i = 0; i < count; ++i) others += it.shared[first + i] >= shared;
@@ -334,7 +334,7 @@ __device__ __forceinline__ void find_items(const FastParams& f, Items& it) {
     }
     __syncthreads();
     // (of one sequence alone there is nothing to gain)
-    const int cut = unequal ? static_cast<int>(it.best[first] & 0xfffffff) * 8 : count > 1 ? most : 0;
+    const int cut = unequal ? static_cast<int>(it.best[first] & 0xfffffff) * 8 : count > 1 ? least : 0;
     const int common = cut > 0 && shared >= cut ? cut : 0;
     const bool begins = in && first == r && cut > 0;
     const int pre = begins ? tiles_of(cut, TILE) : 0, own = tiles_of(len - common, TILE);
