@@ -187,14 +187,14 @@ int kcmm_paged_attn_decode_f32_on_stream(
  * head (head_dim 64: 64; groups of few rows: 16), which are that many sequences of a
  * group times their heads, take their common tokens together; a group of more does so
  * several times.  Common is one length: the least, or where shared lengths differ by
- * more than an eighth, the one that saves most reads; what a sequence shares beyond it, or all if it shares less, it reads by
- * itself.  Every other shape reads all of every sequence by itself, 1.2 to 3.6 times as
- * long as kcmm_paged_attn_decode_*_on_stream: use that where the tables of all sequences
- * hold their shared blocks.
+ * more than an eighth, the one that saves most reads; what a sequence shares beyond it,
+ * or all if it shares less, it reads by itself.  Every other shape reads all of every
+ * sequence by itself, 1.2 to 3.6 times as long as kcmm_paged_attn_decode_*_on_stream: use
+ * that where the tables of all sequences hold their shared blocks.
  *
  * scratch_ptr: device memory of the caller's, aligned to 256 bytes, of
- * scratch_bytes >= kcmm_paged_attn_shared_scratch_bytes; its contents on entry do
- * not matter.  Calls that may run at the same time need scratch of their own.
+ * scratch_bytes >= kcmm_paged_attn_shared_scratch_bytes, apart from all other buffers; its
+ * contents on entry do not matter.  out may be q, or is apart from it.  Calls that may run at the same time need scratch of their own.
  * Nothing is allocated and no state is kept: a call may be captured into a HIP
  * graph at once, and the graph reads and writes the buffers it was given.  An
  * infinity in V that a sequence reads may come out as NaN.

@@ -685,6 +685,15 @@ int kcmm_paged_attn_prefill_on_stream(kcmm_pool_t* pool, uint32_t layer_idx, uin
 
 extern "C++" {
 namespace {
+// A buffer of a call; address 0: not there.
+struct Span {
+    uint64_t at, bytes;
+};
+bool apart(const Span& a, const Span& b) {
+    return a.at == 0 || b.at == 0 || a.at + a.bytes <= b.at || b.at + b.bytes <= a.at;
+}
+bool same_or_apart(const Span& a, const Span& b) { return a.at == b.at || apart(a, b); }
+
 // Shapes that the shared-prefix attention takes (kv geometry: the pool's).
 bool shared_shapes_ok(kcmm_pool_t* pool, const char* fn, uint32_t batch, uint32_t hq, uint32_t mbps) {
     const kcmm::PoolGeometry& g = pool->core->geo();
@@ -753,6 +762,14 @@ int kcmm_paged_attn_decode_shared_on_stream(kcmm_pool_t* pool, uint32_t layer_id
     }
     if (q % 16 != 0 || out % 16 != 0) {
         pool->set_error(std::string(fn) + ": q and out must be aligned to 16 bytes");
+        return -1;
+    }
+    const uint64_t rows = static_cast<uint64_t>(batch) * hq * d * (g.dtype == kcmm::kF32 ? 4 : 2);
+    const Span work{scratch, need}, in{q, rows}, result{out, rows};
+    if (!apart(work, in) || !apart(work, result) || !apart(work, {bt, 4ull * batch * mbps}) ||
+        !apart(work, {sl, 4ull * batch}) || !apart(work, {shared_lens, 4ull * batch}) ||
+        !apart(work, {group_starts, 4ull * num_groups + 4}) || !same_or_apart(in, result)) {
+        pool->set_error(std::string(fn) + ": scratch overlaps another buffer, or out a part of q");
         return -1;
     }
     std::string err;
@@ -1338,14 +1355,6 @@ int kcmm_silu_mul_bf16_on_stream(uint64_t gate_up, uint64_t act, uint32_t rows,
 extern "C++" {
 namespace {
 
-// A buffer of a call; address 0: not there.
-struct Span {
-    uint64_t at, bytes;
-};
-bool apart(const Span& a, const Span& b) {
-    return a.at == 0 || b.at == 0 || a.at + a.bytes <= b.at || b.at + b.bytes <= a.at;
-}
-bool same_or_apart(const Span& a, const Span& b) { return a.at == b.at || apart(a, b); }
 bool aligned(uint64_t to, std::initializer_list<uint64_t> ptrs) {
     for (uint64_t p : ptrs)
         if (p % to != 0) return false;

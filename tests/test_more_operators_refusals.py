@@ -145,3 +145,18 @@ def test_shared_attention_of_tables_near_2_to_31(hostcheck_lib):
         with pytest.raises(KcmmError, match="2\\^31"):
             pool.shared_scratch_bytes(1, 1, 49981)
         assert pool.shared_scratch_bytes(1, 1, 49980) > 0
+
+
+@pytest.mark.parametrize("change,why", [
+    (dict(out_ptr=at(0)), "no device"), (dict(out_ptr=at(0) + 2048), "overlaps"),
+    (dict(scratch_ptr=at(0)), "overlaps"), (dict(scratch_ptr=at(1)), "overlaps"),
+    (dict(out_ptr=at(7) + 2048), "overlaps"), (dict(query_ptr=at(7) - 16), "overlaps"),
+    (dict(query_ptr=at(7) - 4096), "no device"), (dict(block_tables_ptr=at(7) - 64), "overlaps"),
+    (dict(block_tables_ptr=at(7) - 128), "no device"), (dict(seq_lens_ptr=at(7) + 4), "overlaps"),
+    (dict(shared_lens_ptr=at(7) - 12), "overlaps"), (dict(group_starts_ptr=at(7) - 8), "overlaps"),
+    (dict(group_starts_ptr=at(7) - 12), "no device"),
+])
+def test_shared_attention_buffers(hostcheck_lib, change, why):
+    with pool_of(hostcheck_lib) as pool:
+        with pytest.raises(KcmmError, match=why):
+            pool.paged_attn_decode_shared(**{**SHARED, **change})
