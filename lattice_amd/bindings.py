@@ -711,7 +711,10 @@ class KcmmPool:
         pos = None
         if positions_ptr:
             pos = KcmmRopePositions(positions_ptr, num_axes)
-            for i, a in enumerate(pair_axes or ()):
+            axes = list(pair_axes or ())
+            if len(axes) > 128 or not all(0 <= a <= 255 for a in axes):
+                raise KcmmError("rope_append_chunk: pair_axes must be at most 128 axis numbers")
+            for i, a in enumerate(axes):
                 pos.axis_of_pair[i] = a
         rc = self.lib.kcmm_rope_append_chunk_on_stream(
             self.handle, layer_idx, qkv_ptr, q_out_ptr, block_tables_ptr, seq_lens_ptr,

@@ -160,3 +160,11 @@ def test_shared_attention_buffers(hostcheck_lib, change, why):
     with pool_of(hostcheck_lib) as pool:
         with pytest.raises(KcmmError, match=why):
             pool.paged_attn_decode_shared(**{**SHARED, **change})
+
+
+@pytest.mark.parametrize("axes", [[256] * 32, [0] * 31 + [-256], [0] * 129, [1 << 32]])
+def test_axes_that_are_no_bytes(hostcheck_lib, axes):
+    """They would wrap round to an axis that is there."""
+    with pool_of(hostcheck_lib) as pool:
+        with pytest.raises(KcmmError, match="pair_axes"):
+            pool.rope_append_chunk(**CHUNK, positions_ptr=at(8), num_axes=2, pair_axes=axes)
