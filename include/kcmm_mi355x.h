@@ -638,7 +638,7 @@ typedef struct kcmm_lora {
  *  nor does what an adapter holds reach a token that has another.  An infinity in an
  *  adapter's B may come out as NaN.  y may be base.
  *  low_ptr: scratch memory of the caller's, 4 m slices rank bytes, for the low-rank
- *  values scales[a] x A_a^T (sums in fp32, kept to 2^-16 of each).  Calls that may run at
+ *  values scales[a] x A_a^T (sums in fp32, kept to 2^-16 of each, or 2^-134).  Calls that may run at
  *  the same time need one each.  1 <= m <= 2^20; n % 16 == 0, <= 2^22; k % 8 ==
  *  0, <= 2^20; rank % 8 == 0, <= 128; adapters <= 65535.  x, a, b, low, base and y
  *  aligned to 16 bytes; y (unless it is base) and low overlap nothing else.

@@ -215,9 +215,11 @@ __global__ __launch_bounds__(512) void lora_shrink(LoraParams p, int turns) {
             float part[8];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                // (a value that bf16 takes for an infinity leaves nothing)
+                // (the last fp32 values would round to an infinity: the largest bf16 instead, so
+                // that they too leave what the second part holds; an infinity leaves nothing)
+                constexpr float kMost = 3.38953139e38f;
                 v[e] *= scale;
-                part[e] = bf16_round_hw(v[e]);
+                part[e] = fabsf(v[e]) < INFINITY ? bf16_round_hw(fminf(fmaxf(v[e], -kMost), kMost)) : v[e];
                 part[4 + e] = fabsf(part[e]) < INFINITY ? v[e] - part[e] : 0.0f;
             }
             // rows 4 lg .. +3 of each 16, of column ln: half a piece

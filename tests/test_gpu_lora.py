@@ -306,3 +306,35 @@ def test_infinities_and_nan_in_every_form(gpu_lib, m, widths, k, rank, order, in
     assert np.array_equal(got[same], good[same])
     assert not np.isfinite(got[bad]).any() and np.isnan(got[two, cut]).all()
     assert not np.isfinite(got[two, 3]).any()
+
+
+@pytest.mark.parametrize("m,n", [(5, 16), (600, 4112), (1100, 8224)])
+@pytest.mark.parametrize("scale,b", [(1.7e38, 2.0 ** -10), (1.7075e38, 2.0 ** -10), (-1.7075e38, 2.0 ** -10),
+                                     (2.0 ** -100, 1.0), (2.0 ** -126, 2.0 ** 30), (2.0 ** -133, 2.0 ** 30)])
+def test_values_at_the_ends_of_the_range(gpu_lib, m, n, scale, b):
+    """Low-rank values up to the last that fp32 holds, where bf16 has none left, and
+    down to its least: two parts keep 2^-16 of each, or 2^-134 (half of bf16's
+    smallest step)."""
+    import torch
+    k = rank = 8
+    rng = np.random.default_rng(m)
+    x, a, w = np.zeros((m, k), np.float32), np.zeros((1, rank, k), np.float32), np.zeros((1, n, rank), np.float32)
+    x[:, 0], a[0, 0, 0] = E.bf16(rng.uniform(1.0, 1.9922, m).astype(np.float32)), 1.0
+    x[0, 0] = 1.9921875                     # 255 / 128: times 1.7075e38 above the largest bf16
+    w[0, :, 0] = b
+    y = torch.empty(m, n, dtype=torch.bfloat16, device="cuda")
+    base, low = torch.zeros_like(y), torch.empty(m * rank, device="cuda")
+    dev = [dev16(torch, v) for v in (x, a, w)]
+    ids, s = torch.zeros(m, dtype=torch.int32, device="cuda"), torch.tensor([scale], dtype=torch.float32, device="cuda")
+    torch.cuda.synchronize()
+    gpu_lib.lora_add_bf16(dev[0].data_ptr(), dev[1].data_ptr(), dev[2].data_ptr(), ids.data_ptr(), low.data_ptr(),
+                          base.data_ptr(), y.data_ptr(), m, n, k, adapters=1, rank=rank, scales_ptr=s.data_ptr())
+    torch.cuda.synchronize()
+    v = x[:, 0].astype(np.float64) * float(s[0])
+    assert np.abs(v).max() < 2.0 ** 128
+    want = (v * b)[:, None]
+    # the parts, the product's fp32 result, the store (its own smallest step with it)
+    tol = (2.0 ** -16 * np.abs(v) + 2.0 ** -134)[:, None] * b + (2.0 ** -23 + E.BF16_HALF) * np.abs(want) * (1 + 2.0 ** -8) + \
+        2.0 ** -134
+    off = np.abs(y.double().cpu().numpy() - want)
+    assert np.all(off <= tol), float(np.max(off / tol))
